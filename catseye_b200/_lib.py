@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libcatsgpu.so")
 HEADER = os.path.join(os.path.dirname(HERE), "include", "catsgpu.h")
 
 _vp, _fp, _ip = C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)
-_i, _u64, _f, _ch, _sz = C.c_int, C.c_ulonglong, C.c_float, C.c_char, C.c_size_t
+_i, _ll, _u64, _f, _ch, _sz = C.c_int, C.c_longlong, C.c_ulonglong, C.c_float, C.c_char, C.c_size_t
 
 
 class LlmConfigC(C.Structure):
@@ -20,14 +20,21 @@ class LlmConfigC(C.Structure):
                                        "seq_len", "wtype", "tp_rank", "tp_size")]
 
 
+class KvC(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("table", C.c_void_p)] + [
+        (n, C.c_int) for n in ("n_pages", "n_layers", "n_kv_heads", "head_size", "n_seqs", "max_pages")]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "cats_gpu_init": (_i, [_i]),
     "cats_gpu_term": (None, []),
+    "cats_gpu_device": (_i, []),
     "cats_gpu_last_error": (_i, []),
     "cats_gpu_clear_error": (None, []),
     "cats_gpu_error_string": (C.c_char_p, [_i]),
     "cats_gpu_device_error": (_i, []),
+    "cats_gpu_clear_device_error": (None, []),
     "cats_gpu_register_weight": (_i, [_vp, _i, _i, _i]),
     "cats_gpu_unregister_weight": (None, [_vp]),
     "cats_gpu_weight_device_bytes": (_sz, [_vp]),
@@ -81,6 +88,21 @@ SIGNATURES = {
     "cats_gpu_llm_weight_bytes": (_sz, [_vp]),
     "cats_gpu_llm_time_matvec": (_i, [_vp, _i, _i, C.POINTER(C.c_float), C.POINTER(C.c_double)]),
     "cats_gpu_synth_tensor": (_i, [_vp, _i, _i, _i, _u64, _i, _f, _f]),
+    "cats_gpu_kv_page_bytes": (_sz, [_i, _i, _i]),
+    "cats_gpu_kv_append_dev": (_i, [_vp, _i, _vp, _vp, _i, _ll, _ll, _i, _vp, _i, _i, _vp]),
+    "cats_gpu_kv_read_dev": (_i, [_vp, _i, _vp, _vp, _i, _ll, _ll, _i, _vp, _i, _i, _vp]),
+    "cats_gpu_kv_attention_dev": (_i, [_vp, _i, _vp, _vp, _i, _i, _ll, _ll, _i, _vp, _i, _i, _i, _vp]),
+    "cats_gpu_kv_copy_pages_dev": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "cats_gpu_kv_pages_create": (_vp, [_i, _i, _i]),
+    "cats_gpu_kv_pages_destroy": (None, [_vp]),
+    "cats_gpu_kv_pages_write": (_i, [_vp, _i, _i, _i, _vp, _vp, _ip]),
+    "cats_gpu_kv_pages_fork": (_i, [_vp, _i, _i, _i]),
+    "cats_gpu_kv_pages_truncate": (_i, [_vp, _i, _i]),
+    "cats_gpu_kv_pages_compact": (_i, [_vp, _vp, _vp, _ip]),
+    "cats_gpu_kv_pages_length": (_i, [_vp, _i]),
+    "cats_gpu_kv_pages_free": (_i, [_vp]),
+    "cats_gpu_kv_pages_table": (_vp, [_vp]),
+    "cats_gpu_logprobs_dev": (_i, [_vp, _i, _i, _i, _ll, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "cats_sgemm": (None, [_ch, _ch, _i, _i, _i, _f, _vp, _vp, _f, _vp]),
     "cats_gemm_rnn": (None, [_i, _i, _i, _f, _vp, _vp, _f, _vp]),
     "cats_gemm_rnt": (None, [_i, _i, _i, _f, _vp, _vp, _f, _vp]),
@@ -160,4 +182,15 @@ def call_void(fn, *args, what=None):
 def init(device=-1):
     lib = load()
     check(lib.cats_gpu_init(device), "cats_gpu_init")
+    return lib
+
+
+def check_device(device):
+    """Raise unless a tensor's CUDA device is the one the library runs on."""
+    lib = load()
+    mine = lib.cats_gpu_device()
+    if mine < 0:
+        mine = init().cats_gpu_device()
+    if device.index != mine:
+        raise CatsGpuError(f"the tensors are on {device}, the library on cuda:{mine}")
     return lib

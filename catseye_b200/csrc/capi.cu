@@ -196,6 +196,12 @@ int capi_fail(int code, const char *what) { return fail(code, what); }
 int noalloc_device_error(bool clear);   // noalloc.cu: the no-allocation sgemm's status word
 // the library's stream (after cats_gpu_init), for entry points in other files
 cudaStream_t capi_stream() { return g.stream; }
+// initialised (CATS_OK), the asynchronous operators' error word, a CUDA status recorded, and
+// the library's device: entry points in other files
+int capi_ready() { return ensure_init() ? CATS_OK : g.last_err; }
+int *capi_err_word() { return g.d_err ? g.d_err + 1 : nullptr; }
+int capi_check(cudaError_t e, const char *what) { return check(e, what); }
+int capi_device() { return g.device; }
 }
 
 // ===================================================================== C ABI
@@ -223,8 +229,9 @@ int cats_gpu_init(int device)
     // its later work there.  A non-blocking stream let a product start before
     // the kernels writing its operands had finished.
     if (check(cudaStreamCreateWithFlags(&g.stream, cudaStreamDefault), "cats_gpu_init")) return g.last_err;
-    if (check(cudaMalloc(&g.d_err, 4), "cats_gpu_init")) return g.last_err;
-    cudaMemset(g.d_err, 0, 4);
+    // [0] bounded waits that gave up, [1] what the asynchronous operators (kv_capi.cu) left out
+    if (check(cudaMalloc(&g.d_err, 8), "cats_gpu_init")) return g.last_err;
+    cudaMemset(g.d_err, 0, 8);
     g.device = device;
     g.init = true;
     return CATS_OK;
@@ -249,6 +256,7 @@ void cats_gpu_term(void)
     g.init = false;
 }
 
+int cats_gpu_device(void) { return g.init ? g.device : -1; }
 int cats_gpu_last_error(void) { return g.last_err; }
 void cats_gpu_clear_error(void)
 {
@@ -259,9 +267,15 @@ const char *cats_gpu_error_string(int code) { return err_name(code); }
 
 int cats_gpu_device_error(void)
 {
-    int h = 0;
-    if (g.init) cudaMemcpy(&h, g.d_err, 4, cudaMemcpyDeviceToHost);
-    return h | cats::noalloc_device_error(false);
+    int h[2] = {0, 0};
+    if (g.init) cudaMemcpy(h, g.d_err, 8, cudaMemcpyDeviceToHost);
+    return h[0] | h[1] | cats::noalloc_device_error(false);
+}
+
+void cats_gpu_clear_device_error(void)
+{
+    if (g.init) cudaMemset(g.d_err, 0, 8);
+    cats::noalloc_device_error(true);
 }
 
 int cats_gpu_register_weight(const void *w, int type, int n, int d)

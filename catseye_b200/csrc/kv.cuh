@@ -1,0 +1,165 @@
+// kv.cuh — the paged KV cache held in Q4_0 blocks: its layout, the block
+// quantizer, and the launchers that the C API (kv.cu) and the batched step
+// (batch.cu) share.
+//
+// A page holds CATS_KV_PAGE = 64 tokens of every layer and kv head:
+//   pool[page][layer][kv head][chunk], chunk = 72 * head_size bytes.
+// A chunk, for HB = head_size / 32 blocks per row:
+//   K codes   [64 tokens][c 0..3][HB][4 B]   byte i: elements 8c + 2i (low
+//             nibble) and 8c + 2i + 1 of block b
+//   V codes   [32 token pairs][g 0..7][HB][2 tokens][2 B]   nibble n: element
+//             4g + n of block b
+//   K scales  [64 tokens][HB] fp16
+//   V scales  [32 token pairs][HB][2 tokens] fp16
+// The order is that of the tensor cores' fragments (m16n8k16): lane (g, c) of
+// a warp finds the codes of token g it feeds to q k^T in one 4*HB-byte load,
+// and those of token pair c it feeds to p v in another, each load of a warp
+// covering whole consecutive 128-byte lines.
+//
+// A value is d * (code - 8).  d keeps 8 significant bits (a bf16 rounding of
+// -m / 8, m the block's value of largest magnitude, held as fp16), so that
+// the product with a code of at most 3 magnitude bits is exact in fp16: what
+// the tensor cores multiply is the cache's value itself, not a rounding of it.
+#pragma once
+#include "common.cuh"
+#include <cuda_bf16.h>
+
+namespace cats {
+
+constexpr int KV_PAGE = 64;
+constexpr int KV_MAX_HS = 128;
+
+// element types of rows given to the cache's operators (ggml's numbers)
+enum KvType : int { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 30 };
+
+#define CATS_DEVERR_PAGE_RANGE 0x40   // a run named a row, sequence, position or page outside its range; it was left out
+
+// One layer of a cache as the kernels see it.
+struct KvView {
+    uint8_t *pool;           // + the layer's offset
+    const int *table;        // [n_seqs][max_pages] page numbers, -1 = none
+    size_t page_bytes;
+    int n_pages, n_kv, hs, n_seqs, max_pages;
+    int *err;
+
+    __device__ __forceinline__ uint8_t *chunk(int page, int head) const
+    {
+        return pool + (size_t)page * page_bytes + (size_t)head * (72 * hs);
+    }
+    // the page of (sequence, page index), -1 (recorded) when there is none
+    __device__ __forceinline__ int page(int seq, int idx) const
+    {
+        int p = -1;
+        if (seq >= 0 && seq < n_seqs && idx >= 0 && idx < max_pages) p = __ldg(table + (size_t)seq * max_pages + idx);
+        if (p >= 0 && p < n_pages) return p;
+        if (err) atomicOr(err, CATS_DEVERR_PAGE_RANGE);
+        return -1;
+    }
+};
+
+// rows first .. first + n - 1 of a batch are positions pos .. of a sequence
+struct KvRun {
+    int first, n, seq, pos;
+};
+
+// The rows r0 <= r < r1 of a run that lie in a tensor of `rows` rows; a run
+// that names others is recorded (so a length of any size ends the loop).
+__device__ __forceinline__ int2 kv_run_rows(const KvRun &run, int rows, int *err)
+{
+    if (run.n <= 0) return make_int2(0, 0);
+    const long long r0 = run.first < 0 ? -(long long)run.first : 0, r1 = min((long long)run.n, (long long)rows - run.first);
+    if ((r0 > 0 || r1 < run.n) && err) atomicOr(err, CATS_DEVERR_PAGE_RANGE);
+    return r0 < r1 ? make_int2((int)r0, (int)r1) : make_int2(0, 0);
+}
+
+// byte offsets inside a chunk
+__host__ __device__ constexpr int kv_v_codes(int hs) { return 32 * hs; }
+__host__ __device__ constexpr int kv_k_scales(int hs) { return 64 * hs; }
+__host__ __device__ constexpr int kv_v_scales(int hs) { return 68 * hs; }
+
+// four elements 4*e4 .. 4*e4+3 of a head's row (block b = e4 / 8, g = e4 % 8):
+// the two bytes of their codes, K or V
+__device__ __forceinline__ int kv_code_off(bool is_v, int hs, int slot, int e4)
+{
+    const int hb = hs >> 5, b = e4 >> 3, g = e4 & 7;
+    return is_v ? 32 * hs + (((slot >> 1) * 8 + g) * hb + b) * 4 + 2 * (slot & 1)
+                : (slot * 4 + (g >> 1)) * 4 * hb + 4 * b + 2 * (g & 1);
+}
+__device__ __forceinline__ int kv_scale_off(bool is_v, int hs, int slot, int b)
+{
+    const int hb = hs >> 5;
+    return is_v ? 68 * hs + (((slot >> 1) * hb + b) * 2 + (slot & 1)) * 2 : 64 * hs + (slot * hb + b) * 2;
+}
+
+// Quantize a block of 32 held four elements a lane by eight consecutive lanes
+// (mask: those lanes), and store it at (chunk, slot).  The code is floor(x/d +
+// 1/2) + 8, decided exactly: (q +- 1/2) * d has at most 13 significant bits,
+// so comparing x with it in fp32 settles what the approximate quotient
+// cannot.  A block with a NaN or an infinity reads back as NaN.
+__device__ __forceinline__ void kv_store4(uint8_t *chunk, bool is_v, int hs, int slot, int e4, const float (&x)[4],
+                                          unsigned mask)
+{
+    float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+    // NaN and infinity: x - x is 0 for every finite x
+    const float z = (x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]);
+    const bool bad = __any_sync(mask, !(z == 0.f)) != 0;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
+        lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
+    }
+    const float m = hi >= -lo ? hi : lo;
+    float d = __bfloat162float(__float2bfloat16_rn(m * -0.125f));
+    const __half dh = __float2half_rn(fminf(fmaxf(d, -8160.f), 8160.f));
+    d = __half2float(dh);
+    unsigned codes = 0x8888u;
+    if (!bad && d != 0.f) {
+        const float da = fabsf(d), inv = 1.f / da;
+        codes = 0u;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float xs = d < 0.f ? -x[j] : x[j];
+            float q = floorf(fminf(fmaxf(xs * inv, -8.f), 7.f) + 0.5f);
+            if (xs >= (q + 0.5f) * da) q += 1.f;
+            else if (xs < (q - 0.5f) * da) q -= 1.f;
+            const int code = (int)fminf(fmaxf(q, -8.f), 7.f) + 8;
+            codes |= (unsigned)code << (4 * j);
+        }
+    }
+    *reinterpret_cast<uint16_t *>(chunk + kv_code_off(is_v, hs, slot, e4)) = (uint16_t)codes;
+    if ((e4 & 7) == 0)
+        *reinterpret_cast<__half *>(chunk + kv_scale_off(is_v, hs, slot, e4 >> 3)) = bad ? __ushort_as_half(0x7fff) : dh;
+}
+
+// four elements 4*e4 .. of a stored row
+__device__ __forceinline__ float4 kv_load4(const uint8_t *chunk, bool is_v, int hs, int slot, int e4)
+{
+    const unsigned c = *reinterpret_cast<const uint16_t *>(chunk + kv_code_off(is_v, hs, slot, e4));
+    const float d = __half2float(*reinterpret_cast<const __half *>(chunk + kv_scale_off(is_v, hs, slot, e4 >> 3)));
+    return make_float4(d * (float)((int)(c & 15) - 8), d * (float)((int)(c >> 4 & 15) - 8),
+                       d * (float)((int)(c >> 8 & 15) - 8), d * (float)((int)(c >> 12 & 15) - 8));
+}
+
+// Rows of attention or of a cache's tensors: `rows` of them, ld elements apart.
+struct KvRows {
+    void *p;
+    long long ld;
+    int rows;
+    int vec;   // 1: every group of four elements is aligned to its own size
+};
+
+struct KvBatch {
+    const KvRun *runs;
+    int n_runs, max_rows, max_len;
+};
+
+cudaError_t launch_kv_append(const KvView &c, int type, const KvRows &k, const KvRows &v, const KvBatch &b,
+                             cudaStream_t st);
+cudaError_t launch_kv_read(const KvView &c, int type, const KvRows &k, const KvRows &v, const KvBatch &b,
+                           cudaStream_t st);
+cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, const KvRows &q, int n_heads,
+                                const KvBatch &b, cudaStream_t st);
+// pages dst[i] = src[i] (host lists; no page is both copied to and copied from, or copied to twice)
+cudaError_t launch_kv_copy(uint8_t *pool, size_t page_bytes, const int *src, const int *dst, int n, cudaStream_t st);
+
+} // namespace cats

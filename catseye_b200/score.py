@@ -1,0 +1,37 @@
+"""Log probabilities of given tokens over libcatsgpu (cats_gpu_logprobs_dev)."""
+from . import _lib
+from .kv import _type
+
+MAX_K = 32
+
+
+def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
+    """Of the rows of logits [rows, vocab] (CUDA; float32, float16 or bfloat16;
+    rows may be a wider tensor's): (log softmax at targets [rows] or None,
+    entropy [rows] or None, ids of the k <= 32 likeliest [rows, k], their log
+    probabilities [rows, k]).  A negative target gives 0; of equal logits the
+    lower id comes first.  stream: a cudaStream_t, or None for the library's."""
+    import torch
+    if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits: a CUDA tensor [rows, vocab] with contiguous rows is wanted")
+    rows, vocab = logits.shape
+    dev = logits.device
+    lib = _lib.check_device(dev)
+    ld = logits.stride(0) if rows > 1 else vocab
+    if ld < vocab:
+        raise ValueError("logits: rows overlap")
+    if targets is not None and (targets.dtype != torch.int32 or targets.shape != (rows,) or targets.device != dev or
+                                not targets.is_contiguous()):
+        raise ValueError("targets: a contiguous int32 tensor [rows] on the logits' device is wanted")
+    if not 0 <= k <= MAX_K:
+        raise ValueError(f"k: 0 to {MAX_K} is wanted, not {k}")
+    # one buffer: logprob, entropy, top log probabilities; the ids beside it
+    f = torch.empty(rows * (2 + k), dtype=torch.float32, device=dev)
+    ids = torch.empty(rows, k, dtype=torch.int32, device=dev)
+    p = f.data_ptr()
+    _lib.check(lib.cats_gpu_logprobs_dev(
+        logits.data_ptr(), _type(logits), rows, vocab, ld, targets.data_ptr() if targets is not None else None, k,
+        p if targets is not None else None, p + 4 * rows if entropy else None, ids.data_ptr() if k else None,
+        p + 8 * rows if k else None, stream), "logprobs")
+    return (f[:rows] if targets is not None else None, f[rows:2 * rows] if entropy else None, ids,
+            f[2 * rows:].view(rows, k))

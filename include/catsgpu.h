@@ -31,10 +31,12 @@ extern "C" {
 
 /* ggml type numbers, as in llm/catseye_llm.h:2557-2580 */
 #define CATS_TYPE_F32  0
+#define CATS_TYPE_F16  1
 #define CATS_TYPE_Q4_0 2
 #define CATS_TYPE_Q8_0 8
 #define CATS_TYPE_Q3_K 11
 #define CATS_TYPE_Q6_K 14
+#define CATS_TYPE_BF16 30
 
 /* status codes */
 #define CATS_OK             0
@@ -56,11 +58,13 @@ int cats_gpu_init(int device);
  * 106-112, called from cats_llm_free :641-643) and sgemm_ocl_finish
  * (sgemm_ocl2.h:262-266). */
 void cats_gpu_term(void);
+int cats_gpu_device(void);               /* the device cats_gpu_init selected; -1 before it */
 int cats_gpu_last_error(void);           /* sticky status of the last failing call */
 void cats_gpu_clear_error(void);
 const char *cats_gpu_error_string(int code);
 /* device error word OR-ed by kernels whose bounded waits expired (0 = none) */
 int cats_gpu_device_error(void);
+void cats_gpu_clear_device_error(void);
 
 /* ------------------------------------------------------ weight registry */
 
@@ -300,6 +304,103 @@ int cats_gpu_llm_time_matvec(cats_gpu_llm *m, int kind, int reps, float *ms_per_
  * layout to host memory (tests regenerate the device model's weights). */
 int cats_gpu_synth_tensor(void *host_dst, int type, int n, int d, unsigned long long seed,
                           int tensor_id, float std, float constant);
+
+/* --------------------------------------- paged KV cache in Q4_0 blocks */
+
+/* A KV cache of 4.5 bits a value (the reference keeps fp32, llm/catseye_llm.h:
+ * 621-622), in pages of CATS_KV_PAGE tokens that sequences can share.  pool is
+ * [n_pages][n_layers][n_kv_heads] chunks of 72 * head_size bytes (device,
+ * 16-byte aligned; cats_gpu_kv_page_bytes a page); table is the page number
+ * of each CATS_KV_PAGE tokens of each sequence, [n_seqs][max_pages] (device;
+ * -1 = none).  head_size: a multiple of 32 up to 128 (larger:
+ * CATS_ERR_UNSUPPORTED).
+ *
+ * A chunk (one page, layer and kv head), with HB = head_size / 32:
+ *   K codes  [64 tokens][c = 0..3][HB blocks][4 bytes]: byte i holds elements
+ *            8c + 2i (low nibble) and 8c + 2i + 1 of the block
+ *   V codes  [32 token pairs][g = 0..7][HB][2 tokens][2 bytes]: nibble n holds
+ *            element 4g + n
+ *   K scales [64][HB] fp16; V scales [32 pairs][HB][2 tokens] fp16
+ * A value is scale * (code - 8).  The scale of a block of 32 is -m / 8, m its
+ * value of largest magnitude (the positive one when both signs reach it),
+ * rounded to 8 significant bits and at most 8160 in magnitude; the code is the
+ * nearest one (halves up).  A block that holds a NaN or an infinity reads back
+ * as NaN.
+ *
+ * runs describes a batch: n_runs x {first row, rows, sequence, position of the
+ * first row} (device ints); row i of a run sits at position pos + i.  A run
+ * may be empty; rows outside every run are left as they are.  max_rows (the
+ * longest run) and max_len (the largest position + 1) size the launch: smaller
+ * values than the true ones cost time, not results.  What a run names outside
+ * its range (a row, sequence, position or page) is left out (attention rows at
+ * such a position, and rows read from there, get zeros) and sets a bit of
+ * cats_gpu_device_error().  A position is appended at most once in a call.
+ * type: CATS_TYPE_F32, _F16 or _BF16; ld_*: elements from one row to the next
+ * (any alignment of the type; rows of groups of four aligned elements are
+ * faster).  All are asynchronous on `stream` (NULL: the library's). */
+#define CATS_KV_PAGE 64
+typedef struct {
+    void *pool;
+    const int *table;
+    int n_pages, n_layers, n_kv_heads, head_size;
+    int n_seqs, max_pages;
+} cats_gpu_kv;
+size_t cats_gpu_kv_page_bytes(int n_layers, int n_kv_heads, int head_size);   /* 0: not a size it takes */
+/* k, v: [rows][n_kv_heads * head_size], quantized into the pages of `layer`. */
+int cats_gpu_kv_append_dev(const cats_gpu_kv *c, int layer, const void *k, const void *v, int type, long long ld_k,
+                           long long ld_v, int rows, const int *runs, int n_runs, int max_rows, void *stream);
+/* The inverse: the values the cache holds, rounded to `type`. */
+int cats_gpu_kv_read_dev(const cats_gpu_kv *c, int layer, void *k, void *v, int type, long long ld_k, long long ld_v,
+                         int rows, const int *runs, int n_runs, int max_rows, void *stream);
+/* Causal attention of the rows q [rows][n_heads * head_size] over the cache:
+ * out = softmax(q k / sqrt(head_size)) v over positions 0 .. the row's own of
+ * its sequence (append the batch first), n_heads / n_kv_heads query heads to
+ * a kv head (llm/catseye_llm.h:1677-1723).  A row at a negative position sees
+ * nothing and gets zeros.  Sums and softmax statistics are fp32; fp32 rows
+ * enter the tensor cores as two fp16 halves each of q and of the
+ * probabilities, other types as one. */
+int cats_gpu_kv_attention_dev(const cats_gpu_kv *c, int layer, void *out, const void *q, int type, int n_heads,
+                              long long ld_out, long long ld_q, int rows, const int *runs, int n_runs, int max_rows,
+                              int max_len, void *stream);
+/* Pages dst[i] = pages src[i], every layer and head (host lists, read before
+ * the call returns; captured into a graph by value).  No page may be the
+ * destination of two copies, nor of one and the source of another
+ * (CATS_ERR_ARG).  The table is not needed. */
+int cats_gpu_kv_copy_pages_dev(const cats_gpu_kv *c, const int *src, const int *dst, int n, void *stream);
+
+/* Bookkeeping of the pages (host only, no GPU needed).  Sequences start
+ * empty; the lowest free page is taken first.
+ *  _write: positions pos .. pos + n - 1 of a sequence (pos not past its end)
+ *    become writable: missing pages are taken, pages shared with another
+ *    sequence replaced.  src/dst (room for n / CATS_KV_PAGE + 2 each) receive
+ *    the *n_copies page copies to make first.  CATS_ERR_NOMEM, with nothing
+ *    changed, when too few pages are free.
+ *  _fork: dst_seq becomes the first len tokens of src_seq, sharing its pages.
+ *  _truncate: keep a sequence's first len tokens (0 frees it).
+ *  _compact: renumber so that the used pages come first; src/dst (room for
+ *    n_pages) receive the copies to make.
+ * _table is the host table [n_seqs][max_pages] to upload after any of them. */
+typedef struct cats_gpu_kv_pages cats_gpu_kv_pages;
+cats_gpu_kv_pages *cats_gpu_kv_pages_create(int n_pages, int n_seqs, int max_pages);
+void cats_gpu_kv_pages_destroy(cats_gpu_kv_pages *p);
+int cats_gpu_kv_pages_write(cats_gpu_kv_pages *p, int seq, int pos, int n, int *src, int *dst, int *n_copies);
+int cats_gpu_kv_pages_fork(cats_gpu_kv_pages *p, int src_seq, int dst_seq, int len);
+int cats_gpu_kv_pages_truncate(cats_gpu_kv_pages *p, int seq, int len);
+int cats_gpu_kv_pages_compact(cats_gpu_kv_pages *p, int *src, int *dst, int *n_copies);
+int cats_gpu_kv_pages_length(const cats_gpu_kv_pages *p, int seq);   /* tokens; -1: no such sequence */
+int cats_gpu_kv_pages_free(const cats_gpu_kv_pages *p);              /* free pages */
+const int *cats_gpu_kv_pages_table(const cats_gpu_kv_pages *p);
+
+/* Log probabilities: of the first `vocab` of each row of logits [rows][ld]
+ * (CATS_TYPE_F32, _F16 or _BF16), logprob[row] = log softmax at targets[row]
+ * (0 for a negative target; both NULL: not wanted), entropy[row] (nats; may
+ * be NULL), and the k <= 32 likeliest tokens with their log probabilities,
+ * [rows][k], the lower id first among equals (id -1 and -inf past the
+ * vocabulary).  A logit of -inf has probability 0.  A row with a NaN or +inf,
+ * or with nothing but -inf, has no distribution: NaN, and ids -1.  A target
+ * past the vocabulary gives NaN and sets a bit of cats_gpu_device_error(). */
+int cats_gpu_logprobs_dev(const void *logits, int type, int rows, int vocab, long long ld, const int *targets, int k,
+                          float *logprob, float *entropy, int *top_ids, float *top_logprob, void *stream);
 
 /* ------------------------------------------------------------ CNN sgemm */
 
