@@ -1,6 +1,6 @@
 // kv.cu — operators on the paged Q4_0 KV cache: rows appended and read back,
 // causal attention over it, page copies.  kv.cuh has the layout.
-#include "kv.cuh"
+#include "kv_attn.cuh"
 #include <algorithm>
 #include <climits>
 
@@ -165,6 +165,17 @@ __global__ void __launch_bounds__(128) k_kv_attn_simple(const __grid_constant__ 
 cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, const KvRows &q, int n_heads,
                                 const KvBatch &b, cudaStream_t st)
 {
+    KvAttn a{};
+    a.c = c;
+    a.out = out;
+    a.q = q;
+    a.runs = b.runs;
+    a.type = type;
+    a.n_runs = b.n_runs;
+    a.n_heads = n_heads;
+    a.mul = n_heads / c.n_kv;
+    a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hs);
+    if ((long long)b.max_rows * a.mul <= 128) return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
     const long long items = (long long)std::max(b.max_rows, 1) * n_heads;
     const dim3 grid((unsigned)std::min<long long>((items + 3) / 4, 65535), (unsigned)std::min(b.n_runs, 32768));
     switch (type) {

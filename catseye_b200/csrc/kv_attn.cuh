@@ -1,0 +1,188 @@
+// kv_attn.cuh — what the attention kernels over the paged Q4_0 cache share:
+// fragments of cached codes as fp16, the tensor-core instruction, rows of
+// queries, and the plain loop for rows that a NaN in the cache touched.
+#pragma once
+#include "kv.cuh"
+
+namespace cats {
+
+// An attention call as the kernels take it.
+struct KvAttn {
+    KvView c;
+    KvRows out, q;
+    const KvRun *runs;
+    int type, n_runs, n_heads, mul, tiles;   // tiles: row tiles per run in the grid
+    float scale_log2;                        // log2(e) / sqrt(head size)
+};
+
+// The four halves pairs of a code word: half i of each 16-bit side, (code - 8)
+// times the side's scale.  A nibble under the exponent of 1024 (or 64, four
+// bits up) is 1024 + code (64 + code) exactly; the difference is exact and so
+// is the product (the scale has 8 significant bits).
+__device__ __forceinline__ void kv_dequant(uint32_t w, __half2 s, uint32_t (&x)[4])
+{
+    const uint32_t w8 = w >> 8;
+    uint32_t t[4];
+    t[0] = (w & 0x000f000fu) | 0x64006400u;
+    t[1] = (w & 0x00f000f0u) | 0x54005400u;
+    t[2] = (w8 & 0x000f000fu) | 0x64006400u;
+    t[3] = (w8 & 0x00f000f0u) | 0x54005400u;
+    const __half2 b0 = __half2half2(__ushort_as_half(0x6408)), b1 = __half2half2(__ushort_as_half(0x5480));   // 1032, 72
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 v = __hmul2(__hsub2(*reinterpret_cast<__half2 *>(&t[i]), i & 1 ? b1 : b0), s);
+        x[i] = *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
+__device__ __forceinline__ void kv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// what fp16 leaves of (lo, hi): the second half of a split
+__device__ __forceinline__ uint32_t kv_pack_rest(float lo, float hi, uint32_t top)
+{
+    const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&top));
+    return kv_pack(lo - t.x, hi - t.y);
+}
+__device__ __forceinline__ float kv_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// N consecutive elements of a row of any supported type, as floats
+template <int N> __device__ __forceinline__ void kv_load_row(const KvRows &t, int type, size_t i, float (&x)[N])
+{
+    static_assert(N % 4 == 0, "groups of four");
+    if (type == KV_F32) {
+        const float *p = static_cast<const float *>(t.p) + i;
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            if (t.vec) {
+                const float4 v = *reinterpret_cast<const float4 *>(p + j);
+                x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
+            } else {
+                x[j] = p[j]; x[j + 1] = p[j + 1]; x[j + 2] = p[j + 2]; x[j + 3] = p[j + 3];
+            }
+        }
+        return;
+    }
+    const uint16_t *p = static_cast<const uint16_t *>(t.p) + i;
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        uint16_t h[4];
+        if (t.vec) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p + j);
+            h[0] = (uint16_t)v.x; h[1] = (uint16_t)(v.x >> 16); h[2] = (uint16_t)v.y; h[3] = (uint16_t)(v.y >> 16);
+        } else {
+            h[0] = p[j]; h[1] = p[j + 1]; h[2] = p[j + 2]; h[3] = p[j + 3];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            x[j + e] = type == KV_F16 ? __half2float(__ushort_as_half(h[e])) : __uint_as_float((uint32_t)h[e] << 16);
+    }
+}
+
+__device__ __forceinline__ void kv_store_row4(const KvRows &t, int type, size_t i, const float4 &v)
+{
+    if (type == KV_F32) {
+        float *p = static_cast<float *>(t.p) + i;
+        if (t.vec) {
+            *reinterpret_cast<float4 *>(p) = v;
+        } else {
+            p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w;
+        }
+        return;
+    }
+    uint16_t *p = static_cast<uint16_t *>(t.p) + i;
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    uint16_t h[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        h[e] = type == KV_F16 ? __half_as_ushort(__float2half_rn(f[e])) : __bfloat16_as_ushort(__float2bfloat16_rn(f[e]));
+    if (t.vec) {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+    } else {
+        p[0] = h[0]; p[1] = h[1]; p[2] = h[2]; p[3] = h[3];
+    }
+}
+
+// A power of two that brings a row's largest magnitude to [2^13, 2^14): fp16
+// halves of it keep their bits, whatever the row's scale.
+__device__ __forceinline__ float kv_row_scale(float amax)
+{
+    if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
+    const int ex = (int)(__float_as_uint(amax) >> 23);
+    return __uint_as_float((uint32_t)min(267 - ex, 254) << 23);
+}
+
+// The last position row r of a run sees (-1: none; recorded when it lies past
+// the table or the sequence does not exist).
+__device__ __forceinline__ int kv_limit(const KvView &c, const KvRun &run, int r)
+{
+    const long long at = (long long)run.pos + r;
+    if (at >= 0 && (at >= (long long)c.max_pages * KV_PAGE || run.seq < 0 || run.seq >= c.n_seqs)) {
+        if (c.err) atomicOr(c.err, CATS_DEVERR_PAGE_RANGE);
+        return -1;
+    }
+    if (run.seq < 0 || run.seq >= c.n_seqs) {
+        if (c.err) atomicOr(c.err, CATS_DEVERR_PAGE_RANGE);
+        return -1;
+    }
+    return at < 0 ? -1 : (int)at;
+}
+
+// Elements 4*e4 .. of one row by the plain loop.  The tensor cores multiply a
+// masked position's zero probability with its value too, so a NaN in the cache
+// reaches the rows of its tile that do not see it: those come here (`row` of
+// a, head h, positions 0 .. lim).  What does see a NaN is NaN.
+static __device__ __noinline__ float4 kv_plain_row4(const KvAttn &a, int seq, int row, int h, int lim, int e4)
+{
+    const KvView &c = a.c;
+    const int g = h / a.mul, hs = c.hs;
+    const int *table = c.table + (size_t)seq * c.max_pages;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int t = 0; t <= lim; t++) {
+        const int page = table[t / KV_PAGE];
+        if (page < 0 || page >= c.n_pages) continue;
+        const __half d = *reinterpret_cast<const __half *>(c.chunk(page, g) + kv_scale_off(true, hs, t % KV_PAGE, e4 >> 3));
+        if (__hisnan(d)) return make_float4(NAN, NAN, NAN, NAN);
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int t = 0; t <= lim; t++) {
+        const int page = table[t / KV_PAGE];
+        if (page < 0 || page >= c.n_pages) continue;
+        const uint8_t *ch = c.chunk(page, g);
+        float s = 0.f;
+        for (int e = 0; e < hs / 4; e++) {
+            float x[4];
+            kv_load_row<4>(a.q, a.type, (size_t)row * a.q.ld + (size_t)h * hs + 4 * e, x);
+            const float4 k = kv_load4(ch, false, hs, t % KV_PAGE, e);
+            s += x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w;
+        }
+        s *= a.scale_log2;
+        const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.f : exp2f(m - mn), p = exp2f(s - mn);
+        const float4 v = kv_load4(ch, true, hs, t % KV_PAGE, e4);
+        l = l * al + p;
+        o = make_float4(o.x * al + p * v.x, o.y * al + p * v.y, o.z * al + p * v.z, o.w * al + p * v.w);
+        m = mn;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+cudaError_t launch_kv_attn_split(const KvAttn &a, int max_rows, int max_len, cudaStream_t st);
+
+} // namespace cats
