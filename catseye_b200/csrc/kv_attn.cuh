@@ -15,18 +15,28 @@ struct KvAttn {
     float scale_log2;                        // log2(e) / sqrt(head size)
 };
 
-// The four halves pairs of a code word: half i of each 16-bit side, (code - 8)
-// times the side's scale.  A nibble under the exponent of 1024 (or 64, four
-// bits up) is 1024 + code (64 + code) exactly; the difference is exact and so
-// is the product (the scale has 8 significant bits).
-__device__ __forceinline__ void kv_dequant(uint32_t w, __half2 s, uint32_t (&x)[4])
+// The four pairs of halves of a code word: nibble i of each 16-bit side, (code
+// - 8) times the side's scale.  A nibble under the exponent of 1024 (or 64,
+// four bits up) is 1024 + code (64 + code) exactly; the difference is exact
+// and so is the product (the scale has 8 significant bits).
+struct KvMagic {
+    uint32_t e1024, e64;
+};
+__device__ __forceinline__ KvMagic kv_magic()
+{
+    KvMagic m;   // in registers for good: an instruction takes one immediate, which is the mask
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m.e1024));
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(m.e64));
+    return m;
+}
+__device__ __forceinline__ void kv_dequant(uint32_t w, __half2 s, const KvMagic &mg, uint32_t (&x)[4])
 {
     const uint32_t w8 = w >> 8;
     uint32_t t[4];
-    t[0] = (w & 0x000f000fu) | 0x64006400u;
-    t[1] = (w & 0x00f000f0u) | 0x54005400u;
-    t[2] = (w8 & 0x000f000fu) | 0x64006400u;
-    t[3] = (w8 & 0x00f000f0u) | 0x54005400u;
+    t[0] = (w & 0x000f000fu) | mg.e1024;
+    t[1] = (w & 0x00f000f0u) | mg.e64;
+    t[2] = (w8 & 0x000f000fu) | mg.e1024;
+    t[3] = (w8 & 0x00f000f0u) | mg.e64;
     const __half2 b0 = __half2half2(__ushort_as_half(0x6408)), b1 = __half2half2(__ushort_as_half(0x5480));   // 1032, 72
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -37,10 +47,20 @@ __device__ __forceinline__ void kv_dequant(uint32_t w, __half2 s, uint32_t (&x)[
 
 __device__ __forceinline__ void kv_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
 {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
                  "{%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// d = a b + c0, with the start in registers of its own
+__device__ __forceinline__ void kv_mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                            const float (&c0)[4])
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0[0]), "f"(c0[1]), "f"(c0[2]), "f"(c0[3]));
 }
 
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
@@ -49,16 +69,19 @@ __device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// what fp16 leaves of (lo, hi): the second half of a split
-__device__ __forceinline__ uint32_t kv_pack_rest(float lo, float hi, uint32_t top)
+// what fp16 leaves of v: the second half of a split
+__device__ __forceinline__ float kv_rest(float v) { return v - __half2float(__float2half_rn(v)); }
+// an 8 x 8 matrix of halves, transposed across the warp
+__device__ __forceinline__ uint32_t kv_transpose8(uint32_t v)
 {
-    const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&top));
-    return kv_pack(lo - t.x, hi - t.y);
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 __device__ __forceinline__ float kv_exp2(float x)
 {
     float r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -119,13 +142,13 @@ __device__ __forceinline__ void kv_store_row4(const KvRows &t, int type, size_t 
     }
 }
 
-// A power of two that brings a row's largest magnitude to [2^13, 2^14): fp16
+// A power of two that brings a row's largest magnitude to [2^9, 2^10): fp16
 // halves of it keep their bits, whatever the row's scale.
 __device__ __forceinline__ float kv_row_scale(float amax)
 {
     if (!(amax > 0.f) || !(amax < INFINITY)) return 1.f;
     const int ex = (int)(__float_as_uint(amax) >> 23);
-    return __uint_as_float((uint32_t)min(267 - ex, 254) << 23);
+    return __uint_as_float((uint32_t)max(min(263 - ex, 254), 1) << 23);
 }
 
 // The last position row r of a run sees (-1: none; recorded when it lies past

@@ -22,21 +22,23 @@
 // 8-15 of the same instruction (22 bits, no second product).  fp16 and bf16
 // rows use the 16 rows for 16 queries, or 8 when that is enough.
 #include "kv_attn.cuh"
+#include "tc.cuh"
 #include <algorithm>
 #include <climits>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace cats {
 namespace cg = cooperative_groups;
 
-constexpr int SP_STAGES = 2;
+constexpr int SP_STAGES = 3;
+constexpr int SP_WARPS = 4;
+constexpr int SP_TOK = 32;          // tokens of a stage: half a page
 constexpr float SP_P_BITS = 15.f;   // probabilities are held times 2^15: fp16 keeps those down to 2^-39
 
-__host__ __device__ constexpr int sp_chunk(int hb) { return 2304 * hb; }
-__host__ __device__ constexpr size_t sp_smem(int hb, int warps)
-{
-    return (size_t)warps * SP_STAGES * (sp_chunk(hb) + 8);   // rings | barriers
-}
+// a stage: K codes [32 tokens], V codes, K scales, V scales
+__host__ __device__ constexpr int sp_stage(int hb) { return 1152 * hb; }
+__host__ __device__ constexpr size_t sp_smem(int hb) { return (size_t)SP_WARPS * SP_STAGES * (sp_stage(hb) + 8); }   // rings | barriers
 
 template <int HB> struct Words {
     uint32_t w[HB];
@@ -56,38 +58,83 @@ template <int HB> __device__ __forceinline__ Words<HB> lds_words(const uint8_t *
     }
     return r;
 }
-template <int HB> __device__ __forceinline__ void lds_scales(const uint8_t *p, __half2 (&s)[HB])
+template <int HB> struct Halves {
+    __half h[HB];
+};
+template <int HB> __device__ __forceinline__ Halves<HB> lds_halves(const uint8_t *p)
 {
+    Halves<HB> r;
     if constexpr (HB % 2 == 0) {
+        const Words<HB / 2> v = lds_words<HB / 2>(p);
 #pragma unroll
-        for (int i = 0; i < HB / 2; i++) {
-            const __half2 v = reinterpret_cast<const __half2 *>(p)[i];
-            s[2 * i] = __low2half2(v);
-            s[2 * i + 1] = __high2half2(v);
-        }
+        for (int b = 0; b < HB; b++) r.h[b] = __ushort_as_half((uint16_t)(v.w[b / 2] >> (b % 2 * 16)));
     } else {
 #pragma unroll
-        for (int b = 0; b < HB; b++) s[b] = __half2half2(reinterpret_cast<const __half *>(p)[b]);
+        for (int b = 0; b < HB; b++) r.h[b] = reinterpret_cast<const __half *>(p)[b];
     }
+    return r;
 }
+
+// One row of a unit, normalised and stored four elements at a time.
+__device__ __forceinline__ void finish4(const KvAttn &a, const KvRun &run, const int2 &span, int kvh, long long rr, int e4,
+                                        float4 acc, float l)
+{
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    const int tok = span.x + (int)(rr / a.mul), h = kvh * a.mul + (int)(rr % a.mul), row = run.first + tok;
+    const float sum = acc.x + acc.y + acc.z + acc.w;
+    if (sum != sum && l == l) acc = kv_plain_row4(a, run.seq, row, h, run.pos + tok, e4);
+    kv_store_row4(a.out, a.type, (size_t)row * a.out.ld + (size_t)h * a.c.hs + 4 * e4, acc);
+}
+
+// Half pages that row tile `tile` of a run reaches, as steps of a CTA (one a
+// warp); at least one for a tile that has rows, which have to be written.
+__device__ __forceinline__ int steps_of(const KvAttn &a, const KvRun &run, const int2 &span, long long tile, int rows)
+{
+    const long long n_q = (long long)(span.y - span.x) * a.mul;
+    if (tile * rows >= n_q) return 0;
+    const int last = span.x + (int)((min(n_q, (tile + 1) * rows) - 1) / a.mul);
+    const long long halves = min(((long long)run.pos + last) / SP_TOK + 1, 2ll * a.c.max_pages);
+    return max(1, (int)((halves + SP_WARPS - 1) / SP_WARPS));
+}
+
+// What a streamed call keeps between its two kernels: per CTA the unit that
+// begins in it and goes on in others ((entry, kv head, parts, 0)), and two
+// partial results: of the unit it began with (0) and of the one it ended in (1).
+struct SpWork {
+    int4 *split;
+    float *part;
+};
+__host__ __device__ constexpr int sp_part(int rows, int hs) { return rows * (hs + 2); }
 
 // SPLIT: fp32 rows, 8 of them, halves in rows g and g + 8.  Else ROWS query
 // rows of 16 bits (8: rows g + 8 of the tile stay zero).
-template <bool SPLIT, int ROWS, int HB, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS <= 4 ? 3 : 1) k_kv_attn_split(const __grid_constant__ KvAttn a)
+// A unit is a tile of query rows of a run and a kv head.  STREAM: the units'
+// pages, end to end, are cut into one equal stretch a CTA, whatever the
+// lengths; a unit that lies in several CTAs leaves partial results that
+// k_kv_attn_join adds.  Else: a cluster a unit, its pages interleaved over the
+// CTAs.
+constexpr int SP_MAX_ENTRIES = 1024;   // row tiles whose lengths a streamed CTA scans
+
+__host__ __device__ constexpr int sp_rows(bool split, int nt) { return (split ? 4 : 8) * nt; }
+__host__ __device__ constexpr int sp_resident(int nt) { return nt == 1 ? 4 : 3; }   // CTAs an SM
+
+template <bool SPLIT, int NT, int HB, bool STREAM>
+__global__ void __launch_bounds__(SP_WARPS * 32, sp_resident(NT))
+k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork wk)
 {
-    constexpr int HS = 32 * HB, CHUNK = sp_chunk(HB);
-    constexpr int NR = ROWS / 8;   // rows a lane holds: g, or g and g + 8
-    static_assert(!SPLIT || ROWS == 8, "");
+    constexpr int HS = 32 * HB, STAGE = sp_stage(HB), WARPS = SP_WARPS;
+    constexpr int ROWS = sp_rows(SPLIT, NT);
+    constexpr int NS = SPLIT ? NT : 2 * NT;   // query rows whose scores a lane holds
     extern __shared__ __align__(128) uint8_t smem[];
-    // at the end a warp's rows take its ring's first stage, the CTA's joined rows the second of warp 0
-    static_assert(SP_STAGES >= 2 && ROWS * (HS + 2) * 4 <= CHUNK, "");
-    float *joined = reinterpret_cast<float *>(smem + CHUNK);   // [ROWS][HS], m[ROWS], l[ROWS]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (size_t)WARPS * SP_STAGES * CHUNK);
+    // at the end a warp's rows take its ring, then the CTA's joined rows that of warp 0
+    static_assert(ROWS * (HS + 2) * 4 <= SP_STAGES * STAGE, "");
+    float *joined = reinterpret_cast<float *>(smem);   // [ROWS][HS], m[ROWS], l[ROWS]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (size_t)WARPS * SP_STAGES * STAGE);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    uint8_t *ring = smem + (size_t)warp * SP_STAGES * CHUNK;
+    uint8_t *ring = smem + (size_t)warp * SP_STAGES * STAGE;
     uint64_t *bar = bars + warp * SP_STAGES;
     if (lane == 0) {
         for (int i = 0; i < SP_STAGES; i++) mbar_init(&bar[i], 1);
@@ -96,221 +143,371 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS <= 4 ? 3 : 1) k_kv_attn_spli
     __syncwarp();
     uint32_t phase = 0;    // a bit a stage
     bool broken = false;   // a wait gave up (recorded): no copy is issued any more, the rows are NaN
+    const KvMagic magic = kv_magic();
 
-    const int unit = blockIdx.x / C;
-    const int tile0 = unit % a.tiles, kvh = unit / a.tiles % a.c.n_kv, ri = unit / a.tiles / a.c.n_kv;
-    const KvRun run = a.runs[ri];
-    const int2 span = kv_run_rows(run, a.q.rows, rank == 0 ? a.c.err : nullptr);
-    const long long n_q = (long long)(span.y - span.x) * a.mul;   // query rows of this kv head
-
-    for (long long tile = tile0; tile * ROWS < n_q; tile += a.tiles) {
-        // this lane's query rows
-        int lim[NR], row[NR], head[NR];
-        const int used = (int)min((long long)ROWS, n_q - tile * ROWS);
-#pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const long long r = tile * ROWS + g + 8 * i;
-            row[i] = -1;
-            lim[i] = -1;
-            head[i] = 0;
-            if (r < n_q) {
-                const int tok = span.x + (int)(r / a.mul);
-                row[i] = run.first + tok;
-                head[i] = kvh * a.mul + (int)(r % a.mul);
-                lim[i] = kv_limit(a.c, run, tok);
+    int ri, kvh, entry = 0, at = 0, steps = 0;   // STREAM: entry = run * tiles + tile; steps at .. of it come next
+    long long tile, left = 0, total = 0, begin = 0;
+    bool beyond = false;   // STREAM: some run has more row tiles than the launch counted on
+    if constexpr (STREAM) {
+        long long *pre = reinterpret_cast<long long *>(smem);   // steps before each entry; then the warps' sums
+        const int entries = a.n_runs * a.tiles;
+        static_assert((SP_MAX_ENTRIES + WARPS + 1) * 8 <= WARPS * SP_STAGES * STAGE, "");
+        long long *sums = pre + SP_MAX_ENTRIES;
+        for (int base = 0; base < entries; base += WARPS * 32) {
+            const int i = base + tid;
+            long long v = 0;
+            if (i < entries) {
+                const KvRun r = a.runs[i / a.tiles];
+                const int2 sp = kv_run_rows(r, a.q.rows, blockIdx.x == 0 ? a.c.err : nullptr);
+                v = (long long)steps_of(a, r, sp, i % a.tiles, ROWS) * a.c.n_kv;
+                beyond |= (long long)(sp.y - sp.x) * a.mul > (long long)a.tiles * ROWS;
             }
+            long long x = v;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            if (lane == 31) sums[warp] = x;
+            __syncthreads();
+            long long before = total;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                if (w < warp) before += sums[w];
+                total += sums[w];
+            }
+            if (i < entries) pre[i] = before + x - v;
+            __syncthreads();
         }
-        int top = lim[0], low = row[0] >= 0 ? lim[0] : INT_MAX;
-        if constexpr (NR == 2) {
-            top = max(top, lim[1]);
-            if (row[1] >= 0) low = min(low, lim[1]);
+        beyond = __syncthreads_or(beyond) != 0;
+        begin = total * blockIdx.x / gridDim.x;
+        left = total * (blockIdx.x + 1) / gridDim.x - begin;
+        int hi = entries;   // the entry that holds step `begin`: the last with pre <= begin
+        while (hi - entry > 1) {
+            const int mid = (entry + hi) / 2;
+            if (pre[mid] <= begin) entry = mid;
+            else hi = mid;
+        }
+        const long long into = left > 0 ? begin - pre[entry] : 0;
+        ri = entry / a.tiles;
+        tile = entry % a.tiles;
+        const KvRun r = a.runs[ri];
+        const int per = max(1, steps_of(a, r, kv_run_rows(r, a.q.rows, nullptr), tile, ROWS));
+        kvh = (int)(into / per);
+        at = (int)(into % per);
+        if (tid == 0) wk.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+    } else {
+        const int unit = blockIdx.x / C;
+        tile = unit % a.tiles;
+        kvh = unit / a.tiles % a.c.n_kv;
+        ri = unit / a.tiles / a.c.n_kv;
+    }
+    long long extra = blockIdx.x;   // STREAM: units past the counted tiles, one in gridDim.x
+
+    for (;;) {
+        KvRun run;
+        int2 span;
+        int now = 0;   // STREAM: steps of this unit that are this CTA's
+        if constexpr (STREAM) {
+            if (left > 0) {
+                for (;;) {   // past units that are done and tiles without rows
+                    if (entry >= a.n_runs * a.tiles) break;   // (the runs changed under the kernel)
+                    run = a.runs[ri];
+                    span = kv_run_rows(run, a.q.rows, nullptr);
+                    steps = steps_of(a, run, span, tile, ROWS);
+                    if (steps > 0 && at < steps) break;
+                    at = 0;
+                    if (steps > 0 && ++kvh < a.c.n_kv) continue;
+                    kvh = 0;
+                    entry++;
+                    ri = entry / a.tiles;
+                    tile = entry % a.tiles;
+                }
+                if (entry >= a.n_runs * a.tiles) break;
+                now = (int)min(left, (long long)(steps - at));
+                left -= now;
+            } else {
+                bool found = false;
+                at = 0;
+                if (beyond) {
+                    long long i = extra;
+                    for (ri = 0; ri < a.n_runs && !found; ri++) {
+                        run = a.runs[ri];
+                        span = kv_run_rows(run, a.q.rows, nullptr);
+                        const long long over =
+                            max(0ll, ((long long)(span.y - span.x) * a.mul + ROWS - 1) / ROWS - a.tiles) * a.c.n_kv;
+                        if (i < over) {
+                            found = true;
+                            tile = a.tiles + i / a.c.n_kv;
+                            kvh = (int)(i % a.c.n_kv);
+                            now = steps = steps_of(a, run, span, tile, ROWS);
+                        }
+                        i -= over;
+                    }
+                    extra += gridDim.x;
+                }
+                if (!found) break;
+            }
+        } else {
+            run = a.runs[ri];
+            span = kv_run_rows(run, a.q.rows, rank == 0 ? a.c.err : nullptr);
+        }
+        const long long n_q = (long long)(span.y - span.x) * a.mul;   // query rows of this kv head
+        if (!STREAM && tile * ROWS >= n_q) break;
+        // The query row of column `col` of column tile t: fp32 rows take two
+        // columns, their halves.
+        const int used = (int)min((long long)ROWS, n_q - tile * ROWS);
+        auto token = [&](int r) { return span.x + (int)((tile * ROWS + r) / a.mul); };
+        // the rows whose scores this lane holds: columns 2c, 2c + 1 of the tiles
+        int lim[NS];
+        int top = -1, low = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const int r = SPLIT ? 4 * i + c : 8 * (i >> 1) + 2 * c + (i & 1);
+            lim[i] = -1;
+            if (r < used) {
+                lim[i] = kv_limit(a.c, run, token(r));
+                top = max(top, lim[i]);
+                low = min(low, lim[i]);
+            }
         }
         top = __reduce_max_sync(0xffffffffu, top);
         low = __reduce_min_sync(0xffffffffu, low);
-        const int n_pages = top / KV_PAGE + (top >= 0);
+        int n_tiles = top < 0 ? 0 : top / SP_TOK + 1;   // (a streamed CTA's end of them)
+        if (STREAM) n_tiles = min(n_tiles, (at + now) * WARPS);
 
-        // queries as A fragments: word (c, b) of a key holds elements 8c + {0..7}
-        // of block b in the pairs (e, e + 4)
-        uint32_t qf[2 * HB][4];
-        float kf[NR];
-        {
-            float x[NR][8 * HB];
+        // Queries as B fragments (column g).  Word (c, b) of a key holds elements
+        // 8c + {0..7} of block b, element e in nibble e.
+        // 16 bits: the words masked with 000f000f (00f000f0) read as the fp16
+        // subnormals code * 2^-24 (* 2^-20), so the queries of the former are held
+        // 16 times larger, the products come out as 2^-20 q code, the -8 of a code
+        // enters as the accumulator's start, -8 * 2^-20 * sum q, and a block's sum is
+        // scaled after the product.  That start is some ten times the sum's size,
+        // whose last bits the tensor cores then drop: fp32 rows take the keys'
+        // values themselves instead.
+        uint32_t qf[NT][2 * HB][2];
+        float kf[NS], start[NT][SPLIT ? 1 : HB][4];
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
+        for (int t = 0; t < NT; t++) {
+            const int r = SPLIT ? 4 * t + (g >> 1) : 8 * t + g;
+            float x[8 * HB], amax = 0.f;
 #pragma unroll
-                for (int b = 0; b < HB; b++) {
-                    float v[8];
+            for (int b = 0; b < HB; b++) {
+                float v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) v[e] = 0.f;
-                    if (row[i] >= 0)
-                        kv_load_row<8>(a.q, a.type, (size_t)row[i] * a.q.ld + (size_t)head[i] * HS + 32 * b + 8 * c, v);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[i][8 * b + e] = v[e];
+                for (int e = 0; e < 8; e++) v[e] = 0.f;
+                if (r < used) {
+                    const int tok = token(r), h = kvh * a.mul + (int)((tile * ROWS + r) % a.mul);
+                    kv_load_row<8>(a.q, a.type, (size_t)(run.first + tok) * a.q.ld + (size_t)h * HS + 32 * b + 8 * c, v);
                 }
-                float amax = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8 * HB; e++) amax = fmaxf(amax, fabsf(x[i][e]));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const float sc = a.type == KV_F16 ? 1.f : kv_row_scale(amax);   // fp16 rows are what they are
-                kf[i] = a.scale_log2 / sc;
-#pragma unroll
-                for (int e = 0; e < 8 * HB; e++) x[i][e] *= sc;
+                for (int e = 0; e < 8; e++) {
+                    x[8 * b + e] = v[e];
+                    amax = fmaxf(amax, fabsf(v[e]));
+                }
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const float sc = kv_row_scale(amax), k = a.scale_log2 * (SPLIT ? 1.f : 1048576.f) / sc;
+            if constexpr (SPLIT) {
+                kf[t] = __shfl_sync(0xffffffffu, k, 8 * c);
+            } else {
+                kf[2 * t] = __shfl_sync(0xffffffffu, k, 8 * c);
+                kf[2 * t + 1] = __shfl_sync(0xffffffffu, k, 8 * c + 4);
             }
 #pragma unroll
-            for (int b = 0; b < HB; b++)
+            for (int e = 0; e < 8 * HB; e++) {
+                x[e] *= sc;
+                if (SPLIT && (g & 1)) x[e] = kv_rest(x[e]);
+            }
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+            for (int b = 0; b < HB; b++) {
+                float sum = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {   // pair 2h + u: columns 2c.. (u = 0) or 2c + 8..
-                        const int e = 8 * b + 2 * h + u;
-                        const uint32_t t = kv_pack(x[0][e], x[0][e + 4]);
-                        qf[2 * b + h][2 * u] = t;
-                        if constexpr (SPLIT) qf[2 * b + h][2 * u + 1] = kv_pack_rest(x[0][e], x[0][e + 4], t);
-                        else if constexpr (NR == 2) qf[2 * b + h][2 * u + 1] = kv_pack(x[NR - 1][e], x[NR - 1][e + 4]);
-                        else qf[2 * b + h][2 * u + 1] = 0u;
-                    }
+                for (int u = 0; u < 4; u++) {   // pair u: elements u, u + 4
+                    const float f = SPLIT || (u & 1) ? 1.f : 16.f;
+                    qf[t][2 * b + (u >> 1)][u & 1] = kv_pack(f * x[8 * b + u], f * x[8 * b + u + 4]);
+                    sum += x[8 * b + u] + x[8 * b + u + 4];
+                }
+                if constexpr (!SPLIT) {
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                    sum *= -8.f / 1048576.f;
+                    start[t][b][0] = start[t][b][2] = __shfl_sync(0xffffffffu, sum, 8 * c);
+                    start[t][b][1] = start[t][b][3] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+                }
+            }
         }
 
-        float o[4 * HB][4];   // tile (b, n): column j of it is element 32b + 4j + n
+        // O^T: tile (b, u): rows g (g + 8) are elements 32b + 4g + 2u (+ 1)
+        float o[NT][2 * HB][4];
 #pragma unroll
-        for (int i = 0; i < 4 * HB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m[NR], l[NR];
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
+            for (int i = 0; i < 2 * HB; i++) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+        float m[NS], l[NS];
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
             m[i] = -INFINITY;
             l[i] = 0.f;
         }
 
-        // this warp's pages: first, first + step, ...; lane j keeps the number of the
-        // page 32 k + j steps on
-        const int first = rank * WARPS + warp, step = C * WARPS;
-        const int mine = first < n_pages ? (n_pages - first + step - 1) / step : 0;
-        auto look = [&](int i) {
-            const int p = first + i * step;
-            return i < mine ? a.c.page(run.seq, p) : -1;
-        };
+        // this warp's half pages: first, first + step, ...; lane j keeps the page of
+        // the 32 k + j th
+        const int first = (STREAM ? at : rank) * WARPS + warp, step = STREAM ? WARPS : C * WARPS;
+        const int mine = first < n_tiles ? (n_tiles - first + step - 1) / step : 0;
+        auto look = [&](int i) { return i < mine ? a.c.page(run.seq, (first + i * step) / 2) : -1; };
         int pages = look(lane), ahead = mine > 32 ? look(32 + lane) : -1;   // of i's group of 32, and the next
-        auto issue = [&](int i, int page) {
+        auto issue = [&](int i, int page, int st) {
             if (page >= 0 && lane == 0) {
-                mbar_arrive_expect_tx(&bar[i % SP_STAGES], CHUNK);
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                 smem_u32(ring + (i % SP_STAGES) * CHUNK)),
-                             "l"(a.c.chunk(page, kvh)), "r"(CHUNK), "r"(smem_u32(&bar[i % SP_STAGES]))
-                             : "memory");
+                const int half = (first + i * step) & 1;
+                const uint8_t *src = a.c.chunk(page, kvh);
+                uint8_t *dst = ring + st * STAGE;
+                mbar_arrive_expect_tx(&bar[st], STAGE);
+                bulk_g2s_keep(dst, src + half * 16 * HS, 16 * HS, &bar[st]);
+                bulk_g2s_keep(dst + 16 * HS, src + kv_v_codes(HS) + half * 16 * HS, 16 * HS, &bar[st]);
+                bulk_g2s_keep(dst + 32 * HS, src + kv_k_scales(HS) + half * 2 * HS, 2 * HS, &bar[st]);
+                bulk_g2s_keep(dst + 34 * HS, src + kv_v_scales(HS) + half * 2 * HS, 2 * HS, &bar[st]);
             }
         };
         int here[SP_STAGES];   // pages in the ring, the next one to use first
 #pragma unroll
         for (int i = 0; i < SP_STAGES; i++) {
             here[i] = __shfl_sync(0xffffffffu, pages, i);
-            issue(i, here[i]);
+            issue(i, here[i], i);
         }
 
+        // 32 tokens from p0 on; EDGE: some of them lie past some row's last position
+        auto take = [&](const uint8_t *ch, int p0, auto edge_tag) {
+            constexpr bool EDGE = decltype(edge_tag)::value;
+            float s[NT][2][4];   // S^T: tokens 16i + g and + 8 of columns 2c, 2c + 1
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int ta = 16 * i + g;
+                const Words<HB> wa = lds_words<HB>(ch + (ta * 4 + c) * 4 * HB), wb = lds_words<HB>(ch + ((ta + 8) * 4 + c) * 4 * HB);
+                const Halves<HB> da = lds_halves<HB>(ch + 32 * HS + ta * 2 * HB), db = lds_halves<HB>(ch + 32 * HS + (ta + 8) * 2 * HB);
+#pragma unroll
+                for (int t = 0; t < NT; t++) s[t][i][0] = s[t][i][1] = s[t][i][2] = s[t][i][3] = 0.f;
+#pragma unroll
+                for (int b = 0; b < HB; b++) {
+                    if constexpr (SPLIT) {
+                        uint32_t xa[4], xb[4];
+                        kv_dequant(wa.w[b], __half2half2(da.h[b]), magic, xa);
+                        kv_dequant(wb.w[b], __half2half2(db.h[b]), magic, xb);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t f[4] = {xa[2 * h], xb[2 * h], xa[2 * h + 1], xb[2 * h + 1]};
+#pragma unroll
+                            for (int t = 0; t < NT; t++) kv_mma(s[t][i], f, qf[t][2 * b + h][0], qf[t][2 * b + h][1]);
+                        }
+                    } else {
+                        const uint32_t va = wa.w[b] >> 8, vb = wb.w[b] >> 8;
+                        const uint32_t f0[4] = {wa.w[b] & 0x000f000fu, wb.w[b] & 0x000f000fu, wa.w[b] & 0x00f000f0u, wb.w[b] & 0x00f000f0u};
+                        const uint32_t f1[4] = {va & 0x000f000fu, vb & 0x000f000fu, va & 0x00f000f0u, vb & 0x00f000f0u};
+                        const float ka = __half2float(da.h[b]), kb = __half2float(db.h[b]);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            float d[4];
+                            kv_mma_from(d, f0, qf[t][2 * b][0], qf[t][2 * b][1], start[t][b]);
+                            kv_mma(d, f1, qf[t][2 * b + 1][0], qf[t][2 * b + 1][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) s[t][i][e] = fmaf(e < 2 ? ka : kb, d[e], s[t][i][e]);
+                        }
+                    }
+                }
+            }
+            uint32_t pf[NT][2][2];
+            float alpha[NS];
+            bool moved = false;
+#pragma unroll
+            for (int r = 0; r < NS; r++) {
+                const int t = SPLIT ? r : r >> 1, e = SPLIT ? 0 : r & 1;
+                float v[4];   // tokens g, g + 8, g + 16, g + 24
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float *d = s[t][k >> 1] + 2 * (k & 1);
+                    v[k] = SPLIT ? d[0] + d[1] : d[e];
+                    if (EDGE && p0 + 8 * k + g > lim[r]) v[k] = -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float mn = fmaxf(m[r], mx * kf[r]);
+                alpha[r] = m[r] == -INFINITY ? 0.f : kv_exp2(m[r] - mn);
+                moved |= mn != m[r];
+                m[r] = mn;
+                const float ref = mn == -INFINITY ? 0.f : SP_P_BITS - mn;
+                float sum = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v[k] = kv_exp2(fmaf(v[k], kf[r], ref));
+                    sum += v[k];
+                    if constexpr (SPLIT) pf[t][k >> 1][k & 1] = kv_pack(v[k], kv_rest(v[k]));
+                    else s[t][k >> 1][2 * (k & 1) + e] = v[k];
+                }
+                l[r] = l[r] * alpha[r] + sum;   // this lane's tokens; the others' at the end
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if constexpr (!SPLIT) pf[t][i][u] = kv_pack(s[t][i][2 * u], s[t][i][2 * u + 1]);
+                        pf[t][i][u] = kv_transpose8(pf[t][i][u]);   // (token, column) -> (column, token): a B fragment
+                    }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int n = 0; n < 2 * HB; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[t][n][e] *= SPLIT ? alpha[t] : alpha[2 * t + (e & 1)];
+            }
+            // O^T += V^T P^T
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                Words<HB> vw[2], vs[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int pair = 8 * i + 4 * u + c;
+                    vw[u] = lds_words<HB>(ch + 16 * HS + (pair * 8 + g) * 4 * HB);
+                    vs[u] = lds_words<HB>(ch + 34 * HS + pair * 4 * HB);
+                    if (EDGE) {   // tokens nobody sees may read as NaN
+                        const int tk = p0 + 2 * pair;
+                        const uint32_t keep = tk + 1 <= top ? 0xffffffffu : tk <= top ? 0xffffu : 0u;
+#pragma unroll
+                        for (int b = 0; b < HB; b++) vs[u].w[b] &= keep;
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < HB; b++) {
+                    uint32_t x0[4], x1[4];
+                    kv_dequant(vw[0].w[b], *reinterpret_cast<__half2 *>(&vs[0].w[b]), magic, x0);
+                    kv_dequant(vw[1].w[b], *reinterpret_cast<__half2 *>(&vs[1].w[b]), magic, x1);
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const uint32_t f[4] = {x0[2 * u], x0[2 * u + 1], x1[2 * u], x1[2 * u + 1]};
+#pragma unroll
+                        for (int t = 0; t < NT; t++) kv_mma(o[t][2 * b + u], f, pf[t][i][0], pf[t][i][1]);
+                    }
+                }
+            }
+        };
+
+        int st = 0;
         for (int i = 0; i < mine; i++) {
-            const int st = i % SP_STAGES, page = here[0];
-            const int p0 = (first + i * step) * KV_PAGE;
+            const int page = here[0], p0 = (first + i * step) * SP_TOK;
             if (page >= 0) {
                 const bool ok = mbar_wait_bounded(&bar[st], phase >> st & 1, a.c.err, CATS_DEVERR_MBAR_FULL);
                 if (!__all_sync(0xffffffffu, ok)) broken = true;
                 phase ^= 1u << st;
             }
             if (page >= 0 && !broken) {
-                const uint8_t *ch = ring + st * CHUNK;
-                // S = Q K^T
-                float s[8][4];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-                    const int t = 8 * j + g;
-                    const Words<HB> kw = lds_words<HB>(ch + (t * 4 + c) * 4 * HB);
-                    __half2 ks[HB];
-                    lds_scales<HB>(ch + kv_k_scales(HS) + t * 2 * HB, ks);
-#pragma unroll
-                    for (int b = 0; b < HB; b++) {
-                        uint32_t x[4];
-                        kv_dequant(kw.w[b], ks[b], x);
-                        kv_mma(s[j], qf[2 * b], x[0], x[1]);
-                        kv_mma(s[j], qf[2 * b + 1], x[2], x[3]);
-                    }
-                }
-                const bool edge = p0 + KV_PAGE - 1 > low;
-                uint32_t pf[4][4];
-                float alpha[NR];
-                bool moved = false;
-#pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float v = (SPLIT ? s[j][e] + s[j][e + 2] : s[j][2 * r + e]) * kf[r];
-                            if (edge && p0 + 8 * j + 2 * c + e > lim[r]) v = -INFINITY;
-                            s[j][2 * r + e] = v;
-                            mx = fmaxf(mx, v);
-                        }
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    const float mn = fmaxf(m[r], mx);
-                    alpha[r] = m[r] == -INFINITY ? 0.f : kv_exp2(m[r] - mn);
-                    moved |= mn != m[r];
-                    m[r] = mn;
-                    const float ref = mn == -INFINITY ? 0.f : mn - SP_P_BITS;
-                    float sum = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const float p = kv_exp2(s[j][2 * r + e] - ref);
-                            s[j][2 * r + e] = p;
-                            sum += p;
-                        }
-                    l[r] = l[r] * alpha[r] + sum;   // this lane's columns; its quad's at the end
-                }
-                if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                    for (int n = 0; n < 4 * HB; n++) {
-                        o[n][0] *= alpha[0];
-                        o[n][1] *= alpha[0];
-                        o[n][2] *= SPLIT ? alpha[0] : alpha[NR - 1];
-                        o[n][3] *= SPLIT ? alpha[0] : alpha[NR - 1];
-                    }
-                }
-#pragma unroll
-                for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const float *p = s[2 * kt + u];
-                        pf[kt][2 * u] = kv_pack(p[0], p[1]);
-                        pf[kt][2 * u + 1] = SPLIT ? kv_pack_rest(p[0], p[1], pf[kt][2 * u]) : NR == 2 ? kv_pack(p[2], p[3]) : 0u;
-                    }
-                // O += P V
-                const bool ragged = p0 + KV_PAGE - 1 > top;   // tokens nobody wrote may read as NaN
-#pragma unroll
-                for (int kt = 0; kt < 4; kt++) {
-                    Words<HB> vw[2], vs[2];
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const int pair = 8 * kt + 4 * u + c;
-                        vw[u] = lds_words<HB>(ch + kv_v_codes(HS) + (pair * 8 + g) * 4 * HB);
-                        vs[u] = lds_words<HB>(ch + kv_v_scales(HS) + pair * 4 * HB);
-                        if (ragged) {
-                            const int t = p0 + 2 * pair;
-                            const uint32_t keep = t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
-#pragma unroll
-                            for (int b = 0; b < HB; b++) vs[u].w[b] &= keep;
-                        }
-                    }
-#pragma unroll
-                    for (int b = 0; b < HB; b++) {
-                        uint32_t x0[4], x1[4];
-                        kv_dequant(vw[0].w[b], *reinterpret_cast<__half2 *>(&vs[0].w[b]), x0);
-                        kv_dequant(vw[1].w[b], *reinterpret_cast<__half2 *>(&vs[1].w[b]), x1);
-#pragma unroll
-                        for (int n = 0; n < 4; n++) kv_mma(o[4 * b + n], pf[kt], x0[n], x1[n]);
-                    }
-                }
+                if (p0 + SP_TOK - 1 > low) take(ring + st * STAGE, p0, std::true_type{});
+                else take(ring + st * STAGE, p0, std::false_type{});
             }
             __syncwarp();   // every lane has read this stage
             const int nx = i + SP_STAGES;
@@ -322,151 +519,268 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS <= 4 ? 3 : 1) k_kv_attn_spli
             for (int k = 0; k + 1 < SP_STAGES; k++) here[k] = here[k + 1];
             const int next = __shfl_sync(0xffffffffu, pages, nx & 31);
             here[SP_STAGES - 1] = broken ? -1 : next;
-            issue(nx, here[SP_STAGES - 1]);
+            issue(nx, here[SP_STAGES - 1], st);
+            st = st + 1 == SP_STAGES ? 0 : st + 1;
         }
 
         // ---- the warp's rows to its own ring (its copies are all consumed)
         float *part = reinterpret_cast<float *>(ring);   // [ROWS][HS], m[ROWS], l[ROWS]
 #pragma unroll
-        for (int r = 0; r < NR; r++) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (broken) l[r] = NAN;
-            if (c == 0) {
-                part[ROWS * HS + g + 8 * r] = m[r];
-                part[ROWS * HS + ROWS + g + 8 * r] = l[r];
+        for (int i = 0; i < NS; i++) {
+            const int t = SPLIT ? i : i >> 1, e = SPLIT ? 0 : i & 1, r = SPLIT ? 4 * i + c : 8 * t + 2 * c + e;
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
+            if (broken) l[i] = NAN;
+            if (g == 0) {
+                part[ROWS * HS + r] = m[i];
+                part[ROWS * HS + ROWS + r] = l[i];
             }
 #pragma unroll
-            for (int b = 0; b < HB; b++)
+            for (int b = 0; b < HB; b++) {
+                float f[4];
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    float4 v;
-                    float *f = reinterpret_cast<float *>(&v);
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        f[n] = SPLIT ? o[4 * b + n][e] + o[4 * b + n][e + 2] : o[4 * b + n][2 * r + e];
-                    *reinterpret_cast<float4 *>(part + (g + 8 * r) * HS + 32 * b + 4 * (2 * c + e)) = v;
+                for (int n = 0; n < 4; n++) {
+                    const float *d = o[t][2 * b + (n >> 1)] + 2 * (n & 1);
+                    f[n] = SPLIT ? d[0] + d[1] : d[e];
                 }
+                *reinterpret_cast<float4 *>(part + r * HS + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
+            }
         }
         __syncthreads();
         // ---- the CTA's warps joined, in their order
-        for (int i = tid; i < used * (HS / 4); i += WARPS * 32) {
-            const int r = i / (HS / 4), e4 = i % (HS / 4);
-            float mm = -INFINITY;
+        constexpr int ITEMS = (ROWS * (HS / 4) + WARPS * 32 - 1) / (WARPS * 32);
+        float4 acc[ITEMS];
+        float2 ml[ITEMS];
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) {
+            const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
+            acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            ml[k] = make_float2(-INFINITY, 0.f);
+            if (r >= ROWS) continue;
 #pragma unroll
             for (int w = 0; w < WARPS; w++)
-                mm = fmaxf(mm, reinterpret_cast<const float *>(smem + (size_t)w * SP_STAGES * CHUNK)[ROWS * HS + r]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float ll = 0.f;
+                ml[k].x = fmaxf(ml[k].x, reinterpret_cast<const float *>(smem + (size_t)w * SP_STAGES * STAGE)[ROWS * HS + r]);
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
-                const float *p = reinterpret_cast<const float *>(smem + (size_t)w * SP_STAGES * CHUNK);
-                const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - mm);
+                const float *p = reinterpret_cast<const float *>(smem + (size_t)w * SP_STAGES * STAGE);
+                const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - ml[k].x);
                 const float4 v = *reinterpret_cast<const float4 *>(p + r * HS + 4 * e4);
-                ll += f * p[ROWS * HS + ROWS + r];
-                acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-            }
-            *reinterpret_cast<float4 *>(joined + r * HS + 4 * e4) = acc;
-            if (e4 == 0) {
-                joined[ROWS * HS + r] = mm;
-                joined[ROWS * HS + ROWS + r] = ll;
+                ml[k].y += f * p[ROWS * HS + ROWS + r];
+                acc[k].x += f * v.x; acc[k].y += f * v.y; acc[k].z += f * v.z; acc[k].w += f * v.w;
             }
         }
-        if (C > 1) cl.sync();
-        else __syncthreads();
-        // ---- the cluster's CTAs joined, and the rows stored
-        for (int i = rank * WARPS * 32 + tid; i < used * (HS / 4); i += C * WARPS * 32) {
-            const int r = i / (HS / 4), e4 = i % (HS / 4);
-            float4 acc;
-            float ll;
-            if (C == 1) {
-                acc = *reinterpret_cast<const float4 *>(joined + r * HS + 4 * e4);
-                ll = joined[ROWS * HS + ROWS + r];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; k++) {
+            const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
+            if (r >= ROWS) continue;
+            *reinterpret_cast<float4 *>(joined + r * HS + 4 * e4) = acc[k];
+            if (e4 == 0) {
+                joined[ROWS * HS + r] = ml[k].x;
+                joined[ROWS * HS + ROWS + r] = ml[k].y;
+            }
+        }
+        if constexpr (STREAM) {
+            __syncthreads();
+            if (now == steps) {
+                for (int i = tid; i < used * (HS / 4); i += WARPS * 32) {
+                    const int r = i / (HS / 4), e4 = i % (HS / 4);
+                    finish4(a, run, span, kvh, tile * ROWS + r, e4, *reinterpret_cast<const float4 *>(joined + r * HS + 4 * e4),
+                            joined[ROWS * HS + ROWS + r]);
+                }
             } else {
-                float mm = -INFINITY;
-                for (int k = 0; k < C; k++) mm = fmaxf(mm, cl.map_shared_rank(joined, k)[ROWS * HS + r]);
-                acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                ll = 0.f;
-                for (int k = 0; k < C; k++) {
-                    const float *p = cl.map_shared_rank(joined, k);
-                    const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - mm);
-                    const float4 v = *reinterpret_cast<const float4 *>(p + r * HS + 4 * e4);
-                    ll += f * p[ROWS * HS + ROWS + r];
-                    acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+                float *dst = wk.part + (size_t)(2 * blockIdx.x + (at == 0)) * sp_part(ROWS, HS);
+                for (int i = tid; i < sp_part(ROWS, HS) / 2; i += WARPS * 32)
+                    reinterpret_cast<float2 *>(dst)[i] = reinterpret_cast<const float2 *>(joined)[i];
+                if (at == 0 && tid == 0) {
+                    // the unit begins here: the last CTA that has steps of it
+                    const long long end = begin + (total * (blockIdx.x + 1) / gridDim.x - begin) - now + steps;
+                    const int last = (int)((end * gridDim.x - 1) / total);
+                    wk.split[blockIdx.x] = make_int4(entry, kvh, last - (int)blockIdx.x + 1, 0);
                 }
             }
-            const float inv = ll == 0.f ? 0.f : 1.f / ll;
-            acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-            const long long rr = tile * ROWS + r;
-            const int tok = span.x + (int)(rr / a.mul), h = kvh * a.mul + (int)(rr % a.mul), orow = run.first + tok;
-            const float sum = acc.x + acc.y + acc.z + acc.w;
-            if (sum != sum && ll == ll) acc = kv_plain_row4(a, run.seq, orow, h, run.pos + tok, e4);
-            kv_store_row4(a.out, a.type, (size_t)orow * a.out.ld + (size_t)h * HS + 4 * e4, acc);
+            at += now;
+            fence_proxy_async_smem();
+            __syncthreads();   // the next unit's copies may overwrite the rows
+        } else {
+            if (C > 1) cl.sync();
+            else __syncthreads();
+            // ---- the cluster's CTAs joined, and the rows stored
+            for (int i = rank * WARPS * 32 + tid; i < used * (HS / 4); i += C * WARPS * 32) {
+                const int r = i / (HS / 4), e4 = i % (HS / 4);
+                float4 acc = *reinterpret_cast<const float4 *>(joined + r * HS + 4 * e4);
+                float ll = joined[ROWS * HS + ROWS + r];
+                if (C > 1) {
+                    float mm = -INFINITY;
+                    for (int k = 0; k < C; k++) mm = fmaxf(mm, cl.map_shared_rank(joined, k)[ROWS * HS + r]);
+                    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    ll = 0.f;
+                    for (int k = 0; k < C; k++) {
+                        const float *p = cl.map_shared_rank(joined, k);
+                        const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - mm);
+                        const float4 v = *reinterpret_cast<const float4 *>(p + r * HS + 4 * e4);
+                        ll += f * p[ROWS * HS + ROWS + r];
+                        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+                    }
+                }
+                finish4(a, run, span, kvh, tile * ROWS + r, e4, acc, ll);
+            }
+            fence_proxy_async_smem();
+            if (C > 1) cl.sync();   // nobody's rows are read any more
+            else __syncthreads();
+            tile += a.tiles;
         }
-        if (C > 1) cl.sync();   // nobody's rows are read any more
-        else __syncthreads();
     }
+    if (STREAM) pdl_launch_dependents();
 }
 
-template <bool SPLIT, int ROWS, int HB, int WARPS>
+// The units that lie in several CTAs' stretches: blockIdx.x is the CTA one
+// begins in, blockIdx.y its row; eight groups of threads take every eighth
+// part and are joined in their order.
+template <int ROWS>
+__global__ void __launch_bounds__(256) k_kv_attn_join(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork wk)
+{
+    __shared__ float4 so[8][32];
+    __shared__ float2 sm[8];
+    pdl_wait();
+    const int4 sp = wk.split[blockIdx.x];
+    const int r = blockIdx.y, x = threadIdx.x & 31, y = threadIdx.x >> 5, hs = a.c.hs;
+    if (sp.z == 0) return;
+    const KvRun run = a.runs[sp.x / a.tiles];
+    const int2 span = kv_run_rows(run, a.q.rows, nullptr);
+    const long long rr = (long long)(sp.x % a.tiles) * ROWS + r;
+    if (rr >= (long long)(span.y - span.x) * a.mul) return;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float mp, float lp, const float4 &v) {
+        const float mn = fmaxf(m, mp);
+        const float f = m == -INFINITY ? 0.f : kv_exp2(m - mn), g = mp == -INFINITY ? 0.f : kv_exp2(mp - mn);
+        m = mn;
+        l = l * f + lp * g;
+        acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
+    };
+#pragma unroll 4
+    for (int k = y; k < sp.z; k += 8) {
+        const float *p = wk.part + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * sp_part(ROWS, hs);
+        const float4 v = 4 * x < hs ? *reinterpret_cast<const float4 *>(p + r * hs + 4 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+        add(p[ROWS * hs + r], p[ROWS * hs + ROWS + r], v);
+    }
+    so[y][x] = acc;
+    if (x == 0) sm[y] = make_float2(m, l);
+    __syncthreads();
+    if (y > 0 || 4 * x >= hs) return;
+    for (int k = 1; k < min(8, sp.z); k++) add(sm[k].x, sm[k].y, so[k][x]);
+    finish4(a, run, span, sp.y, rr, x, acc, l);
+}
+
+// The partial results of a streamed call live in memory of the call's own,
+// ordered on its stream (a graph that captures the call owns it), so calls on
+// several streams and captured ones share nothing.  The pool keeps what it
+// once had.
+static cudaMemPool_t work_pool()
+{
+    static cudaMemPool_t pools[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (!pools[dev]) {
+        cudaMemPoolProps pr{};
+        pr.allocType = cudaMemAllocationTypePinned;
+        pr.location.type = cudaMemLocationTypeDevice;
+        pr.location.id = dev;
+        uint64_t keep = UINT64_MAX;
+        cudaMemPool_t p = nullptr;
+        if (cudaMemPoolCreate(&p, &pr) != cudaSuccess ||
+            cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        pools[dev] = p;
+    }
+    return pools[dev];
+}
+
+template <bool SPLIT, int NT, int HB, bool STREAM>
 static cudaError_t launch_one(const KvAttn &a, int units, int C, cudaStream_t st)
 {
+    constexpr int ROWS = sp_rows(SPLIT, NT);
     static unsigned long long done = 0;
-    const size_t smem = sp_smem(HB, WARPS);
-    auto *k = k_kv_attn_split<SPLIT, ROWS, HB, WARPS>;
-    cudaError_t e = once_per_device(done, [&] {
-        cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        return r ? r : cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    });
+    const size_t smem = sp_smem(HB);
+    auto *k = k_kv_attn_split<SPLIT, NT, HB, STREAM>;
+    cudaError_t e = once_per_device(
+        done, [&] { return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
     if (e) return e;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)C;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)units * C);
-    cfg.blockDim = dim3(WARPS * 32);
+    cfg.blockDim = dim3(SP_WARPS * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, a);
+    SpWork wk{nullptr, nullptr};
+    if (!STREAM) {
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = (unsigned)C;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.gridDim = dim3((unsigned)units * C);
+        return cudaLaunchKernelEx(&cfg, k, a, wk);
+    }
+    const int grid = 148 * sp_resident(NT);
+    const size_t split = round_up((size_t)grid * sizeof(int4), 256), part = (size_t)grid * 2 * sp_part(ROWS, 32 * HB) * 4;
+    cudaMemPool_t pool = work_pool();
+    uint8_t *p = nullptr;
+    if (!pool) return cudaErrorMemoryAllocation;
+    if ((e = cudaMallocFromPoolAsync(reinterpret_cast<void **>(&p), split + part, pool, st))) return e;
+    wk.split = reinterpret_cast<int4 *>(p);
+    wk.part = reinterpret_cast<float *>(p + split);
+    cfg.gridDim = dim3(grid);
+    cfg.numAttrs = 0;
+    e = cudaLaunchKernelEx(&cfg, k, a, wk);
+    if (!e) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3(grid, ROWS);
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelEx(&cfg, k_kv_attn_join<ROWS>, a, wk);
+    }
+    const cudaError_t f = cudaFreeAsync(p, st);
+    return e ? e : f;
 }
 
-template <bool SPLIT, int ROWS, int WARPS>
+template <bool SPLIT, int NT, bool STREAM>
 static cudaError_t launch_hb(const KvAttn &a, int units, int C, cudaStream_t st)
 {
     switch (a.c.hs / 32) {
-    case 1: return launch_one<SPLIT, ROWS, 1, WARPS>(a, units, C, st);
-    case 2: return launch_one<SPLIT, ROWS, 2, WARPS>(a, units, C, st);
-    case 3: return launch_one<SPLIT, ROWS, 3, WARPS>(a, units, C, st);
-    case 4: return launch_one<SPLIT, ROWS, 4, WARPS>(a, units, C, st);
+    case 1: return launch_one<SPLIT, NT, 1, STREAM>(a, units, C, st);
+    case 2: return launch_one<SPLIT, NT, 2, STREAM>(a, units, C, st);
+    case 3: return launch_one<SPLIT, NT, 3, STREAM>(a, units, C, st);
+    case 4: return launch_one<SPLIT, NT, 4, STREAM>(a, units, C, st);
     }
     return cudaErrorInvalidValue;
-}
-
-template <int WARPS> static cudaError_t launch_rows(const KvAttn &a, int rows, int units, int C, cudaStream_t st)
-{
-    if (a.type == KV_F32) return launch_hb<true, 8, WARPS>(a, units, C, st);
-    return rows == 8 ? launch_hb<false, 8, WARPS>(a, units, C, st) : launch_hb<false, 16, WARPS>(a, units, C, st);
 }
 
 cudaError_t launch_kv_attn_split(const KvAttn &a0, int max_rows, int max_len, cudaStream_t st)
 {
     KvAttn a = a0;
+    const bool split = a.type == KV_F32;
     const long long q = (long long)std::max(max_rows, 1) * a.mul;
-    const int rows = a.type == KV_F32 || q <= 8 ? 8 : 16;
+    const int nt = q <= sp_rows(split, 1) ? 1 : 2, rows = sp_rows(split, nt), slots = 148 * sp_resident(nt);
     a.tiles = (int)std::min<long long>((q + rows - 1) / rows, 1 << 16);
-    const long long units = (long long)a.n_runs * a.c.n_kv * a.tiles;
-    const int pages = std::max(1, max_len / KV_PAGE + (max_len % KV_PAGE != 0));
+    const long long units = (long long)a.n_runs * a.c.n_kv * a.tiles, halves = std::max(1, max_len / SP_TOK + (max_len % SP_TOK != 0));
     if (units > (1ll << 26)) return cudaErrorInvalidValue;
-    // Few units and many pages: twelve warps a CTA, one CTA an SM, up to 16 CTAs a
-    // cluster.  Else four warps, three CTAs an SM, up to 8.
-    const bool wide = units * 8 < 296 && pages >= 24;
-    const int warps = wide ? 12 : 4, most = wide ? 16 : 8, want = wide ? 148 : 444;
+    // Many pages: streamed, one CTA for each of the SMs' slots.  Else a cluster a
+    // unit, up to 8 CTAs while each warp has half a page.
+    const bool stream = (long long)a.n_runs * a.tiles <= SP_MAX_ENTRIES && units * halves >= 4ll * slots * SP_WARPS;
     int C = 1;
-    while (C < most && units * C < want && C * 2 * warps <= pages) C *= 2;
-    return wide ? launch_rows<12>(a, rows, (int)units, C, st) : launch_rows<4>(a, rows, (int)units, C, st);
+    while (!stream && C < 8 && units * C < slots && C * 2 * SP_WARPS <= halves) C *= 2;
+    const int u = (int)units;
+    if (stream)
+        return split ? nt == 1 ? launch_hb<true, 1, true>(a, u, C, st) : launch_hb<true, 2, true>(a, u, C, st)
+               : nt == 1 ? launch_hb<false, 1, true>(a, u, C, st) : launch_hb<false, 2, true>(a, u, C, st);
+    return split ? nt == 1 ? launch_hb<true, 1, false>(a, u, C, st) : launch_hb<true, 2, false>(a, u, C, st)
+           : nt == 1 ? launch_hb<false, 1, false>(a, u, C, st) : launch_hb<false, 2, false>(a, u, C, st);
 }
 
 } // namespace cats
