@@ -20,23 +20,31 @@ struct KvAttn {
 // four bits up) is 1024 + code (64 + code) exactly; the difference is exact
 // and so is the product (the scale has 8 significant bits).
 struct KvMagic {
-    uint32_t e1024, e64;
+    uint32_t low, high, e1024, e64;
 };
 __device__ __forceinline__ KvMagic kv_magic()
 {
-    KvMagic m;   // in registers for good: an instruction takes one immediate, which is the mask
+    KvMagic m;   // in registers for good
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(m.low));
+    asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(m.high));
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m.e1024));
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(m.e64));
     return m;
+}
+__device__ __forceinline__ uint32_t kv_and_or(uint32_t v, uint32_t mask, uint32_t bits)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));   // (v & mask) | bits
+    return r;
 }
 __device__ __forceinline__ void kv_dequant(uint32_t w, __half2 s, const KvMagic &mg, uint32_t (&x)[4])
 {
     const uint32_t w8 = w >> 8;
     uint32_t t[4];
-    t[0] = (w & 0x000f000fu) | mg.e1024;
-    t[1] = (w & 0x00f000f0u) | mg.e64;
-    t[2] = (w8 & 0x000f000fu) | mg.e1024;
-    t[3] = (w8 & 0x00f000f0u) | mg.e64;
+    t[0] = kv_and_or(w, mg.low, mg.e1024);
+    t[1] = kv_and_or(w, mg.high, mg.e64);
+    t[2] = kv_and_or(w8, mg.low, mg.e1024);
+    t[3] = kv_and_or(w8, mg.high, mg.e64);
     const __half2 b0 = __half2half2(__ushort_as_half(0x6408)), b1 = __half2half2(__ushort_as_half(0x5480));   // 1032, 72
 #pragma unroll
     for (int i = 0; i < 4; i++) {

@@ -22,7 +22,6 @@
 // 8-15 of the same instruction (22 bits, no second product).  fp16 and bf16
 // rows use the 16 rows for 16 queries, or 8 when that is enough.
 #include "kv_attn.cuh"
-#include "tc.cuh"
 #include <algorithm>
 #include <climits>
 #include <cooperative_groups.h>
@@ -38,7 +37,12 @@ constexpr float SP_P_BITS = 15.f;   // probabilities are held times 2^15: fp16 k
 
 // a stage: K codes [32 tokens], V codes, K scales, V scales
 __host__ __device__ constexpr int sp_stage(int hb) { return 1152 * hb; }
-__host__ __device__ constexpr size_t sp_smem(int hb) { return (size_t)SP_WARPS * SP_STAGES * (sp_stage(hb) + 8); }   // rings | barriers
+__host__ __device__ constexpr size_t sp_smem(int hb) { return (size_t)SP_WARPS * SP_STAGES * sp_stage(hb); }   // the warps' rings
+
+__device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
 template <int HB> struct Words {
     uint32_t w[HB];
@@ -130,19 +134,11 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
     // at the end a warp's rows take its ring, then the CTA's joined rows that of warp 0
     static_assert(ROWS * (HS + 2) * 4 <= SP_STAGES * STAGE, "");
     float *joined = reinterpret_cast<float *>(smem);   // [ROWS][HS], m[ROWS], l[ROWS]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (size_t)WARPS * SP_STAGES * STAGE);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     cg::cluster_group cl = cg::this_cluster();
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     uint8_t *ring = smem + (size_t)warp * SP_STAGES * STAGE;
-    uint64_t *bar = bars + warp * SP_STAGES;
-    if (lane == 0) {
-        for (int i = 0; i < SP_STAGES; i++) mbar_init(&bar[i], 1);
-        fence_barrier_init();
-    }
-    __syncwarp();
-    uint32_t phase = 0;    // a bit a stage
-    bool broken = false;   // a wait gave up (recorded): no copy is issued any more, the rows are NaN
+    const uint32_t ring_at = smem_u32(ring) + lane * 16;
     const KvMagic magic = kv_magic();
 
     int ri, kvh, entry = 0, at = 0, steps = 0;   // STREAM: entry = run * tiles + tile; steps at .. of it come next
@@ -359,21 +355,26 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
         const int mine = first < n_tiles ? (n_tiles - first + step - 1) / step : 0;
         auto look = [&](int i) { return i < mine ? a.c.page(run.seq, (first + i * step) / 2) : -1; };
         int pages = look(lane), ahead = mine > 32 ? look(32 + lane) : -1;   // of i's group of 32, and the next
+        // half page i into stage st: every lane brings 16 bytes a copy
+        const uint8_t *base = a.c.pool + (size_t)kvh * (72 * HS) + lane * 16;
+        const int scales = lane < 4 * HB ? kv_k_scales(HS) : kv_v_scales(HS) - 64 * HB;
         auto issue = [&](int i, int page, int st) {
-            if (page >= 0 && lane == 0) {
+            if (page >= 0) {
                 const int half = (first + i * step) & 1;
-                const uint8_t *src = a.c.chunk(page, kvh);
-                uint8_t *dst = ring + st * STAGE;
-                mbar_arrive_expect_tx(&bar[st], STAGE);
-                bulk_g2s_keep(dst, src + half * 16 * HS, 16 * HS, &bar[st]);
-                bulk_g2s_keep(dst + 16 * HS, src + kv_v_codes(HS) + half * 16 * HS, 16 * HS, &bar[st]);
-                bulk_g2s_keep(dst + 32 * HS, src + kv_k_scales(HS) + half * 2 * HS, 2 * HS, &bar[st]);
-                bulk_g2s_keep(dst + 34 * HS, src + kv_v_scales(HS) + half * 2 * HS, 2 * HS, &bar[st]);
-            }
-        };
-        int here[SP_STAGES];   // pages in the ring, the next one to use first
+                const uint8_t *src = base + (size_t)page * a.c.page_bytes + half * 16 * HS;
+                const uint32_t dst = ring_at + st * STAGE;
 #pragma unroll
-        for (int i = 0; i < SP_STAGES; i++) {
+                for (int k = 0; k < HB; k++) {
+                    cp16(dst + 512 * k, src + 512 * k);
+                    cp16(dst + 16 * HS + 512 * k, src + kv_v_codes(HS) + 512 * k);
+                }
+                if (lane < 8 * HB) cp16(dst + 32 * HS, src + scales - half * 14 * HS);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int here[SP_STAGES - 1];   // pages in the ring, the next one to use first
+#pragma unroll
+        for (int i = 0; i < SP_STAGES - 1; i++) {
             here[i] = __shfl_sync(0xffffffffu, pages, i);
             issue(i, here[i], i);
         }
@@ -499,31 +500,27 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
 
         int st = 0;
         for (int i = 0; i < mine; i++) {
-            const int page = here[0], p0 = (first + i * step) * SP_TOK;
-            if (page >= 0) {
-                const bool ok = mbar_wait_bounded(&bar[st], phase >> st & 1, a.c.err, CATS_DEVERR_MBAR_FULL);
-                if (!__all_sync(0xffffffffu, ok)) broken = true;
-                phase ^= 1u << st;
-            }
-            if (page >= 0 && !broken) {
-                if (p0 + SP_TOK - 1 > low) take(ring + st * STAGE, p0, std::true_type{});
-                else take(ring + st * STAGE, p0, std::false_type{});
-            }
-            __syncwarp();   // every lane has read this stage
-            const int nx = i + SP_STAGES;
+            const int page = here[0], p0 = (first + i * step) * SP_TOK, nx = i + SP_STAGES - 1;
             if ((nx & 31) == 0) {   // nx starts the next group of 32
                 pages = ahead;
                 ahead = nx + 32 < mine ? look(nx + 32 + lane) : -1;
             }
 #pragma unroll
-            for (int k = 0; k + 1 < SP_STAGES; k++) here[k] = here[k + 1];
-            const int next = __shfl_sync(0xffffffffu, pages, nx & 31);
-            here[SP_STAGES - 1] = broken ? -1 : next;
-            issue(nx, here[SP_STAGES - 1], st);
+            for (int k = 0; k + 2 < SP_STAGES; k++) here[k] = here[k + 1];
+            here[SP_STAGES - 2] = __shfl_sync(0xffffffffu, pages, nx & 31);
+            asm volatile("cp.async.wait_group %0;" ::"n"(SP_STAGES - 2) : "memory");
+            __syncwarp();   // every lane's copies of this stage are there, and all are done with the last one
+            issue(nx, here[SP_STAGES - 2], st == 0 ? SP_STAGES - 1 : st - 1);
+            if (page >= 0) {
+                if (p0 + SP_TOK - 1 > low) take(ring + st * STAGE, p0, std::true_type{});
+                else take(ring + st * STAGE, p0, std::false_type{});
+            }
             st = st + 1 == SP_STAGES ? 0 : st + 1;
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
 
-        // ---- the warp's rows to its own ring (its copies are all consumed)
+        // ---- the warp's rows to its own ring
         float *part = reinterpret_cast<float *>(ring);   // [ROWS][HS], m[ROWS], l[ROWS]
 #pragma unroll
         for (int i = 0; i < NS; i++) {
@@ -531,7 +528,6 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
             l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
-            if (broken) l[i] = NAN;
             if (g == 0) {
                 part[ROWS * HS + r] = m[i];
                 part[ROWS * HS + ROWS + r] = l[i];
@@ -601,7 +597,6 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 }
             }
             at += now;
-            fence_proxy_async_smem();
             __syncthreads();   // the next unit's copies may overwrite the rows
         } else {
             if (C > 1) cl.sync();
@@ -626,7 +621,6 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 }
                 finish4(a, run, span, kvh, tile * ROWS + r, e4, acc, ll);
             }
-            fence_proxy_async_smem();
             if (C > 1) cl.sync();   // nobody's rows are read any more
             else __syncthreads();
             tile += a.tiles;
