@@ -102,9 +102,9 @@ __device__ __forceinline__ int steps_of(const KvAttn &a, const KvRun &run, const
     return max(1, (int)((halves + SP_WARPS - 1) / SP_WARPS));
 }
 
-// What a streamed call keeps between its two kernels: per CTA the unit that
-// begins in it and goes on in others ((entry, kv head, parts, 0)), and two
-// partial results: of the unit it began with (0) and of the one it ended in (1).
+// What a streamed call keeps between its two kernels, two to a CTA: the unit
+// it went on with (0) and the one that begins in it and goes on in others (1),
+// (entry, kv head, CTA it begins in, CTAs; 0 = none), and their partial rows.
 struct SpWork {
     int4 *split;
     float *part;
@@ -191,7 +191,8 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
         const int per = max(1, steps_of(a, r, kv_run_rows(r, a.q.rows, nullptr), tile, ROWS));
         kvh = (int)(into / per);
         at = (int)(into % per);
-        if (tid == 0) wk.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (tid < 2) wk.split[2 * blockIdx.x + tid] = make_int4(0, 0, 0, 0);
+        pdl_launch_dependents();   // (it waits for this kernel's end by itself)
         __syncthreads();
     } else {
         const int unit = blockIdx.x / C;
@@ -273,6 +274,36 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
         int n_tiles = top < 0 ? 0 : top / SP_TOK + 1;   // (a streamed CTA's end of them)
         if (STREAM) n_tiles = min(n_tiles, (at + now) * WARPS);
 
+        // this warp's half pages: first, first + step, ...; lane j keeps the page of
+        // the 32 k + j th
+        const int first = (STREAM ? at : rank) * WARPS + warp, step = STREAM ? WARPS : C * WARPS;
+        const int mine = first < n_tiles ? (n_tiles - first + step - 1) / step : 0;
+        auto look = [&](int i) { return i < mine ? a.c.page(run.seq, (first + i * step) / 2) : -1; };
+        int pages = look(lane), ahead = mine > 32 ? look(32 + lane) : -1;   // of i's group of 32, and the next
+        // half page i into stage st: every lane brings 16 bytes a copy
+        const uint8_t *base = a.c.pool + (size_t)kvh * (72 * HS) + lane * 16;
+        const int scales = lane < 4 * HB ? kv_k_scales(HS) : kv_v_scales(HS) - 64 * HB;
+        auto issue = [&](int i, int page, int st) {
+            if (page >= 0) {
+                const int half = (first + i * step) & 1;
+                const uint8_t *src = base + (size_t)page * a.c.page_bytes + half * 16 * HS;
+                const uint32_t dst = ring_at + st * STAGE;
+#pragma unroll
+                for (int k = 0; k < HB; k++) {
+                    cp16(dst + 512 * k, src + 512 * k);
+                    cp16(dst + 16 * HS + 512 * k, src + kv_v_codes(HS) + 512 * k);
+                }
+                if (lane < 8 * HB) cp16(dst + 32 * HS, src + scales - half * 14 * HS);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int here[SP_STAGES - 1];   // pages in the ring, the next one to use first
+#pragma unroll
+        for (int i = 0; i < SP_STAGES - 1; i++) {
+            here[i] = __shfl_sync(0xffffffffu, pages, i);
+            issue(i, here[i], i);
+        }
+
         // Queries as B fragments (column g).  Word (c, b) of a key holds elements
         // 8c + {0..7} of block b, element e in nibble e.
         // 16 bits: the words masked with 000f000f (00f000f0) read as the fp16
@@ -347,36 +378,6 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
         for (int i = 0; i < NS; i++) {
             m[i] = -INFINITY;
             l[i] = 0.f;
-        }
-
-        // this warp's half pages: first, first + step, ...; lane j keeps the page of
-        // the 32 k + j th
-        const int first = (STREAM ? at : rank) * WARPS + warp, step = STREAM ? WARPS : C * WARPS;
-        const int mine = first < n_tiles ? (n_tiles - first + step - 1) / step : 0;
-        auto look = [&](int i) { return i < mine ? a.c.page(run.seq, (first + i * step) / 2) : -1; };
-        int pages = look(lane), ahead = mine > 32 ? look(32 + lane) : -1;   // of i's group of 32, and the next
-        // half page i into stage st: every lane brings 16 bytes a copy
-        const uint8_t *base = a.c.pool + (size_t)kvh * (72 * HS) + lane * 16;
-        const int scales = lane < 4 * HB ? kv_k_scales(HS) : kv_v_scales(HS) - 64 * HB;
-        auto issue = [&](int i, int page, int st) {
-            if (page >= 0) {
-                const int half = (first + i * step) & 1;
-                const uint8_t *src = base + (size_t)page * a.c.page_bytes + half * 16 * HS;
-                const uint32_t dst = ring_at + st * STAGE;
-#pragma unroll
-                for (int k = 0; k < HB; k++) {
-                    cp16(dst + 512 * k, src + 512 * k);
-                    cp16(dst + 16 * HS + 512 * k, src + kv_v_codes(HS) + 512 * k);
-                }
-                if (lane < 8 * HB) cp16(dst + 32 * HS, src + scales - half * 14 * HS);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        int here[SP_STAGES - 1];   // pages in the ring, the next one to use first
-#pragma unroll
-        for (int i = 0; i < SP_STAGES - 1; i++) {
-            here[i] = __shfl_sync(0xffffffffu, pages, i);
-            issue(i, here[i], i);
         }
 
         // 32 tokens from p0 on; EDGE: some of them lie past some row's last position
@@ -566,106 +567,118 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 acc[k].x += f * v.x; acc[k].y += f * v.y; acc[k].z += f * v.z; acc[k].w += f * v.w;
             }
         }
-        __syncthreads();
+        if (STREAM && now < steps) {
+            float *dst = wk.part + (size_t)(2 * blockIdx.x + (at == 0)) * sp_part(ROWS, HS);
 #pragma unroll
-        for (int k = 0; k < ITEMS; k++) {
-            const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
-            if (r >= ROWS) continue;
-            *reinterpret_cast<float4 *>(joined + r * HS + 4 * e4) = acc[k];
-            if (e4 == 0) {
-                joined[ROWS * HS + r] = ml[k].x;
-                joined[ROWS * HS + ROWS + r] = ml[k].y;
+            for (int k = 0; k < ITEMS; k++) {
+                const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
+                if (r >= ROWS) continue;
+                *reinterpret_cast<float4 *>(dst + r * HS + 4 * e4) = acc[k];
+                if (e4 == 0) {
+                    dst[ROWS * HS + r] = ml[k].x;
+                    dst[ROWS * HS + ROWS + r] = ml[k].y;
+                }
+            }
+            if (tid == 0) {
+                const long long start = total * (blockIdx.x + 1) / gridDim.x - left - now - at;   // the unit's first step
+                const int owner = (int)(((start + 1) * gridDim.x - 1) / total);
+                const int last = (int)(((start + steps) * gridDim.x - 1) / total);
+                wk.split[2 * blockIdx.x + (at == 0)] = make_int4(entry, kvh, owner, last - owner + 1);
+            }
+        } else if (STREAM || C == 1) {
+#pragma unroll
+            for (int k = 0; k < ITEMS; k++) {
+                const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
+                if (r < used) finish4(a, run, span, kvh, tile * ROWS + r, e4, acc[k], ml[k].y);
             }
         }
+        __syncthreads();   // the warps' rows are read: the rings are free
         if constexpr (STREAM) {
-            __syncthreads();
-            if (now == steps) {
-                for (int i = tid; i < used * (HS / 4); i += WARPS * 32) {
-                    const int r = i / (HS / 4), e4 = i % (HS / 4);
-                    finish4(a, run, span, kvh, tile * ROWS + r, e4, *reinterpret_cast<const float4 *>(joined + r * HS + 4 * e4),
-                            joined[ROWS * HS + ROWS + r]);
-                }
-            } else {
-                float *dst = wk.part + (size_t)(2 * blockIdx.x + (at == 0)) * sp_part(ROWS, HS);
-                for (int i = tid; i < sp_part(ROWS, HS) / 2; i += WARPS * 32)
-                    reinterpret_cast<float2 *>(dst)[i] = reinterpret_cast<const float2 *>(joined)[i];
-                if (at == 0 && tid == 0) {
-                    // the unit begins here: the last CTA that has steps of it
-                    const long long end = begin + (total * (blockIdx.x + 1) / gridDim.x - begin) - now + steps;
-                    const int last = (int)((end * gridDim.x - 1) / total);
-                    wk.split[blockIdx.x] = make_int4(entry, kvh, last - (int)blockIdx.x + 1, 0);
-                }
-            }
             at += now;
-            __syncthreads();   // the next unit's copies may overwrite the rows
         } else {
-            if (C > 1) cl.sync();
-            else __syncthreads();
-            // ---- the cluster's CTAs joined, and the rows stored
-            for (int i = rank * WARPS * 32 + tid; i < used * (HS / 4); i += C * WARPS * 32) {
-                const int r = i / (HS / 4), e4 = i % (HS / 4);
-                float4 acc = *reinterpret_cast<const float4 *>(joined + r * HS + 4 * e4);
-                float ll = joined[ROWS * HS + ROWS + r];
-                if (C > 1) {
-                    float mm = -INFINITY;
-                    for (int k = 0; k < C; k++) mm = fmaxf(mm, cl.map_shared_rank(joined, k)[ROWS * HS + r]);
-                    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    ll = 0.f;
-                    for (int k = 0; k < C; k++) {
-                        const float *p = cl.map_shared_rank(joined, k);
-                        const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - mm);
-                        const float4 v = *reinterpret_cast<const float4 *>(p + r * HS + 4 * e4);
-                        ll += f * p[ROWS * HS + ROWS + r];
-                        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+            if (C > 1) {
+#pragma unroll
+                for (int k = 0; k < ITEMS; k++) {
+                    const int i = tid + k * WARPS * 32, r = i / (HS / 4), e4 = i % (HS / 4);
+                    if (r >= ROWS) continue;
+                    *reinterpret_cast<float4 *>(joined + r * HS + 4 * e4) = acc[k];
+                    if (e4 == 0) {
+                        joined[ROWS * HS + r] = ml[k].x;
+                        joined[ROWS * HS + ROWS + r] = ml[k].y;
                     }
                 }
-                finish4(a, run, span, kvh, tile * ROWS + r, e4, acc, ll);
+                cl.sync();
+            }
+            // ---- the cluster's CTAs joined, and the rows stored
+            for (int i = rank * WARPS * 32 + tid; C > 1 && i < used * (HS / 4); i += C * WARPS * 32) {
+                const int r = i / (HS / 4), e4 = i % (HS / 4);
+                float mm = -INFINITY;
+                for (int k = 0; k < C; k++) mm = fmaxf(mm, cl.map_shared_rank(joined, k)[ROWS * HS + r]);
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                float ll = 0.f;
+                for (int k = 0; k < C; k++) {
+                    const float *p = cl.map_shared_rank(joined, k);
+                    const float mw = p[ROWS * HS + r], f = mw == -INFINITY ? 0.f : kv_exp2(mw - mm);
+                    const float4 v = *reinterpret_cast<const float4 *>(p + r * HS + 4 * e4);
+                    ll += f * p[ROWS * HS + ROWS + r];
+                    sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+                }
+                finish4(a, run, span, kvh, tile * ROWS + r, e4, sum, ll);
             }
             if (C > 1) cl.sync();   // nobody's rows are read any more
-            else __syncthreads();
             tile += a.tiles;
         }
     }
-    if (STREAM) pdl_launch_dependents();
 }
 
-// The units that lie in several CTAs' stretches: blockIdx.x is the CTA one
-// begins in, blockIdx.y its row; eight groups of threads take every eighth
-// part and are joined in their order.
+// The units that lie in several CTAs' stretches.  Block i looks at CTA i's two:
+// as the k-th of a unit's P CTAs it joins rows k, k + P, ...: a warp a row, or,
+// past eight parts, the row its warps share, every eighth part each.
 template <int ROWS>
-__global__ void __launch_bounds__(256) k_kv_attn_join(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork wk)
+__global__ void __launch_bounds__(256, 4) k_kv_attn_join(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork wk)
 {
     __shared__ float4 so[8][32];
     __shared__ float2 sm[8];
     pdl_wait();
-    const int4 sp = wk.split[blockIdx.x];
-    const int r = blockIdx.y, x = threadIdx.x & 31, y = threadIdx.x >> 5, hs = a.c.hs;
-    if (sp.z == 0) return;
-    const KvRun run = a.runs[sp.x / a.tiles];
-    const int2 span = kv_run_rows(run, a.q.rows, nullptr);
-    const long long rr = (long long)(sp.x % a.tiles) * ROWS + r;
-    if (rr >= (long long)(span.y - span.x) * a.mul) return;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float mp, float lp, const float4 &v) {
-        const float mn = fmaxf(m, mp);
-        const float f = m == -INFINITY ? 0.f : kv_exp2(m - mn), g = mp == -INFINITY ? 0.f : kv_exp2(mp - mn);
-        m = mn;
-        l = l * f + lp * g;
-        acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
-    };
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, hs = a.c.hs;
+    for (int slot = 0; slot < 2; slot++) {
+        const int4 sp = wk.split[2 * blockIdx.x + slot];
+        if (sp.w == 0) continue;
+        const int owner = sp.z, P = sp.w, k0 = (int)blockIdx.x - owner;
+        const bool shared = P > 8;
+        const int r = shared ? k0 : k0 + P * y;
+        if (shared ? r >= ROWS : false) continue;
+        const KvRun run = a.runs[sp.x / a.tiles];
+        const int2 span = kv_run_rows(run, a.q.rows, nullptr);
+        const long long rr = (long long)(sp.x % a.tiles) * ROWS + r;
+        const bool real = r < ROWS && rr < (long long)(span.y - span.x) * a.mul;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float mp, float lp, const float4 &v) {
+            const float mn = fmaxf(m, mp);
+            const float f = m == -INFINITY ? 0.f : kv_exp2(m - mn), g = mp == -INFINITY ? 0.f : kv_exp2(mp - mn);
+            m = mn;
+            l = l * f + lp * g;
+            acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
+        };
+        if (real) {
 #pragma unroll 4
-    for (int k = y; k < sp.z; k += 8) {
-        const float *p = wk.part + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * sp_part(ROWS, hs);
-        const float4 v = 4 * x < hs ? *reinterpret_cast<const float4 *>(p + r * hs + 4 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
-        add(p[ROWS * hs + r], p[ROWS * hs + ROWS + r], v);
+            for (int k = shared ? y : 0; k < P; k += shared ? 8 : 1) {
+                const float *p = wk.part + (size_t)(2 * (owner + k) + (k == 0)) * sp_part(ROWS, hs);
+                const float4 v = 4 * x < hs ? *reinterpret_cast<const float4 *>(p + r * hs + 4 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
+                add(p[ROWS * hs + r], p[ROWS * hs + ROWS + r], v);
+            }
+        }
+        if (shared) {
+            __syncthreads();   // the slot before is done with them
+            so[y][x] = acc;
+            if (x == 0) sm[y] = make_float2(m, l);
+            __syncthreads();
+            if (y > 0) continue;
+            for (int k = 1; k < 8; k++) add(sm[k].x, sm[k].y, so[k][x]);
+        }
+        if (real && 4 * x < hs) finish4(a, run, span, sp.y, rr, x, acc, l);
     }
-    so[y][x] = acc;
-    if (x == 0) sm[y] = make_float2(m, l);
-    __syncthreads();
-    if (y > 0 || 4 * x >= hs) return;
-    for (int k = 1; k < min(8, sp.z); k++) add(sm[k].x, sm[k].y, so[k][x]);
-    finish4(a, run, span, sp.y, rr, x, acc, l);
 }
 
 // The partial results of a streamed call live in memory of the call's own,
@@ -720,7 +733,7 @@ static cudaError_t launch_one(const KvAttn &a, int units, int C, cudaStream_t st
         return cudaLaunchKernelEx(&cfg, k, a, wk);
     }
     const int grid = 148 * sp_resident(NT);
-    const size_t split = round_up((size_t)grid * sizeof(int4), 256), part = (size_t)grid * 2 * sp_part(ROWS, 32 * HB) * 4;
+    const size_t split = round_up((size_t)grid * 2 * sizeof(int4), 256), part = (size_t)grid * 2 * sp_part(ROWS, 32 * HB) * 4;
     cudaMemPool_t pool = work_pool();
     uint8_t *p = nullptr;
     if (!pool) return cudaErrorMemoryAllocation;
@@ -734,7 +747,7 @@ static cudaError_t launch_one(const KvAttn &a, int units, int C, cudaStream_t st
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.numAttrs = 1;
-        cfg.gridDim = dim3(grid, ROWS);
+        cfg.gridDim = dim3(grid);
         cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = 0;
         e = cudaLaunchKernelEx(&cfg, k_kv_attn_join<ROWS>, a, wk);
