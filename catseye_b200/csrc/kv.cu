@@ -109,59 +109,6 @@ cudaError_t launch_kv_read(const KvView &c, int type, const KvRows &k, const KvR
 }
 
 // -------------------------------------------------------------- attention
-// One warp per (row, query head): its positions in order, an online softmax,
-// each lane four elements of the head.
-template <class T>
-__global__ void __launch_bounds__(128) k_kv_attn_simple(const __grid_constant__ KvView c,
-                                                        const __grid_constant__ KvRows out,
-                                                        const __grid_constant__ KvRows q,
-                                                        const KvRun *__restrict__ runs, int n_runs, int n_heads)
-{
-    const int lane = threadIdx.x & 31, mul = n_heads / c.n_kv;
-    const float scale = 1.f / sqrtf((float)c.hs);
-    const bool mine = 4 * lane < c.hs;
-    for (int ri = blockIdx.y; ri < n_runs; ri += gridDim.y) {
-        const KvRun run = runs[ri];
-        const int2 span = kv_run_rows(run, q.rows, c.err);
-        const long long items = (long long)(span.y - span.x) * n_heads;
-        for (long long i = blockIdx.x * 4LL + (threadIdx.x >> 5); i < items; i += gridDim.x * 4LL) {
-            const int r = span.x + (int)(i / n_heads), h = (int)(i % n_heads), row = run.first + r;
-            // positions past the table's end hold nothing: such a row sees nothing
-            long long at = (long long)run.pos + r;
-            if (at >= (long long)c.max_pages * KV_PAGE || run.seq < 0 || run.seq >= c.n_seqs) {
-                if (c.err) atomicOr(c.err, CATS_DEVERR_PAGE_RANGE);
-                at = -1;
-            }
-            const int pos = (int)at;
-            float x[4] = {0.f, 0.f, 0.f, 0.f}, o[4] = {0.f, 0.f, 0.f, 0.f};
-            if (mine) load4<T>(static_cast<const T *>(q.p) + (size_t)row * q.ld + (size_t)h * c.hs + 4 * lane, q.vec, x);
-            float m = -INFINITY, l = 0.f;
-            for (int t = 0; t <= pos; t++) {
-                const int page = c.page(run.seq, t / KV_PAGE);
-                if (page < 0) continue;
-                const uint8_t *ch = c.chunk(page, h / mul);
-                float4 kk = make_float4(0.f, 0.f, 0.f, 0.f), vv = kk;
-                if (mine) {
-                    kk = kv_load4(ch, false, c.hs, t % KV_PAGE, lane);
-                    vv = kv_load4(ch, true, c.hs, t % KV_PAGE, lane);
-                }
-                const float s = warp_sum(x[0] * kk.x + x[1] * kk.y + x[2] * kk.z + x[3] * kk.w) * scale;
-                const float mn = fmaxf(m, s), a = m == -INFINITY ? 0.f : expf(m - mn), p = expf(s - mn);
-                l = l * a + p;
-                o[0] = o[0] * a + p * vv.x;
-                o[1] = o[1] * a + p * vv.y;
-                o[2] = o[2] * a + p * vv.z;
-                o[3] = o[3] * a + p * vv.w;
-                m = mn;
-            }
-            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[j] *= inv;
-            if (mine) store4<T>(static_cast<T *>(out.p) + (size_t)row * out.ld + (size_t)h * c.hs + 4 * lane, out.vec, o);
-        }
-    }
-}
-
 cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, const KvRows &q, int n_heads,
                                 const KvBatch &b, cudaStream_t st)
 {
@@ -175,16 +122,7 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
     a.n_heads = n_heads;
     a.mul = n_heads / c.n_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hs);
-    if ((long long)b.max_rows * a.mul <= 128) return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
-    const long long items = (long long)std::max(b.max_rows, 1) * n_heads;
-    const dim3 grid((unsigned)std::min<long long>((items + 3) / 4, 65535), (unsigned)std::min(b.n_runs, 32768));
-    switch (type) {
-    case KV_F32: k_kv_attn_simple<float><<<grid, 128, 0, st>>>(c, out, q, b.runs, b.n_runs, n_heads); break;
-    case KV_F16: k_kv_attn_simple<__half><<<grid, 128, 0, st>>>(c, out, q, b.runs, b.n_runs, n_heads); break;
-    case KV_BF16: k_kv_attn_simple<__nv_bfloat16><<<grid, 128, 0, st>>>(c, out, q, b.runs, b.n_runs, n_heads); break;
-    default: return cudaErrorInvalidValue;
-    }
-    return cudaGetLastError();
+    return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
 }
 
 // ------------------------------------------------------------- page copies
