@@ -122,6 +122,7 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
     a.n_heads = n_heads;
     a.mul = n_heads / c.n_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hs);
+    if (kv_attn_tile_takes(a, b.max_rows)) return launch_kv_attn_tile(a, b.max_rows, st);
     return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
 }
 

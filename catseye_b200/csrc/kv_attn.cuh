@@ -214,6 +214,8 @@ static __device__ __noinline__ float4 kv_plain_row4(const KvAttn &a, int seq, in
     return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
+bool kv_attn_tile_takes(const KvAttn &a, int max_rows);
+cudaError_t launch_kv_attn_tile(const KvAttn &a, int max_rows, cudaStream_t st);
 cudaError_t launch_kv_attn_split(const KvAttn &a, int max_rows, int max_len, cudaStream_t st);
 
 } // namespace cats

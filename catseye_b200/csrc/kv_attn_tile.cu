@@ -1,0 +1,490 @@
+// kv_attn_tile.cu — attention over the paged Q4_0 cache for many query rows
+// (prompts), 16-bit rows, on the 5th-generation tensor cores.
+//
+// A CTA takes 256 query rows of a kv head (tokens x the query heads that share
+// it) as two tiles of 128, and goes through the sequence 128 tokens at a time:
+//   S_i = Q_i K^T      tcgen05, A and B in shared memory, S (fp32) in TMEM
+//   P_i = 2^(S - m)    a thread a row: no shuffles; written over S as fp16
+//   O_i += P_i V       A = P in TMEM, B = V in shared memory, O in TMEM
+// with the running maximum m and sum of a softmax per row.  The two tiles take
+// turns: while one's probabilities are computed the other's products run.
+//
+// Roles: warps 0-3 and 4-7 the rows of the two tiles (they also bring Q in and
+// store O), warps 8-11 dequantize the cache's codes into the products' operand
+// layout (128-byte swizzle, two stages), warp 12 issues the products.  The
+// codes are read once per 256 rows; the values (code - 8) * scale are exact in
+// fp16 (kv.cuh), so the products' operands are the cache's values.
+//
+// Bound by the exponentials and the tensor cores alike: a 128 x 128 tile costs
+// 1024 cycles of both (16 exponentials a cycle; 2 x 512 cycles of products).
+// So the accumulator is not rescaled for every new maximum: m is only moved
+// when a row's maximum passes it by 2^8, which happens once or twice a row.
+//
+// Every wait is bounded; TMEM is freed on every path.
+#include "kv_attn.cuh"
+#include "tc.cuh"
+#include <algorithm>
+#include <climits>
+
+namespace cats {
+
+constexpr int TI_ROWS = 256, TI_KV = 128;
+constexpr int TI_SOFT = 8, TI_DEQ = 4, TI_MMA_WARP = TI_SOFT + TI_DEQ, TI_THREADS = (TI_MMA_WARP + 1) * 32;
+constexpr float TI_P_BITS = 7.f, TI_LAG = 8.f;   // probabilities are held times 2^7 and may reach 2^15
+
+// shared memory, from a 1024-byte boundary: Q [2][HS/64][128 rows][128 B], K the
+// same per stage, V [2 pages][HS rows][128 B] per stage, barriers
+template <int HS> struct TileSmem {
+    static constexpr int SLICE = 128 * 128;                  // 128 rows of 64 halves
+    static constexpr int Q_TILE = HS / 64 * SLICE, K_STAGE = HS / 64 * SLICE, V_PAGE = HS * 128, V_STAGE = 2 * V_PAGE;
+    static constexpr int K = 2 * Q_TILE, V = K + 2 * K_STAGE, BAR = V + 2 * V_STAGE;
+    static constexpr int BYTES = BAR + 256 + 1024;           // + the alignment's slack
+};
+
+enum TileBar { B_Q, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_O = B_P + 2, B_N = B_O + 2 };
+
+__device__ __forceinline__ void ti_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"(acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void ti_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+        "r"(acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void ti_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void ti_ld32(uint32_t (&v)[32], uint32_t addr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void ti_st16(uint32_t addr, const uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void ti_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ti_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int HS>
+__global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_constant__ KvAttn a)
+{
+    using L = TileSmem<HS>;
+    constexpr int HB = HS / 32;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::BAR);
+    volatile int *abort_s = reinterpret_cast<volatile int *>(bar + B_N);
+    volatile int *hole = abort_s + 1;   // [4], by KV tile: pages of it that do not exist (bit 0, 1)
+    uint32_t *slot = const_cast<uint32_t *>(reinterpret_cast<volatile uint32_t *>(abort_s + 5));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    if (tid == 0) {
+        mbar_init(&bar[B_Q], TI_SOFT);
+        for (int s = 0; s < 2; s++) {
+            mbar_init(&bar[B_KF + s], TI_DEQ);
+            mbar_init(&bar[B_KE + s], 1);
+            mbar_init(&bar[B_VF + s], TI_DEQ);
+            mbar_init(&bar[B_VE + s], 1);
+            mbar_init(&bar[B_S + s], 1);
+            mbar_init(&bar[B_P + s], TI_SOFT / 2);
+            mbar_init(&bar[B_O + s], 1);
+        }
+        *abort_s = 0;
+        fence_barrier_init();
+    }
+    if (warp == TI_MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;   // S_0, S_1 (128 columns each; P_i over the first 64 of S_i), O_0, O_1
+
+    const int kvh = blockIdx.y;
+    const KvRun run = a.runs[blockIdx.z];
+    const int2 span = kv_run_rows(run, a.q.rows, blockIdx.x == 0 && kvh == 0 ? a.c.err : nullptr);
+    const long long n_q = (long long)(span.y - span.x) * a.mul;
+    const long long cap = (long long)a.c.max_pages * KV_PAGE;
+    const bool seq_ok = run.seq >= 0 && run.seq < a.c.n_seqs;
+
+    // counts of waits on each barrier so far: their parities
+    uint32_t kv_it = 0, q_it = 0, s_it[2] = {0, 0}, o_it[2] = {0, 0};
+
+    // the longest tiles (the last ones) first
+    const long long mine = n_q > 0 ? (n_q + TI_ROWS - 1) / TI_ROWS : 0;
+    for (long long back = blockIdx.x; back < mine; back += a.tiles) {
+        const long long tile = mine - 1 - back;
+        // per Q tile: KV tiles, the first position that some row does not see
+        int n[2], low[2], top = -1;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const long long r0 = tile * TI_ROWS + 128 * i, r1 = min(n_q, r0 + 128) - 1;
+            n[i] = 0;
+            low[i] = -1;
+            if (r0 < n_q && seq_ok) {
+                const long long p0 = (long long)run.pos + span.x + r0 / a.mul, p1 = (long long)run.pos + span.x + r1 / a.mul;
+                const long long t = min(p1, cap - 1);
+                n[i] = t < 0 ? 0 : (int)(t / TI_KV) + 1;
+                low[i] = p1 >= cap ? -1 : (int)max(p0, -1ll);
+                top = max(top, (int)t);
+            }
+        }
+        const int tiles = max(n[0], n[1]);
+
+        if (warp < TI_SOFT) {
+            // ------------------------------------------------ rows
+            const int i = warp >> 2, r = tid & 127;
+            const long long rr = tile * TI_ROWS + 128 * i + r;
+            const bool real = rr < n_q;
+            const int tok = span.x + (real ? (int)(rr / a.mul) : 0), head = kvh * a.mul + (real ? (int)(rr % a.mul) : 0);
+            const int lim = real ? kv_limit(a.c, run, tok) : -1;
+            const size_t at = (size_t)(run.first + tok) * a.q.ld + (size_t)head * HS;
+            float amax = 0.f;
+            for (int e = 0; e < HS; e += 8) {
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (real) kv_load_row<8>(a.q, a.type, at + e, x);
+#pragma unroll
+                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(x[k]));
+            }
+            const float sc = kv_row_scale(amax), kf = a.scale_log2 / sc;
+            for (int e = 0; e < HS; e += 8) {   // elements 32b + 8c + .. are chunk 4b + c, in the keys' order
+                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (real) kv_load_row<8>(a.q, a.type, at + e, x);
+                uint32_t p[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) p[u] = kv_pack(sc * x[u], sc * x[u + 4]);
+                const int ci = e >> 3;
+                *reinterpret_cast<uint4 *>(sm + i * L::Q_TILE + (ci >> 3) * L::SLICE + sw128(r, ci & 7)) =
+                    make_uint4(p[0], p[1], p[2], p[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar[B_Q]);
+
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21, S = tmem + lanes + 128 * i, O = tmem + lanes + 256 + 128 * i;
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int j = 0; j < n[i]; j++) {
+                ok = tc_wait(&bar[B_S + i], s_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                s_it[i]++;
+                tc_fence_after();
+                const int p0 = j * TI_KV, holes = hole[(kv_it + j) & 3];
+                const bool edge = p0 + TI_KV - 1 > low[i] || holes;
+                auto seen = [&](int t) { return p0 + t <= lim && !(holes >> (t >> 6) & 1); };
+                float mx = -INFINITY;
+#pragma unroll
+                for (int ch = 0; ch < 4; ch++) {
+                    uint32_t v[32];
+                    ti_ld32(v, S + 32 * ch);
+                    ti_wait_ld();
+                    if (edge) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++)
+                            if (seen(32 * ch + k)) mx = fmaxf(mx, __uint_as_float(v[k]));
+                    } else {
+                        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int k = 0; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
+                        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    }
+                }
+                const float mn = mx * kf;
+                const bool move = mn > m + TI_LAG || (m == -INFINITY && mn > -INFINITY);
+                if (__any_sync(0xffffffffu, move)) {
+                    const float to = move ? mn : m, al = m == -INFINITY ? (move ? 0.f : 1.f) : kv_exp2(m - to);
+                    m = to;
+                    l *= al;
+                    if (j > 0) {   // the products so far are complete: S came after them
+#pragma unroll 1
+                        for (int ch = 0; ch < HS; ch += 32) {
+                            uint32_t v[32], w[16];
+                            ti_ld32(v, O + ch);
+                            ti_wait_ld();
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                                for (int k = 0; k < 16; k++) w[k] = __float_as_uint(__uint_as_float(v[16 * h + k]) * al);
+                                ti_st16(O + ch + 16 * h, w);
+                            }
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ch = 0; ch < 4; ch++) {
+                    uint32_t v[32], w[16];
+                    ti_ld32(v, S + 32 * ch);
+                    ti_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        float e0 = kv_exp2(fmaf(__uint_as_float(v[k]), kf, ref)), e1 = kv_exp2(fmaf(__uint_as_float(v[k + 1]), kf, ref));
+                        if (edge) {
+                            if (!seen(32 * ch + k)) e0 = 0.f;
+                            if (!seen(32 * ch + k + 1)) e1 = 0.f;
+                        }
+                        sum[k & 2] += e0;
+                        sum[(k & 2) + 1] += e1;
+                        w[k >> 1] = kv_pack(e0, e1);
+                    }
+                    ti_st16(S + 16 * ch, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                ti_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar[B_P + i]);
+            }
+            if (ok && n[i] > 0) {
+                ok = tc_wait(&bar[B_O + i], o_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                ok = __all_sync(0xffffffffu, ok);
+                o_it[i]++;
+                tc_fence_after();
+            }
+            const float inv = !ok || *abort_s ? NAN : l == 0.f ? 0.f : 1.f / l;
+            const size_t to = (size_t)(run.first + tok) * a.out.ld + (size_t)head * HS;
+#pragma unroll 1
+            for (int ch = 0; ch < HS; ch += 32) {
+                uint32_t v[32];
+#pragma unroll
+                for (int k = 0; k < 32; k++) v[k] = 0u;
+                if (n[i] > 0) {
+                    ti_ld32(v, O + ch);
+                    ti_wait_ld();
+                }
+                if (real) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float4 f = make_float4(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv,
+                                               __uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+                        const float sum = f.x + f.y + f.z + f.w;
+                        if (l == 0.f && inv == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);
+                        else if (sum != sum && l == l && inv == inv) f = kv_plain_row4(a, run.seq, run.first + tok, head, lim, (ch + k) >> 2);
+                        kv_store_row4(a.out, a.type, to + ch + k, f);
+                    }
+                }
+            }
+            tc_fence_before();
+        } else if (warp < TI_MMA_WARP) {
+            // ------------------------------------------------ the cache's codes to operands
+            const int w = warp - TI_SOFT;
+            const KvMagic magic = kv_magic();
+            const int kt = lane >> 2, kc = lane & 3;                       // K: token of 8, 16-byte piece of its codes
+            const int vb = (lane >> 3) % HB, vx = (lane >> 3) / HB, vg = (lane >> 2) & 1, vi = lane & 3;
+            const int vp = w >> 1, oct = 4 * (w & 1) + vi;                 // V: page of the tile, tokens 8 oct .. of it
+            bool ok = true;
+            for (int j = 0; j < tiles && ok; j++) {
+                const uint32_t it = kv_it + j;
+                const int st = it & 1, p0 = j * TI_KV;
+                int pg[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int t = p0 + KV_PAGE * h;
+                    pg[h] = t <= top ? a.c.page(run.seq, t / KV_PAGE) : -1;
+                }
+                // K: warp w takes tokens 32w .. 32w + 31 of the tile
+                uint32_t kw[4][HB];
+                __half ks[4][HB];
+                const int kp = pg[w >> 1];
+                if (kp >= 0) {
+                    const uint8_t *ch = a.c.chunk(kp, kvh);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int t = 32 * (w & 1) + 8 * u + kt;
+                        if constexpr (HB == 4) {
+                            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(ch + (t * 4 + kc) * 16));
+                            kw[u][0] = v.x; kw[u][1] = v.y; kw[u][2] = v.z; kw[u][3] = v.w;
+                            const uint2 s = __ldg(reinterpret_cast<const uint2 *>(ch + kv_k_scales(HS) + t * 8));
+                            ks[u][0] = __ushort_as_half((uint16_t)s.x); ks[u][1] = __ushort_as_half((uint16_t)(s.x >> 16));
+                            ks[u][2] = __ushort_as_half((uint16_t)s.y); ks[u][3] = __ushort_as_half((uint16_t)(s.y >> 16));
+                        } else {
+                            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(ch + (t * 4 + kc) * 8));
+                            kw[u][0] = v.x; kw[u][1] = v.y;
+                            const uint32_t s = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_k_scales(HS) + t * 4));
+                            ks[u][0] = __ushort_as_half((uint16_t)s); ks[u][1] = __ushort_as_half((uint16_t)(s >> 16));
+                        }
+                    }
+                }
+                // V: 8 tokens of page vp, dims 32 vb + 4 g + .. for g = 2 gh + vg
+                constexpr int GH = HB;   // values of gh a lane takes: 4 / (4 / HB)
+                uint32_t vw[GH][4], vs[4];
+                const int vpage = vp ? pg[1] : pg[0];
+#pragma unroll
+                for (int k = 0; k < 4; k++) vs[k] = 0u;
+                if (vpage >= 0) {
+                    const uint8_t *ch = a.c.chunk(vpage, kvh);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        vs[k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_scales(HS) + ((4 * oct + k) * HB + vb) * 4));
+#pragma unroll
+                    for (int u = 0; u < GH; u++) {
+                        const int g = 2 * (u * (4 / HB) + vx) + vg;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            vw[u][k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_codes(HS) + (((4 * oct + k) * 8 + g) * HB + vb) * 4));
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < GH; u++) vw[u][0] = vw[u][1] = vw[u][2] = vw[u][3] = 0u;
+                }
+                if (p0 + TI_KV - 1 > top) {   // tokens nobody sees may read as NaN
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
+                        vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
+                    }
+                }
+                // ---- K into its stage
+                ok = tc_wait(&bar[B_KE + st], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (w == 0 && lane == 0) {
+                    int hl = 0;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) hl |= (pg[h] < 0 && p0 + KV_PAGE * h <= top) << h;
+                    hole[it & 3] = hl;   // read until P(it + 1) is there, written again after it
+                }
+                if (kp >= 0) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int rowi = 32 * w + 8 * u + kt;
+#pragma unroll
+                        for (int b = 0; b < HB; b++) {
+                            uint32_t x[4];
+                            kv_dequant(kw[u][b], __half2half2(ks[u][b]), magic, x);
+                            const int ci = 4 * b + kc;
+                            *reinterpret_cast<uint4 *>(sm + L::K + st * L::K_STAGE + (ci >> 3) * L::SLICE + sw128(rowi, ci & 7)) =
+                                make_uint4(x[0], x[1], x[2], x[3]);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar[B_KF + st]);
+                // ---- V
+                ok = tc_wait(&bar[B_VE + st], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int u = 0; u < GH; u++) {
+                    const int g = 2 * (u * (4 / HB) + vx) + vg;
+                    uint32_t x[4][4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) kv_dequant(vw[u][k], *reinterpret_cast<__half2 *>(&vs[k]), magic, x[k]);
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        const int dim = 32 * vb + 4 * g + d;
+                        *reinterpret_cast<uint4 *>(sm + L::V + st * L::V_STAGE + vp * L::V_PAGE + sw128(dim, oct)) =
+                            make_uint4(x[0][d], x[1][d], x[2][d], x[3][d]);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar[B_VF + st]);
+            }
+        } else if (lane == 0) {
+            // ------------------------------------------------ products
+            constexpr uint32_t id_qk = umma_idesc(0, 128, TI_KV), id_pv = umma_idesc(0, 128, HS);
+            const uint32_t q_at = smem_u32(sm), k_at = smem_u32(sm + L::K), v_at = smem_u32(sm + L::V);
+            auto qk = [&](int i, int st) {
+#pragma unroll
+                for (int k = 0; k < HS / 16; k++)
+                    ti_mma_ss(tmem + 128 * i, umma_desc_sw128(q_at + i * L::Q_TILE + (k >> 2) * L::SLICE + (k & 3) * 32),
+                              umma_desc_sw128(k_at + st * L::K_STAGE + (k >> 2) * L::SLICE + (k & 3) * 32), id_qk, k > 0);
+                ti_commit(&bar[B_S + i]);
+            };
+            bool ok = tiles == 0 || tc_wait(&bar[B_Q], q_it & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+            if (ok && tiles > 0) ok = tc_wait(&bar[B_KF + (kv_it & 1)], (kv_it >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+            if (ok && tiles > 0) {
+                tc_fence_after();
+                for (int i = 0; i < 2; i++)
+                    if (n[i] > 0) qk(i, kv_it & 1);
+                ti_commit(&bar[B_KE + (kv_it & 1)]);
+            }
+            for (int j = 0; j < tiles && ok; j++) {
+                const uint32_t it = kv_it + j;
+                const int st = it & 1, nx = st ^ 1;
+                ok = tc_wait(&bar[B_VF + st], (it >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                if (ok && j + 1 < tiles) ok = tc_wait(&bar[B_KF + nx], ((it + 1) >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                for (int i = 0; i < 2 && ok; i++) {
+                    if (j >= n[i]) continue;
+                    ok = tc_wait(&bar[B_P + i], s_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                    if (!ok) break;
+                    s_it[i]++;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < TI_KV / 16; k++)
+                        ti_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k,
+                                  umma_desc_sw128(v_at + st * L::V_STAGE + (k >> 2) * L::V_PAGE + (k & 3) * 32), id_pv, j > 0 || k > 0);
+                    if (j + 1 < n[i]) qk(i, nx);
+                    else ti_commit(&bar[B_O + i]);
+                }
+                if (!ok) break;
+                ti_commit(&bar[B_VE + st]);
+                if (j + 1 < tiles) ti_commit(&bar[B_KE + nx]);
+            }
+        }
+        kv_it += tiles;
+        q_it++;
+        // Everyone is done with this tile's shared memory and TMEM.
+        __syncthreads();
+        tc_fence_after();
+        if (*abort_s) break;
+    }
+    tc_fence_before();
+    __syncthreads();
+    __syncwarp();
+    if (warp == TI_MMA_WARP)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+template <int HS> static cudaError_t launch_tile(const KvAttn &a, dim3 grid, cudaStream_t st)
+{
+    static unsigned long long done = 0;
+    const int smem = TileSmem<HS>::BYTES;
+    cudaError_t e = once_per_device(
+        done, [&] { return cudaFuncSetAttribute(k_kv_attn_tile<HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (e) return e;
+    k_kv_attn_tile<HS><<<grid, TI_THREADS, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+bool kv_attn_tile_takes(const KvAttn &a, int max_rows)
+{
+    return a.type != KV_F32 && (a.c.hs == 64 || a.c.hs == 128) && a.c.n_kv <= 65535 && a.n_runs <= 65535 &&
+           (long long)max_rows * a.mul >= 64;
+}
+
+cudaError_t launch_kv_attn_tile(const KvAttn &a0, int max_rows, cudaStream_t st)
+{
+    KvAttn a = a0;
+    const long long q = (long long)std::max(max_rows, 1) * a.mul;
+    a.tiles = (int)std::min<long long>((q + TI_ROWS - 1) / TI_ROWS, 1 << 20);
+    const dim3 grid((unsigned)a.tiles, (unsigned)a.c.n_kv, (unsigned)a.n_runs);
+    return a.c.hs == 64 ? launch_tile<64>(a, grid, st) : launch_tile<128>(a, grid, st);
+}
+
+} // namespace cats
