@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     tc_fence_after();
     const uint32_t tmem = *slot;   // S_0, S_1 (128 columns each; P_i over the first 64 of S_i), O_0, O_1
 
-    const int kvh = blockIdx.y;
+    const int kvh = blockIdx.x;
     const KvRun run = a.runs[blockIdx.z];
-    const int2 span = kv_run_rows(run, a.q.rows, blockIdx.x == 0 && kvh == 0 ? a.c.err : nullptr);
+    const int2 span = kv_run_rows(run, a.q.rows, blockIdx.y == 0 && kvh == 0 ? a.c.err : nullptr);
     const long long n_q = (long long)(span.y - span.x) * a.mul;
     const long long cap = (long long)a.c.max_pages * KV_PAGE;
     const bool seq_ok = run.seq >= 0 && run.seq < a.c.n_seqs;
@@ -131,9 +131,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     // counts of waits on each barrier so far: their parities
     uint32_t kv_it = 0, q_it = 0, s_it[2] = {0, 0}, o_it[2] = {0, 0};
 
-    // the longest tiles (the last ones) first
+    // the longest tiles (the last ones) of every head first
     const long long mine = n_q > 0 ? (n_q + TI_ROWS - 1) / TI_ROWS : 0;
-    for (long long back = blockIdx.x; back < mine; back += a.tiles) {
+    for (long long back = blockIdx.y; back < mine; back += a.tiles) {
         const long long tile = mine - 1 - back;
         // per Q tile: KV tiles, the first position that some row does not see
         int n[2], low[2], top = -1;
@@ -193,22 +193,32 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 tc_fence_after();
                 const int p0 = j * TI_KV, holes = hole[(kv_it + j) & 3];
                 const bool edge = p0 + TI_KV - 1 > low[i] || holes;
-                auto seen = [&](int t) { return p0 + t <= lim && !(holes >> (t >> 6) & 1); };
+                auto seen = [&](int t) -> uint32_t {   // which of 32 tokens from t on this row sees
+                    const int n = lim - (p0 + t) + 1;
+                    return n <= 0 || (holes >> (t >> 6) & 1) ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
+                };
                 float mx = -INFINITY;
-#pragma unroll
-                for (int ch = 0; ch < 4; ch++) {
-                    uint32_t v[32];
-                    ti_ld32(v, S + 32 * ch);
-                    ti_wait_ld();
-                    if (edge) {
-#pragma unroll
-                        for (int k = 0; k < 32; k++)
-                            if (seen(32 * ch + k)) mx = fmaxf(mx, __uint_as_float(v[k]));
-                    } else {
+                if (!edge) {
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ch++) {
+                        uint32_t v[32];
+                        ti_ld32(v, S + 32 * ch);
+                        ti_wait_ld();
                         float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int k = 0; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
                         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    }
+                } else {
+#pragma unroll 1
+                    for (int ch = 0; ch < 4; ch++) {
+                        uint32_t v[32];
+                        ti_ld32(v, S + 32 * ch);
+                        ti_wait_ld();
+                        const uint32_t bits = seen(32 * ch);
+#pragma unroll
+                        for (int k = 0; k < 32; k++)
+                            if (bits >> k & 1) mx = fmaxf(mx, __uint_as_float(v[k]));
                     }
                 }
                 const float mn = mx * kf;
@@ -234,18 +244,20 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
                 const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll 1
                 for (int ch = 0; ch < 4; ch++) {
                     uint32_t v[32], w[16];
                     ti_ld32(v, S + 32 * ch);
                     ti_wait_ld();
+                    if (edge) {
+                        const uint32_t bits = seen(32 * ch);
+#pragma unroll
+                        for (int k = 0; k < 32; k++)
+                            if (!(bits >> k & 1)) v[k] = 0xff800000u;   // -inf
+                    }
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        float e0 = kv_exp2(fmaf(__uint_as_float(v[k]), kf, ref)), e1 = kv_exp2(fmaf(__uint_as_float(v[k + 1]), kf, ref));
-                        if (edge) {
-                            if (!seen(32 * ch + k)) e0 = 0.f;
-                            if (!seen(32 * ch + k + 1)) e1 = 0.f;
-                        }
+                        const float e0 = kv_exp2(fmaf(__uint_as_float(v[k]), kf, ref)), e1 = kv_exp2(fmaf(__uint_as_float(v[k + 1]), kf, ref));
                         sum[k & 2] += e0;
                         sum[(k & 2) + 1] += e1;
                         w[k >> 1] = kv_pack(e0, e1);
@@ -295,86 +307,87 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             const int kt = lane >> 2, kc = lane & 3;                       // K: token of 8, 16-byte piece of its codes
             const int vb = (lane >> 3) % HB, vx = (lane >> 3) / HB, vg = (lane >> 2) & 1, vi = lane & 3;
             const int vp = w >> 1, oct = 4 * (w & 1) + vi;                 // V: page of the tile, tokens 8 oct .. of it
-            bool ok = true;
-            for (int j = 0; j < tiles && ok; j++) {
-                const uint32_t it = kv_it + j;
-                const int st = it & 1, p0 = j * TI_KV;
-                int pg[2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int t = p0 + KV_PAGE * h;
-                    pg[h] = t <= top ? a.c.page(run.seq, t / KV_PAGE) : -1;
-                }
+            constexpr int GH = HB;   // values of gh a lane takes: 4 / (4 / HB)
+            struct Raw {             // a KV tile's codes and scales, as this lane takes them
+                uint32_t kw[4][HB], ks[4][HB / 2], vw[GH][4], vs[4];
+                int hole, k_there;
+            };
+            auto pages = [&](int j) {   // page numbers of a tile's two pages
+                const int t = j * TI_KV;
+                return make_int2(j < tiles && t <= top ? a.c.page(run.seq, t / KV_PAGE) : -1,
+                                 j < tiles && t + KV_PAGE <= top ? a.c.page(run.seq, t / KV_PAGE + 1) : -1);
+            };
+            auto fetch = [&](int j, int2 pg, Raw &r) {
+                const int p0 = j * TI_KV;
+                r.hole = (pg.x < 0 && p0 <= top) | (pg.y < 0 && p0 + KV_PAGE <= top) << 1;
                 // K: warp w takes tokens 32w .. 32w + 31 of the tile
-                uint32_t kw[4][HB];
-                __half ks[4][HB];
-                const int kp = pg[w >> 1];
-                if (kp >= 0) {
-                    const uint8_t *ch = a.c.chunk(kp, kvh);
+                const int page = w >> 1 ? pg.y : pg.x;
+                r.k_there = page >= 0;
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const int t = 32 * (w & 1) + 8 * u + kt;
-                        if constexpr (HB == 4) {
-                            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(ch + (t * 4 + kc) * 16));
-                            kw[u][0] = v.x; kw[u][1] = v.y; kw[u][2] = v.z; kw[u][3] = v.w;
-                            const uint2 s = __ldg(reinterpret_cast<const uint2 *>(ch + kv_k_scales(HS) + t * 8));
-                            ks[u][0] = __ushort_as_half((uint16_t)s.x); ks[u][1] = __ushort_as_half((uint16_t)(s.x >> 16));
-                            ks[u][2] = __ushort_as_half((uint16_t)s.y); ks[u][3] = __ushort_as_half((uint16_t)(s.y >> 16));
-                        } else {
-                            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(ch + (t * 4 + kc) * 8));
-                            kw[u][0] = v.x; kw[u][1] = v.y;
-                            const uint32_t s = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_k_scales(HS) + t * 4));
-                            ks[u][0] = __ushort_as_half((uint16_t)s); ks[u][1] = __ushort_as_half((uint16_t)(s >> 16));
-                        }
+                for (int k = 0; k < 4; k++) r.vs[k] = 0u;
+                if (page < 0) {
+#pragma unroll
+                    for (int u = 0; u < GH; u++) r.vw[u][0] = r.vw[u][1] = r.vw[u][2] = r.vw[u][3] = 0u;
+                    return;
+                }
+                const uint8_t *ch = a.c.chunk(page, kvh);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int t = 32 * (w & 1) + 8 * u + kt;
+                    if constexpr (HB == 4) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(ch + (t * 4 + kc) * 16));
+                        r.kw[u][0] = v.x; r.kw[u][1] = v.y; r.kw[u][2] = v.z; r.kw[u][3] = v.w;
+                        const uint2 s = __ldg(reinterpret_cast<const uint2 *>(ch + kv_k_scales(HS) + t * 8));
+                        r.ks[u][0] = s.x; r.ks[u][1] = s.y;
+                    } else {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(ch + (t * 4 + kc) * 8));
+                        r.kw[u][0] = v.x; r.kw[u][1] = v.y;
+                        r.ks[u][0] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_k_scales(HS) + t * 4));
                     }
                 }
                 // V: 8 tokens of page vp, dims 32 vb + 4 g + .. for g = 2 gh + vg
-                constexpr int GH = HB;   // values of gh a lane takes: 4 / (4 / HB)
-                uint32_t vw[GH][4], vs[4];
-                const int vpage = vp ? pg[1] : pg[0];
 #pragma unroll
-                for (int k = 0; k < 4; k++) vs[k] = 0u;
-                if (vpage >= 0) {
-                    const uint8_t *ch = a.c.chunk(vpage, kvh);
+                for (int k = 0; k < 4; k++)
+                    r.vs[k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_scales(HS) + ((4 * oct + k) * HB + vb) * 4));
+#pragma unroll
+                for (int u = 0; u < GH; u++) {
+                    const int g = 2 * (u * (4 / HB) + vx) + vg;
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        vs[k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_scales(HS) + ((4 * oct + k) * HB + vb) * 4));
-#pragma unroll
-                    for (int u = 0; u < GH; u++) {
-                        const int g = 2 * (u * (4 / HB) + vx) + vg;
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            vw[u][k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_codes(HS) + (((4 * oct + k) * 8 + g) * HB + vb) * 4));
-                    }
-                } else {
-#pragma unroll
-                    for (int u = 0; u < GH; u++) vw[u][0] = vw[u][1] = vw[u][2] = vw[u][3] = 0u;
+                        r.vw[u][k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_codes(HS) + (((4 * oct + k) * 8 + g) * HB + vb) * 4));
                 }
+            };
+            bool ok = true;
+            Raw next;
+            int2 after = pages(1);
+            fetch(0, pages(0), next);
+            for (int j = 0; j < tiles && ok; j++) {
+                const uint32_t it = kv_it + j;
+                const int st = it & 1, p0 = j * TI_KV;
+                Raw r = next;
+                fetch(j + 1, after, next);   // on its way while this one is worked on
+                after = pages(j + 2);
                 if (p0 + TI_KV - 1 > top) {   // tokens nobody sees may read as NaN
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
-                        vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
+                        r.vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
                     }
                 }
                 // ---- K into its stage
                 ok = tc_wait(&bar[B_KE + st], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                if (w == 0 && lane == 0) {
-                    int hl = 0;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) hl |= (pg[h] < 0 && p0 + KV_PAGE * h <= top) << h;
-                    hole[it & 3] = hl;   // read until P(it + 1) is there, written again after it
-                }
-                if (kp >= 0) {
+                if (w == 0 && lane == 0) hole[it & 3] = r.hole;   // read until P(it + 1) is there, written again after it
+                if (r.k_there) {
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         const int rowi = 32 * w + 8 * u + kt;
 #pragma unroll
                         for (int b = 0; b < HB; b++) {
                             uint32_t x[4];
-                            kv_dequant(kw[u][b], __half2half2(ks[u][b]), magic, x);
+                            const __half2 two = *reinterpret_cast<const __half2 *>(&r.ks[u][b / 2]);
+                            kv_dequant(r.kw[u][b], b & 1 ? __high2half2(two) : __low2half2(two), magic, x);
                             const int ci = 4 * b + kc;
                             *reinterpret_cast<uint4 *>(sm + L::K + st * L::K_STAGE + (ci >> 3) * L::SLICE + sw128(rowi, ci & 7)) =
                                 make_uint4(x[0], x[1], x[2], x[3]);
@@ -393,7 +406,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     const int g = 2 * (u * (4 / HB) + vx) + vg;
                     uint32_t x[4][4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) kv_dequant(vw[u][k], *reinterpret_cast<__half2 *>(&vs[k]), magic, x[k]);
+                    for (int k = 0; k < 4; k++) kv_dequant(r.vw[u][k], *reinterpret_cast<const __half2 *>(&r.vs[k]), magic, x[k]);
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
                         const int dim = 32 * vb + 4 * g + d;
@@ -474,7 +487,7 @@ template <int HS> static cudaError_t launch_tile(const KvAttn &a, dim3 grid, cud
 
 bool kv_attn_tile_takes(const KvAttn &a, int max_rows)
 {
-    return a.type != KV_F32 && (a.c.hs == 64 || a.c.hs == 128) && a.c.n_kv <= 65535 && a.n_runs <= 65535 &&
+    return a.type != KV_F32 && (a.c.hs == 64 || a.c.hs == 128) && a.n_runs <= 65535 &&
            (long long)max_rows * a.mul >= 64;
 }
 
@@ -482,8 +495,8 @@ cudaError_t launch_kv_attn_tile(const KvAttn &a0, int max_rows, cudaStream_t st)
 {
     KvAttn a = a0;
     const long long q = (long long)std::max(max_rows, 1) * a.mul;
-    a.tiles = (int)std::min<long long>((q + TI_ROWS - 1) / TI_ROWS, 1 << 20);
-    const dim3 grid((unsigned)a.tiles, (unsigned)a.c.n_kv, (unsigned)a.n_runs);
+    a.tiles = (int)std::min<long long>((q + TI_ROWS - 1) / TI_ROWS, 65535);
+    const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.tiles, (unsigned)a.n_runs);
     return a.c.hs == 64 ? launch_tile<64>(a, grid, st) : launch_tile<128>(a, grid, st);
 }
 
