@@ -11,7 +11,9 @@
 //
 // Roles: warps 0-3 and 4-7 the rows of the two tiles (they also bring Q in and
 // store O), warps 8-11 dequantize the cache's codes into the products' operand
-// layout (128-byte swizzle, two stages), warp 12 issues the products.  The
+// layout (128-byte swizzle, two stages), warp 12 issues the products, warp 13
+// brings the codes to shared memory with bulk copies, three half tiles ahead.
+// (Codes loaded to registers a tile ahead made each proxy fence wait for them.)  The
 // codes are read once per 256 rows; the values (code - 8) * scale are exact in
 // fp16 (kv.cuh), so the products' operands are the cache's values.
 //
@@ -29,19 +31,22 @@
 namespace cats {
 
 constexpr int TI_ROWS = 256, TI_KV = 128;
-constexpr int TI_SOFT = 8, TI_DEQ = 4, TI_MMA_WARP = TI_SOFT + TI_DEQ, TI_THREADS = (TI_MMA_WARP + 1) * 32;
+constexpr int TI_SOFT = 8, TI_DEQ = 4, TI_MMA_WARP = TI_SOFT + TI_DEQ, TI_LOAD_WARP = TI_MMA_WARP + 1,
+              TI_THREADS = (TI_LOAD_WARP + 1) * 32;
 constexpr float TI_P_BITS = 7.f, TI_LAG = 8.f;   // probabilities are held times 2^7 and may reach 2^15
 
 // shared memory, from a 1024-byte boundary: Q [2][HS/64][128 rows][128 B], K the
-// same per stage, V [2 pages][HS rows][128 B] per stage, barriers
+// same per stage, V [2 pages][HS rows][128 B] per stage, three buffers of raw
+// codes (K and V of a tile by turns), barriers
 template <int HS> struct TileSmem {
     static constexpr int SLICE = 128 * 128;                  // 128 rows of 64 halves
     static constexpr int Q_TILE = HS / 64 * SLICE, K_STAGE = HS / 64 * SLICE, V_PAGE = HS * 128, V_STAGE = 2 * V_PAGE;
-    static constexpr int K = 2 * Q_TILE, V = K + 2 * K_STAGE, BAR = V + 2 * V_STAGE;
+    static constexpr int RAW_UNIT = 72 * HS;                 // K or V of two pages: codes, then scales
+    static constexpr int K = 2 * Q_TILE, V = K + 2 * K_STAGE, RAW = V + 2 * V_STAGE, BAR = RAW + 3 * RAW_UNIT;
     static constexpr int BYTES = BAR + 256 + 1024;           // + the alignment's slack
 };
 
-enum TileBar { B_Q, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_O = B_P + 2, B_N = B_O + 2 };
+enum TileBar { B_Q, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_O = B_P + 2, B_RF = B_O + 2, B_RE = B_RF + 3, B_N = B_RE + 3 };
 
 __device__ __forceinline__ void ti_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
@@ -95,7 +100,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::BAR);
     volatile int *abort_s = reinterpret_cast<volatile int *>(bar + B_N);
     volatile int *hole = abort_s + 1;   // [4], by KV tile: pages of it that do not exist (bit 0, 1)
-    uint32_t *slot = const_cast<uint32_t *>(reinterpret_cast<volatile uint32_t *>(abort_s + 5));
+    volatile int *present = abort_s + 5;   // [3], by raw buffer: which of its two pages are in it
+    uint32_t *slot = const_cast<uint32_t *>(reinterpret_cast<volatile uint32_t *>(abort_s + 8));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     if (tid == 0) {
@@ -108,6 +114,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             mbar_init(&bar[B_S + s], 1);
             mbar_init(&bar[B_P + s], TI_SOFT / 2);
             mbar_init(&bar[B_O + s], 1);
+        }
+        for (int s = 0; s < 3; s++) {
+            mbar_init(&bar[B_RF + s], 1);
+            mbar_init(&bar[B_RE + s], TI_DEQ);
         }
         *abort_s = 0;
         fence_barrier_init();
@@ -160,23 +170,35 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             const int tok = span.x + (real ? (int)(rr / a.mul) : 0), head = kvh * a.mul + (real ? (int)(rr % a.mul) : 0);
             const int lim = real ? kv_limit(a.c, run, tok) : -1;
             const size_t at = (size_t)(run.first + tok) * a.q.ld + (size_t)head * HS;
-            float amax = 0.f;
-            for (int e = 0; e < HS; e += 8) {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (real) kv_load_row<8>(a.q, a.type, at + e, x);
+            float sc, kf;
+            {
+                uint2 x[HS / 4];   // the row, all its loads in flight at once
+                const uint16_t *p = static_cast<const uint16_t *>(a.q.p) + at;
 #pragma unroll
-                for (int k = 0; k < 8; k++) amax = fmaxf(amax, fabsf(x[k]));
-            }
-            const float sc = kv_row_scale(amax), kf = a.scale_log2 / sc;
-            for (int e = 0; e < HS; e += 8) {   // elements 32b + 8c + .. are chunk 4b + c, in the keys' order
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (real) kv_load_row<8>(a.q, a.type, at + e, x);
-                uint32_t p[4];
+                for (int e = 0; e < HS / 4; e++) {
+                    x[e] = make_uint2(0u, 0u);
+                    if (!real) continue;
+                    if (a.q.vec) x[e] = __ldg(reinterpret_cast<const uint2 *>(p) + e);
+                    else x[e] = make_uint2(p[4 * e] | (uint32_t)p[4 * e + 1] << 16, p[4 * e + 2] | (uint32_t)p[4 * e + 3] << 16);
+                }
+                auto value = [&](int e) {   // element e as fp32
+                    const uint32_t w = e & 2 ? x[e >> 2].y : x[e >> 2].x;
+                    return a.type == KV_F16 ? __half2float(__ushort_as_half((uint16_t)(e & 1 ? w >> 16 : w)))
+                                            : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+                };
+                float amax = 0.f;
 #pragma unroll
-                for (int u = 0; u < 4; u++) p[u] = kv_pack(sc * x[u], sc * x[u + 4]);
-                const int ci = e >> 3;
-                *reinterpret_cast<uint4 *>(sm + i * L::Q_TILE + (ci >> 3) * L::SLICE + sw128(r, ci & 7)) =
-                    make_uint4(p[0], p[1], p[2], p[3]);
+                for (int e = 0; e < HS; e++) amax = fmaxf(amax, fabsf(value(e)));
+                sc = kv_row_scale(amax);
+                kf = a.scale_log2 / sc;
+#pragma unroll
+                for (int ci = 0; ci < HS / 8; ci++) {   // elements 32b + 8c + .. are chunk 4b + c, in the keys' order
+                    uint32_t h[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) h[u] = kv_pack(sc * value(8 * ci + u), sc * value(8 * ci + u + 4));
+                    *reinterpret_cast<uint4 *>(sm + i * L::Q_TILE + (ci >> 3) * L::SLICE + sw128(r, ci & 7)) =
+                        make_uint4(h[0], h[1], h[2], h[3]);
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -308,86 +330,58 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             const int vb = (lane >> 3) % HB, vx = (lane >> 3) / HB, vg = (lane >> 2) & 1, vi = lane & 3;
             const int vp = w >> 1, oct = 4 * (w & 1) + vi;                 // V: page of the tile, tokens 8 oct .. of it
             constexpr int GH = HB;   // values of gh a lane takes: 4 / (4 / HB)
-            struct Raw {             // a KV tile's codes and scales, as this lane takes them
-                uint32_t kw[4][HB], ks[4][HB / 2], vw[GH][4], vs[4];
-                int hole, k_there;
+            bool ok = true;
+            auto raw_unit = [&](uint32_t u) {
+                ok = tc_wait(&bar[B_RF + u % 3], (u / 3) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                ok = __all_sync(0xffffffffu, ok);
+                return sm + L::RAW + (u % 3) * L::RAW_UNIT;
             };
-            auto pages = [&](int j) {   // page numbers of a tile's two pages
-                const int t = j * TI_KV;
-                return make_int2(j < tiles && t <= top ? a.c.page(run.seq, t / KV_PAGE) : -1,
-                                 j < tiles && t + KV_PAGE <= top ? a.c.page(run.seq, t / KV_PAGE + 1) : -1);
+            auto stage_free = [&](int b, uint32_t it) {
+                ok = tc_wait(&bar[b + (it & 1)], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                ok = __all_sync(0xffffffffu, ok);
             };
-            auto fetch = [&](int j, int2 pg, Raw &r) {
-                const int p0 = j * TI_KV;
-                r.hole = (pg.x < 0 && p0 <= top) | (pg.y < 0 && p0 + KV_PAGE <= top) << 1;
-                // K: warp w takes tokens 32w .. 32w + 31 of the tile
-                const int page = w >> 1 ? pg.y : pg.x;
-                r.k_there = page >= 0;
-#pragma unroll
-                for (int k = 0; k < 4; k++) r.vs[k] = 0u;
-                if (page < 0) {
-#pragma unroll
-                    for (int u = 0; u < GH; u++) r.vw[u][0] = r.vw[u][1] = r.vw[u][2] = r.vw[u][3] = 0u;
-                    return;
-                }
-                const uint8_t *ch = a.c.chunk(page, kvh);
+            auto arrive = [&](uint64_t *bp) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bp);
+            };
+            for (int j = 0; j < tiles && ok; j++) {
+                const uint32_t it = kv_it + j, u0 = 2 * it;
+                const int st = it & 1, p0 = j * TI_KV;
+                // ---- K: warp w takes tokens 32w .. 32w + 31 of the tile
+                const uint8_t *raw = raw_unit(u0);
+                if (!ok) break;
+                const int there = present[u0 % 3];
+                uint32_t kw[4][HB], ks[4][HB / 2];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int t = 32 * (w & 1) + 8 * u + kt;
+                    const uint8_t *code = raw + (w >> 1) * 32 * HS + (t * 4 + kc) * 4 * HB;
+                    const uint8_t *scale = raw + 64 * HS + (w >> 1) * 4 * HS + t * 2 * HB;
                     if constexpr (HB == 4) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(ch + (t * 4 + kc) * 16));
-                        r.kw[u][0] = v.x; r.kw[u][1] = v.y; r.kw[u][2] = v.z; r.kw[u][3] = v.w;
-                        const uint2 s = __ldg(reinterpret_cast<const uint2 *>(ch + kv_k_scales(HS) + t * 8));
-                        r.ks[u][0] = s.x; r.ks[u][1] = s.y;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(code);
+                        kw[u][0] = v.x; kw[u][1] = v.y; kw[u][2] = v.z; kw[u][3] = v.w;
+                        const uint2 s = *reinterpret_cast<const uint2 *>(scale);
+                        ks[u][0] = s.x; ks[u][1] = s.y;
                     } else {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(ch + (t * 4 + kc) * 8));
-                        r.kw[u][0] = v.x; r.kw[u][1] = v.y;
-                        r.ks[u][0] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_k_scales(HS) + t * 4));
+                        const uint2 v = *reinterpret_cast<const uint2 *>(code);
+                        kw[u][0] = v.x; kw[u][1] = v.y;
+                        ks[u][0] = *reinterpret_cast<const uint32_t *>(scale);
                     }
                 }
-                // V: 8 tokens of page vp, dims 32 vb + 4 g + .. for g = 2 gh + vg
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    r.vs[k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_scales(HS) + ((4 * oct + k) * HB + vb) * 4));
-#pragma unroll
-                for (int u = 0; u < GH; u++) {
-                    const int g = 2 * (u * (4 / HB) + vx) + vg;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        r.vw[u][k] = __ldg(reinterpret_cast<const uint32_t *>(ch + kv_v_codes(HS) + (((4 * oct + k) * 8 + g) * HB + vb) * 4));
-                }
-            };
-            bool ok = true;
-            Raw next;
-            int2 after = pages(1);
-            fetch(0, pages(0), next);
-            for (int j = 0; j < tiles && ok; j++) {
-                const uint32_t it = kv_it + j;
-                const int st = it & 1, p0 = j * TI_KV;
-                Raw r = next;
-                fetch(j + 1, after, next);   // on its way while this one is worked on
-                after = pages(j + 2);
-                if (p0 + TI_KV - 1 > top) {   // tokens nobody sees may read as NaN
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
-                        r.vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
-                    }
-                }
-                // ---- K into its stage
-                ok = tc_wait(&bar[B_KE + st], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
+                arrive(&bar[B_RE + u0 % 3]);
+                stage_free(B_KE, it);
                 if (!ok) break;
-                if (w == 0 && lane == 0) hole[it & 3] = r.hole;   // read until P(it + 1) is there, written again after it
-                if (r.k_there) {
+                // (read until P(it + 1) is there, written again after it)
+                if (w == 0 && lane == 0) hole[it & 3] = ~there & ((p0 <= top) | (p0 + KV_PAGE <= top) << 1);
+                if (there >> (w >> 1) & 1) {
 #pragma unroll
                     for (int u = 0; u < 4; u++) {
                         const int rowi = 32 * w + 8 * u + kt;
 #pragma unroll
                         for (int b = 0; b < HB; b++) {
                             uint32_t x[4];
-                            const __half2 two = *reinterpret_cast<const __half2 *>(&r.ks[u][b / 2]);
-                            kv_dequant(r.kw[u][b], b & 1 ? __high2half2(two) : __low2half2(two), magic, x);
+                            const __half2 two = *reinterpret_cast<const __half2 *>(&ks[u][b / 2]);
+                            kv_dequant(kw[u][b], b & 1 ? __high2half2(two) : __low2half2(two), magic, x);
                             const int ci = 4 * b + kc;
                             *reinterpret_cast<uint4 *>(sm + L::K + st * L::K_STAGE + (ci >> 3) * L::SLICE + sw128(rowi, ci & 7)) =
                                 make_uint4(x[0], x[1], x[2], x[3]);
@@ -395,18 +389,36 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     }
                 }
                 fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar[B_KF + st]);
-                // ---- V
-                ok = tc_wait(&bar[B_VE + st], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
-                ok = __all_sync(0xffffffffu, ok);
+                arrive(&bar[B_KF + st]);
+                // ---- V: 8 tokens of page vp, elements 32 vb + 4 g + .. for g = 2 gh + vg
+                raw = raw_unit(u0 + 1);
+                if (!ok) break;
+                const bool v_there = present[(u0 + 1) % 3] >> vp & 1;
+                uint32_t vw[GH][4], vs[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    vs[k] = *reinterpret_cast<const uint32_t *>(raw + 64 * HS + vp * 4 * HS + ((4 * oct + k) * HB + vb) * 4);
+                    // what nobody sees, or nobody wrote, may read as NaN
+                    const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
+                    if (p0 + TI_KV - 1 > top) vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
+                    if (!v_there) vs[k] = 0u;
+                }
+#pragma unroll
+                for (int u = 0; u < GH; u++) {
+                    const int g = 2 * (u * (4 / HB) + vx) + vg;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        vw[u][k] = *reinterpret_cast<const uint32_t *>(raw + vp * 32 * HS + (((4 * oct + k) * 8 + g) * HB + vb) * 4);
+                }
+                arrive(&bar[B_RE + (u0 + 1) % 3]);
+                stage_free(B_VE, it);
                 if (!ok) break;
 #pragma unroll
                 for (int u = 0; u < GH; u++) {
                     const int g = 2 * (u * (4 / HB) + vx) + vg;
                     uint32_t x[4][4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) kv_dequant(r.vw[u][k], *reinterpret_cast<const __half2 *>(&r.vs[k]), magic, x[k]);
+                    for (int k = 0; k < 4; k++) kv_dequant(vw[u][k], *reinterpret_cast<const __half2 *>(&vs[k]), magic, x[k]);
 #pragma unroll
                     for (int d = 0; d < 4; d++) {
                         const int dim = 32 * vb + 4 * g + d;
@@ -415,8 +427,44 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     }
                 }
                 fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar[B_VF + st]);
+                arrive(&bar[B_VF + st]);
+            }
+        } else if (warp == TI_LOAD_WARP) {
+            // ------------------------------------------------ codes and scales, as they lie
+            if (lane == 0) {
+                auto page = [&](int t) { return t <= top ? a.c.page(run.seq, t / KV_PAGE) : -1; };
+                int pg[2] = {page(0), page(KV_PAGE)};
+                bool ok = true;
+                uint32_t issued = 2 * kv_it;
+                for (int j = 0; j < tiles && ok; j++) {
+                    const int t = (j + 1) * TI_KV, nx[2] = {page(t), page(t + KV_PAGE)};
+                    for (int v = 0; v < 2 && ok; v++) {
+                        const uint32_t u = 2 * (kv_it + j) + v;
+                        uint64_t *full = &bar[B_RF + u % 3];
+                        ok = tc_wait(&bar[B_RE + u % 3], ((u / 3) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                        if (!ok) break;
+                        const int there = (pg[0] >= 0) | (pg[1] >= 0) << 1;
+                        issued = u + 1;
+                        present[u % 3] = there;
+                        if (there == 0) {
+                            mbar_arrive(full);
+                            continue;
+                        }
+                        mbar_arrive_expect_tx(full, ((there & 1) + (there >> 1)) * 36 * HS);
+                        uint8_t *raw = sm + L::RAW + (u % 3) * L::RAW_UNIT;
+                        for (int h = 0; h < 2; h++) {
+                            if (pg[h] < 0) continue;
+                            const uint8_t *ch = a.c.chunk(pg[h], kvh);
+                            bulk_g2s_keep(raw + h * 32 * HS, ch + (v ? kv_v_codes(HS) : 0), 32 * HS, full);
+                            bulk_g2s_keep(raw + 64 * HS + h * 4 * HS, ch + (v ? kv_v_scales(HS) : kv_k_scales(HS)), 4 * HS, full);
+                        }
+                    }
+                    pg[0] = nx[0];
+                    pg[1] = nx[1];
+                }
+                // after a wait that gave up: no copy may be under way when the CTA ends
+                for (uint32_t u = issued < 3 ? 0 : issued - 3; !ok && u < issued; u++)
+                    mbar_wait_bounded(&bar[B_RF + u % 3], (u / 3) & 1, nullptr, 0);
             }
         } else if (lane == 0) {
             // ------------------------------------------------ products
