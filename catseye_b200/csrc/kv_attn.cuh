@@ -93,6 +93,25 @@ __device__ __forceinline__ float kv_exp2(float x)
     return r;
 }
 
+// HB consecutive words of shared memory
+template <int HB> struct Words {
+    uint32_t w[HB];
+};
+template <int HB> __device__ __forceinline__ Words<HB> lds_words(const uint8_t *p)
+{
+    Words<HB> r;
+    if constexpr (HB == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
+    } else if constexpr (HB == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = v.x; r.w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int b = 0; b < HB; b++) r.w[b] = reinterpret_cast<const uint32_t *>(p)[b];
+    }
+    return r;
+}
 // N consecutive elements of a row of any supported type, as floats
 template <int N> __device__ __forceinline__ void kv_load_row(const KvRows &t, int type, size_t i, float (&x)[N])
 {

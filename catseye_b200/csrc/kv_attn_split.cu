@@ -44,24 +44,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const uint8_t *src)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <int HB> struct Words {
-    uint32_t w[HB];
-};
-template <int HB> __device__ __forceinline__ Words<HB> lds_words(const uint8_t *p)
-{
-    Words<HB> r;
-    if constexpr (HB == 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
-    } else if constexpr (HB == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        r.w[0] = v.x; r.w[1] = v.y;
-    } else {
-#pragma unroll
-        for (int b = 0; b < HB; b++) r.w[b] = reinterpret_cast<const uint32_t *>(p)[b];
-    }
-    return r;
-}
 template <int HB> struct Halves {
     __half h[HB];
 };

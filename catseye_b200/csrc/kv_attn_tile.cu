@@ -10,8 +10,8 @@
 // turns: while one's probabilities are computed the other's products run.
 //
 // Roles: warps 0-3 and 4-7 the rows of the two tiles (they also bring Q in and
-// store O), warps 8-11 dequantize the cache's codes into the products' operand
-// layout (128-byte swizzle, two stages), warp 12 issues the products, warp 13
+// store O), warps 8-15 dequantize the cache's codes into the products' operand
+// layout (128-byte swizzle, two stages), warp 16 issues the products, warp 17
 // brings the codes to shared memory with bulk copies, three half tiles ahead.
 // (Codes loaded to registers a tile ahead made each proxy fence wait for them.)  The
 // codes are read once per 256 rows; the values (code - 8) * scale are exact in
@@ -48,6 +48,27 @@ template <int HS> struct TileSmem {
 
 enum TileBar { B_Q, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_O = B_P + 2, B_RF = B_O + 2, B_RE = B_RF + 3, B_N = B_RE + 3 };
 
+// A bounded wait for phase `n` (counted from 0) of a barrier; gives up, too, when
+// the CTA is unwinding.  No pause between the polls: they park the thread
+// themselves, and what waits here is on the critical path.
+__device__ __forceinline__ bool ti_wait(uint64_t *bar, uint32_t n, volatile int *abort_s, int *err, int code)
+{
+    for (uint32_t i = 0; i < CATS_SPIN_LIMIT; i++) {
+        if (mbar_try_wait(bar, n & 1)) return true;
+        if ((i & 15) == 15 && *abort_s) return false;
+    }
+    if (!*abort_s && err) atomicOr(err, code);
+    *abort_s = 1;
+    return false;
+}
+
+__device__ __forceinline__ bool ti_elect()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void ti_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
     asm volatile(
@@ -79,6 +100,14 @@ __device__ __forceinline__ void ti_ld32(uint32_t (&v)[32], uint32_t addr)
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
+__device__ __forceinline__ void ti_ld16(uint32_t (&v)[16], uint32_t addr)
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
 __device__ __forceinline__ void ti_st16(uint32_t addr, const uint32_t (&v)[16])
 {
     asm volatile(
@@ -89,6 +118,35 @@ __device__ __forceinline__ void ti_st16(uint32_t addr, const uint32_t (&v)[16])
 }
 __device__ __forceinline__ void ti_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ti_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A row's maximum has moved: its accumulator (o_cols columns, 0: none yet) and
+// the probabilities of this tile so far (done pieces of 16 columns) follow by
+// al.  Out of line: it runs once or twice a row, and the loop around it has to
+// fit the instruction cache.
+__device__ __noinline__ void ti_rescale(uint32_t O, int o_cols, uint32_t P, int done, float al)
+{
+    uint32_t v[16];
+#pragma unroll 1
+    for (int ch = 0; ch < o_cols; ch += 16) {
+        ti_ld16(v, O + ch);
+        ti_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * al);
+        ti_st16(O + ch, v);
+    }
+    ti_wait_st();
+#pragma unroll 1
+    for (int ch = 0; ch < done; ch++) {
+        ti_ld16(v, P + 16 * ch);
+        ti_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+            v[k] = kv_pack(f.x * al, f.y * al);
+        }
+        ti_st16(P + 16 * ch, v);
+    }
+}
 
 template <int HS>
 __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_constant__ KvAttn a)
@@ -102,7 +160,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     volatile int *hole = abort_s + 1;   // [4], by KV tile: pages of it that do not exist (bit 0, 1)
     volatile int *present = abort_s + 5;   // [3], by raw buffer: which of its two pages are in it
     uint32_t *slot = const_cast<uint32_t *>(reinterpret_cast<volatile uint32_t *>(abort_s + 8));
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
         mbar_init(&bar[B_Q], TI_SOFT);
@@ -208,10 +266,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int j = 0; j < n[i]; j++) {
-                ok = tc_wait(&bar[B_S + i], s_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                ok = ti_wait(&bar[B_S + i], s_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                s_it[i]++;
                 tc_fence_after();
                 const int p0 = j * TI_KV, holes = hole[(kv_it + j) & 3];
                 const bool edge = p0 + TI_KV - 1 > low[i] || holes;
@@ -219,52 +276,6 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     const int n = lim - (p0 + t) + 1;
                     return n <= 0 || (holes >> (t >> 6) & 1) ? 0u : n >= 32 ? ~0u : (1u << n) - 1;
                 };
-                float mx = -INFINITY;
-                if (!edge) {
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ch++) {
-                        uint32_t v[32];
-                        ti_ld32(v, S + 32 * ch);
-                        ti_wait_ld();
-                        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                        for (int k = 0; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
-                        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-                    }
-                } else {
-#pragma unroll 1
-                    for (int ch = 0; ch < 4; ch++) {
-                        uint32_t v[32];
-                        ti_ld32(v, S + 32 * ch);
-                        ti_wait_ld();
-                        const uint32_t bits = seen(32 * ch);
-#pragma unroll
-                        for (int k = 0; k < 32; k++)
-                            if (bits >> k & 1) mx = fmaxf(mx, __uint_as_float(v[k]));
-                    }
-                }
-                const float mn = mx * kf;
-                const bool move = mn > m + TI_LAG || (m == -INFINITY && mn > -INFINITY);
-                if (__any_sync(0xffffffffu, move)) {
-                    const float to = move ? mn : m, al = m == -INFINITY ? (move ? 0.f : 1.f) : kv_exp2(m - to);
-                    m = to;
-                    l *= al;
-                    if (j > 0) {   // the products so far are complete: S came after them
-#pragma unroll 1
-                        for (int ch = 0; ch < HS; ch += 32) {
-                            uint32_t v[32], w[16];
-                            ti_ld32(v, O + ch);
-                            ti_wait_ld();
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                                for (int k = 0; k < 16; k++) w[k] = __float_as_uint(__uint_as_float(v[16 * h + k]) * al);
-                                ti_st16(O + ch + 16 * h, w);
-                            }
-                        }
-                    }
-                }
-                const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
                 for (int ch = 0; ch < 4; ch++) {
@@ -277,6 +288,20 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                         for (int k = 0; k < 32; k++)
                             if (!(bits >> k & 1)) v[k] = 0xff800000u;   // -inf
                     }
+                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 32; k++) m4[k & 3] = fmaxf(m4[k & 3], __uint_as_float(v[k]));
+                    const float mn = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * kf;
+                    const bool far = mn > m + TI_LAG || (m == -INFINITY && mn > -INFINITY);
+                    if (__any_sync(0xffffffffu, far)) {
+                        const float al = far ? (m == -INFINITY ? 0.f : kv_exp2(m - mn)) : 1.f;
+                        l = (l + (sum[0] + sum[1]) + (sum[2] + sum[3])) * al;
+                        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+                        if (far) m = mn;
+                        // (the products so far are complete: S came after them)
+                        ti_rescale(O, j > 0 ? HS : 0, S, ch, al);
+                    }
+                    const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         const float e0 = kv_exp2(fmaf(__uint_as_float(v[k]), kf, ref)), e1 = kv_exp2(fmaf(__uint_as_float(v[k + 1]), kf, ref));
@@ -293,9 +318,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 if (lane == 0) mbar_arrive(&bar[B_P + i]);
             }
             if (ok && n[i] > 0) {
-                ok = tc_wait(&bar[B_O + i], o_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                ok = ti_wait(&bar[B_O + i], o_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
                 ok = __all_sync(0xffffffffu, ok);
-                o_it[i]++;
                 tc_fence_after();
             }
             const float inv = !ok || *abort_s ? NAN : l == 0.f ? 0.f : 1.f / l;
@@ -329,17 +353,29 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             const int kt = lane >> 2, kc = lane & 3;                       // K: token of 8, 16-byte piece of its codes
             const int vb = (lane >> 3) % HB, vx = (lane >> 3) / HB, vg = (lane >> 2) & 1, vi = lane & 3;
             const int vp = w >> 1, oct = 4 * (w & 1) + vi;                 // V: page of the tile, tokens 8 oct .. of it
-            constexpr int GH = HB;   // values of gh a lane takes: 4 / (4 / HB)
+            constexpr int GH = HB;   // eights of elements a lane takes
             bool ok = true;
             auto raw_unit = [&](uint32_t u) {
-                ok = tc_wait(&bar[B_RF + u % 3], (u / 3) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                ok = ti_wait(&bar[B_RF + u % 3], u / 3, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
                 ok = __all_sync(0xffffffffu, ok);
-                return sm + L::RAW + (u % 3) * L::RAW_UNIT;
+                return (int)(u % 3) * L::RAW_UNIT;
             };
             auto stage_free = [&](int b, uint32_t it) {
-                ok = tc_wait(&bar[b + (it & 1)], ((it >> 1) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                ok = ti_wait(&bar[b + (it & 1)], (it >> 1) + 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
                 ok = __all_sync(0xffffffffu, ok);
             };
+            // Where this lane reads and writes; what a loop adds is constant.  K: token 32w +
+            // 8u + kt, chunk 4b + kc; V: tokens 8 oct .., elements 32 vb + 4g + d with
+            // g = 2 (u * 4/HB + vx) + vg.  The swizzle's row bits are the lane's own.
+            const uint8_t *k_code = sm + L::RAW + (w >> 1) * 32 * HS + ((32 * (w & 1) + kt) * 4 + kc) * 4 * HB;
+            const uint8_t *k_scale = sm + L::RAW + 64 * HS + (w >> 1) * 4 * HS + (32 * (w & 1) + kt) * 2 * HB;
+            const uint8_t *v_code = sm + L::RAW + vp * 32 * HS + ((4 * oct * 8 + 2 * vx + vg) * HB + vb) * 4;
+            const uint8_t *v_scale = sm + L::RAW + 64 * HS + vp * 4 * HS + (4 * oct * HB + vb) * 4;
+            uint8_t *k_dst = sm + L::K + (32 * w + kt) * 128, *v_dst = sm + L::V + vp * L::V_PAGE + (32 * vb + 8 * vx + 4 * vg) * 128;
+            const int k_at[2] = {(kc ^ kt) * 16, ((4 + kc) ^ kt) * 16};
+            int v_at[4];
+#pragma unroll
+            for (int d = 0; d < 4; d++) v_at[d] = d * 128 + (oct ^ (4 * vg + d)) * 16;
             auto arrive = [&](uint64_t *bp) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bp);
@@ -348,84 +384,59 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 const uint32_t it = kv_it + j, u0 = 2 * it;
                 const int st = it & 1, p0 = j * TI_KV;
                 // ---- K: warp w takes tokens 32w .. 32w + 31 of the tile
-                const uint8_t *raw = raw_unit(u0);
+                int raw = raw_unit(u0);
                 if (!ok) break;
                 const int there = present[u0 % 3];
-                uint32_t kw[4][HB], ks[4][HB / 2];
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int t = 32 * (w & 1) + 8 * u + kt;
-                    const uint8_t *code = raw + (w >> 1) * 32 * HS + (t * 4 + kc) * 4 * HB;
-                    const uint8_t *scale = raw + 64 * HS + (w >> 1) * 4 * HS + t * 2 * HB;
-                    if constexpr (HB == 4) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(code);
-                        kw[u][0] = v.x; kw[u][1] = v.y; kw[u][2] = v.z; kw[u][3] = v.w;
-                        const uint2 s = *reinterpret_cast<const uint2 *>(scale);
-                        ks[u][0] = s.x; ks[u][1] = s.y;
-                    } else {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(code);
-                        kw[u][0] = v.x; kw[u][1] = v.y;
-                        ks[u][0] = *reinterpret_cast<const uint32_t *>(scale);
-                    }
-                }
-                arrive(&bar[B_RE + u0 % 3]);
                 stage_free(B_KE, it);
                 if (!ok) break;
                 // (read until P(it + 1) is there, written again after it)
                 if (w == 0 && lane == 0) hole[it & 3] = ~there & ((p0 <= top) | (p0 + KV_PAGE <= top) << 1);
                 if (there >> (w >> 1) & 1) {
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const int rowi = 32 * w + 8 * u + kt;
+#pragma unroll 1
+                    for (int u = 0; u < 4; u++) {   // rolled, as below: the roles' loops share the instruction cache
+                        const Words<HB> kw = lds_words<HB>(k_code + raw + u * 128 * HB);
+                        const Words<HB / 2> ks = lds_words<HB / 2>(k_scale + raw + u * 16 * HB);
+                        uint8_t *dst = k_dst + st * L::K_STAGE + u * 1024;
 #pragma unroll
                         for (int b = 0; b < HB; b++) {
                             uint32_t x[4];
-                            const __half2 two = *reinterpret_cast<const __half2 *>(&ks[u][b / 2]);
-                            kv_dequant(kw[u][b], b & 1 ? __high2half2(two) : __low2half2(two), magic, x);
-                            const int ci = 4 * b + kc;
-                            *reinterpret_cast<uint4 *>(sm + L::K + st * L::K_STAGE + (ci >> 3) * L::SLICE + sw128(rowi, ci & 7)) =
-                                make_uint4(x[0], x[1], x[2], x[3]);
+                            const __half2 two = *reinterpret_cast<const __half2 *>(&ks.w[b / 2]);
+                            kv_dequant(kw.w[b], b & 1 ? __high2half2(two) : __low2half2(two), magic, x);
+                            *reinterpret_cast<uint4 *>(dst + k_at[b & 1] + (b >> 1) * L::SLICE) = make_uint4(x[0], x[1], x[2], x[3]);
                         }
                     }
                 }
+                arrive(&bar[B_RE + u0 % 3]);
                 fence_proxy_async_smem();
                 arrive(&bar[B_KF + st]);
                 // ---- V: 8 tokens of page vp, elements 32 vb + 4 g + .. for g = 2 gh + vg
                 raw = raw_unit(u0 + 1);
                 if (!ok) break;
                 const bool v_there = present[(u0 + 1) % 3] >> vp & 1;
-                uint32_t vw[GH][4], vs[4];
+                stage_free(B_VE, it);
+                if (!ok) break;
+                uint32_t vs[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    vs[k] = *reinterpret_cast<const uint32_t *>(raw + 64 * HS + vp * 4 * HS + ((4 * oct + k) * HB + vb) * 4);
+                    vs[k] = *reinterpret_cast<const uint32_t *>(v_scale + raw + k * 4 * HB);
                     // what nobody sees, or nobody wrote, may read as NaN
                     const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
                     if (p0 + TI_KV - 1 > top) vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
                     if (!v_there) vs[k] = 0u;
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < GH; u++) {
-                    const int g = 2 * (u * (4 / HB) + vx) + vg;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        vw[u][k] = *reinterpret_cast<const uint32_t *>(raw + vp * 32 * HS + (((4 * oct + k) * 8 + g) * HB + vb) * 4);
-                }
-                arrive(&bar[B_RE + (u0 + 1) % 3]);
-                stage_free(B_VE, it);
-                if (!ok) break;
-#pragma unroll
-                for (int u = 0; u < GH; u++) {
-                    const int g = 2 * (u * (4 / HB) + vx) + vg;
                     uint32_t x[4][4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) kv_dequant(vw[u][k], *reinterpret_cast<const __half2 *>(&vs[k]), magic, x[k]);
-#pragma unroll
-                    for (int d = 0; d < 4; d++) {
-                        const int dim = 32 * vb + 4 * g + d;
-                        *reinterpret_cast<uint4 *>(sm + L::V + st * L::V_STAGE + vp * L::V_PAGE + sw128(dim, oct)) =
-                            make_uint4(x[0][d], x[1][d], x[2][d], x[3][d]);
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t vw = *reinterpret_cast<const uint32_t *>(v_code + raw + (k * 8 + u * (8 / HB)) * 4 * HB);
+                        kv_dequant(vw, *reinterpret_cast<const __half2 *>(&vs[k]), magic, x[k]);
                     }
+                    uint8_t *dst = v_dst + st * L::V_STAGE + u * (4 / HB) * 1024;
+#pragma unroll
+                    for (int d = 0; d < 4; d++) *reinterpret_cast<uint4 *>(dst + v_at[d]) = make_uint4(x[0][d], x[1][d], x[2][d], x[3][d]);
                 }
+                arrive(&bar[B_RE + (u0 + 1) % 3]);
                 fence_proxy_async_smem();
                 arrive(&bar[B_VF + st]);
             }
@@ -441,7 +452,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     for (int v = 0; v < 2 && ok; v++) {
                         const uint32_t u = 2 * (kv_it + j) + v;
                         uint64_t *full = &bar[B_RF + u % 3];
-                        ok = tc_wait(&bar[B_RE + u % 3], ((u / 3) & 1) ^ 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                        ok = ti_wait(&bar[B_RE + u % 3], u / 3 + 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
                         if (!ok) break;
                         const int there = (pg[0] >= 0) | (pg[1] >= 0) << 1;
                         issued = u + 1;
@@ -466,46 +477,67 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 for (uint32_t u = issued < 3 ? 0 : issued - 3; !ok && u < issued; u++)
                     mbar_wait_bounded(&bar[B_RF + u % 3], (u / 3) & 1, nullptr, 0);
             }
-        } else if (lane == 0) {
+        } else {
             // ------------------------------------------------ products
+            // The whole warp runs this, one elected lane issues: what the instructions
+            // take stays in uniform registers.  (From one lane's own branch an issue took
+            // 90 cycles.)
             constexpr uint32_t id_qk = umma_idesc(0, 128, TI_KV), id_pv = umma_idesc(0, 128, HS);
-            const uint32_t q_at = smem_u32(sm), k_at = smem_u32(sm + L::K), v_at = smem_u32(sm + L::V);
-            auto qk = [&](int i, int st) {
+            const uint64_t q_d = umma_desc_sw128(smem_u32(sm)), k_d = umma_desc_sw128(smem_u32(sm + L::K)),
+                           v_d = umma_desc_sw128(smem_u32(sm + L::V));   // + bytes / 16
+            bool ok = true;
+            auto qk = [&](int i, uint32_t it) {
+                const uint64_t qi = q_d + i * (L::Q_TILE / 16), ks = k_d + (it & 1) * (L::K_STAGE / 16);
+                if (ti_elect()) {
 #pragma unroll
-                for (int k = 0; k < HS / 16; k++)
-                    ti_mma_ss(tmem + 128 * i, umma_desc_sw128(q_at + i * L::Q_TILE + (k >> 2) * L::SLICE + (k & 3) * 32),
-                              umma_desc_sw128(k_at + st * L::K_STAGE + (k >> 2) * L::SLICE + (k & 3) * 32), id_qk, k > 0);
-                ti_commit(&bar[B_S + i]);
+                    for (int k = 0; k < HS / 16; k++)
+                        ti_mma_ss(tmem + 128 * i, qi + ((k >> 2) * L::SLICE + (k & 3) * 32) / 16,
+                                  ks + ((k >> 2) * L::SLICE + (k & 3) * 32) / 16, id_qk, k > 0);
+                    ti_commit(&bar[B_S + i]);
+                }
+                __syncwarp();
             };
-            bool ok = tiles == 0 || tc_wait(&bar[B_Q], q_it & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
-            if (ok && tiles > 0) ok = tc_wait(&bar[B_KF + (kv_it & 1)], (kv_it >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
-            if (ok && tiles > 0) {
+            auto k_full = [&](uint32_t it) {
+                if (ok) ok = ti_wait(&bar[B_KF + (it & 1)], it >> 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
-                for (int i = 0; i < 2; i++)
-                    if (n[i] > 0) qk(i, kv_it & 1);
-                ti_commit(&bar[B_KE + (kv_it & 1)]);
+            };
+            if (tiles > 0) {
+                ok = ti_wait(&bar[B_Q], q_it, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                k_full(kv_it);
+                for (int i = 0; i < 2 && ok; i++)
+                    if (n[i] > 0) qk(i, kv_it);
+                if (ok && ti_elect()) ti_commit(&bar[B_KE + (kv_it & 1)]);
+                __syncwarp();
             }
             for (int j = 0; j < tiles && ok; j++) {
                 const uint32_t it = kv_it + j;
-                const int st = it & 1, nx = st ^ 1;
-                ok = tc_wait(&bar[B_VF + st], (it >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
-                if (ok && j + 1 < tiles) ok = tc_wait(&bar[B_KF + nx], ((it + 1) >> 1) & 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
-                for (int i = 0; i < 2 && ok; i++) {
-                    if (j >= n[i]) continue;
-                    ok = tc_wait(&bar[B_P + i], s_it[i] & 1, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
-                    if (!ok) break;
-                    s_it[i]++;
-                    tc_fence_after();
+                ok = ti_wait(&bar[B_VF + (it & 1)], it >> 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                if (j + 1 < tiles) k_full(it + 1);
+                const uint64_t vs = v_d + (it & 1) * (L::V_STAGE / 16);
 #pragma unroll
-                    for (int k = 0; k < TI_KV / 16; k++)
-                        ti_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k,
-                                  umma_desc_sw128(v_at + st * L::V_STAGE + (k >> 2) * L::V_PAGE + (k & 3) * 32), id_pv, j > 0 || k > 0);
-                    if (j + 1 < n[i]) qk(i, nx);
-                    else ti_commit(&bar[B_O + i]);
+                for (int i = 0; i < 2; i++) {
+                    if (j >= n[i] || !ok) continue;
+                    ok = ti_wait(&bar[B_P + i], s_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    if (ti_elect()) {
+#pragma unroll
+                        for (int k = 0; k < TI_KV / 16; k++)
+                            ti_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, vs + ((k >> 2) * L::V_PAGE + (k & 3) * 32) / 16, id_pv,
+                                      j > 0 || k > 0);
+                        if (j + 1 == n[i]) ti_commit(&bar[B_O + i]);
+                    }
+                    __syncwarp();
+                    if (j + 1 < n[i]) qk(i, it + 1);
                 }
                 if (!ok) break;
-                ti_commit(&bar[B_VE + st]);
-                if (j + 1 < tiles) ti_commit(&bar[B_KE + nx]);
+                if (ti_elect()) {
+                    ti_commit(&bar[B_VE + (it & 1)]);
+                    if (j + 1 < tiles) ti_commit(&bar[B_KE + ((it + 1) & 1)]);
+                }
+                __syncwarp();
             }
         }
         kv_it += tiles;
