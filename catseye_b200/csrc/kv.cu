@@ -7,75 +7,84 @@
 namespace cats {
 
 // ------------------------------------------------------- rows in and out
-template <class T> __device__ __forceinline__ float kv_to_float(T v);
-template <> __device__ __forceinline__ float kv_to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float kv_to_float<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float kv_to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T kv_from_float(float v);
-template <> __device__ __forceinline__ float kv_from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half kv_from_float<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 kv_from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <class T> struct alignas(4 * sizeof(T)) Vec4 { T v[4]; };
-
-template <class T> __device__ __forceinline__ void load4(const T *p, bool vec, float (&x)[4])
+// A thread takes eight elements (a word of K codes) of the two tokens of a
+// pair (whose V codes share words): four neighbours hold a block of 32.
+// APPEND: rows -> blocks; else blocks -> rows.  Rows of k (side 0) and v (side
+// 1) of the runs: grid.x over a row's eights, grid.y over the pairs, grid.z
+// over the runs.  What a thread's column is, is settled once; then it goes
+// down the pairs.
+//
+// Bound by HBM for long prompts: in 2 * hs * size, out 2 * hs * 4.5 bits a
+// token and head.
+template <int type, bool APPEND>
+__global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvView c, const __grid_constant__ KvRows k,
+                                                    const __grid_constant__ KvRows v, const KvRun *__restrict__ runs,
+                                                    int n_runs)
 {
-    if (vec) {
-        const Vec4<T> t = *reinterpret_cast<const Vec4<T> *>(p);
+    const int per_head = c.hs >> 3, per_side = per_head * c.n_kv;
+    const unsigned mask = 0xfu << (threadIdx.x & 28);
+    const KvMagic magic = kv_magic();
+    for (int col = blockIdx.x * 256 + threadIdx.x; col < 2 * per_side; col += gridDim.x * 256) {
+        const bool is_v = col >= per_side;
+        const int e1 = is_v ? col - per_side : col, head = e1 / per_head, e8 = e1 - head * per_head;
+        const KvRows &t = is_v ? v : k;
+        for (int ri = blockIdx.z; ri < n_runs; ri += gridDim.z) {
+            const KvRun run = runs[ri];
+            const int2 span = kv_run_rows(run, k.rows, c.err);
+            if (span.x >= span.y) continue;
+            const long long end = (long long)run.pos + span.y;
+            for (long long pair = (((long long)run.pos + span.x) >> 1) + blockIdx.y; 2 * pair < end; pair += gridDim.y) {
+                // tokens 2 pair, 2 pair + 1: in the run?
+                const long long r0 = 2 * pair - run.pos;
+                const bool in[2] = {r0 >= span.x, r0 + 1 < span.y};
+                const size_t at = (size_t)(run.first + r0) * t.ld + (size_t)head * c.hs + 8 * e8;
+                const int slot = (int)(2 * pair & (KV_PAGE - 1));
+                float x[2][8];
+                if constexpr (APPEND) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = kv_to_float<T>(t.v[j]);
-    } else {
+                    for (int u = 0; u < 2; u++) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = kv_to_float<T>(p[j]);
-    }
-}
-
-template <class T> __device__ __forceinline__ void store4(T *p, bool vec, const float (&x)[4])
-{
-    Vec4<T> t;
-#pragma unroll
-    for (int j = 0; j < 4; j++) t.v[j] = kv_from_float<T>(x[j]);
-    if (vec) {
-        *reinterpret_cast<Vec4<T> *>(p) = t;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++) p[j] = t.v[j];
-    }
-}
-
-// A thread takes four elements of a row: eight neighbours hold a block of 32.
-// APPEND: row -> blocks; else blocks -> row.  Rows of k (side 0) and v (side 1)
-// of one run: grid.x over its rows, grid.y over the runs.
-template <class T, bool APPEND>
-__global__ void __launch_bounds__(256) k_kv_rows(const __grid_constant__ KvView c, const __grid_constant__ KvRows k,
-                                                 const __grid_constant__ KvRows v, const KvRun *__restrict__ runs,
-                                                 int n_runs)
-{
-    const int per_head = c.hs >> 2, per_side = per_head * c.n_kv, per_row = 2 * per_side;
-    const unsigned mask = 0xffu << (threadIdx.x & 24);
-    for (int ri = blockIdx.y; ri < n_runs; ri += gridDim.y) {
-        const KvRun run = runs[ri];
-        const int2 span = kv_run_rows(run, k.rows, c.err);
-        const long long items = (long long)(span.y - span.x) * per_row;
-        for (long long i = blockIdx.x * 256LL + threadIdx.x; i < items; i += gridDim.x * 256LL) {
-            const int r = span.x + (int)(i / per_row), e = (int)(i % per_row);
-            const bool is_v = e >= per_side;
-            const int e1 = is_v ? e - per_side : e, head = e1 / per_head, e4 = e1 - head * per_head;
-            const KvRows &t = is_v ? v : k;
-            const long long pos = (long long)run.pos + r;
-            const int page = c.page(run.seq, pos < 0 ? -1 : (int)min(pos / KV_PAGE, (long long)INT_MAX));
-            T *p = static_cast<T *>(t.p) + (size_t)(run.first + r) * t.ld + (size_t)head * c.hs + 4 * e4;
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (APPEND) {
-                if (page < 0) continue;
-                load4<T>(p, t.vec, x);
-                kv_store4(c.chunk(page, head), is_v, c.hs, (int)(pos % KV_PAGE), e4, x, mask);
-            } else {
-                if (page >= 0) {
-                    const float4 f = kv_load4(c.chunk(page, head), is_v, c.hs, (int)(pos % KV_PAGE), e4);
-                    x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+                        for (int j = 0; j < 8; j++) x[u][j] = 0.f;
+                        if (in[u]) kv_load_row<8>(t, type, at + (u ? t.ld : 0), x[u]);   // (does not wait for the table)
+                    }
                 }
-                store4<T>(p, t.vec, x);
+                const int page = c.page(run.seq, pair < 0 ? -1 : (int)min(pair / (KV_PAGE / 2), (long long)INT_MAX));
+                uint8_t *ch = c.chunk(max(page, 0), head);
+                if constexpr (APPEND) {
+                    if (page < 0) continue;
+                    uint32_t codes[2];
+                    uint16_t scale[2];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) codes[u] = kv_quant8(x[u], mask, &scale[u]);
+                    if (is_v && in[0] && in[1]) {
+                        kv_store_pair8(ch, c.hs, slot, e8, codes[0], codes[1], scale[0], scale[1]);
+                        continue;
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        if (in[u]) kv_store_codes8(ch, is_v, c.hs, slot + u, e8, codes[u], scale[u]);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        if (!in[u]) continue;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) x[u][j] = 0.f;
+                        if (page >= 0) {
+                            uint32_t h[4];
+                            kv_dequant(kv_codes8(ch, is_v, c.hs, slot + u, e8),
+                                       __half2half2(kv_scale8(ch, is_v, c.hs, slot + u, e8)), magic, h);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+                                x[u][j] = f.x;
+                                x[u][j + 4] = f.y;
+                            }
+                        }
+                        const size_t to = at + (u ? t.ld : 0);
+                        kv_store_row4(t, type, to, make_float4(x[u][0], x[u][1], x[u][2], x[u][3]));
+                        kv_store_row4(t, type, to + 4, make_float4(x[u][4], x[u][5], x[u][6], x[u][7]));
+                    }
+                }
             }
         }
     }
@@ -85,12 +94,15 @@ template <bool APPEND>
 static cudaError_t launch_rows(const KvView &c, int type, const KvRows &k, const KvRows &v, const KvBatch &b,
                                cudaStream_t st)
 {
-    const long long items = (long long)std::max(b.max_rows, 1) * c.n_kv * (c.hs / 2);
-    const dim3 grid((unsigned)std::min<long long>((items + 255) / 256, 4096), (unsigned)std::min(b.n_runs, 32768));
+    const int cols = (int)std::min<long long>(((long long)c.n_kv * (c.hs / 4) + 255) / 256, 1024);
+    // some eight CTAs an SM in all, each going down its rows
+    const int runs = std::min(b.n_runs, 32768), rows = std::max(b.max_rows, 1) / 2 + 1;   // pairs
+    const long long down = std::max<long long>(1, 148ll * 16 / std::max<long long>(1, (long long)cols * runs));
+    const dim3 grid((unsigned)cols, (unsigned)std::min<long long>(rows, std::min<long long>(down, 65535)), (unsigned)runs);
     switch (type) {
-    case KV_F32: k_kv_rows<float, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
-    case KV_F16: k_kv_rows<__half, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
-    case KV_BF16: k_kv_rows<__nv_bfloat16, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
+    case KV_F32: k_kv_rows<KV_F32, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
+    case KV_F16: k_kv_rows<KV_F16, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
+    case KV_BF16: k_kv_rows<KV_BF16, APPEND><<<grid, 256, 0, st>>>(c, k, v, b.runs, b.n_runs); break;
     default: return cudaErrorInvalidValue;
     }
     return cudaGetLastError();

@@ -91,44 +91,96 @@ __device__ __forceinline__ int kv_scale_off(bool is_v, int hs, int slot, int b)
     return is_v ? 68 * hs + (((slot >> 1) * hb + b) * 2 + (slot & 1)) * 2 : 64 * hs + (slot * hb + b) * 2;
 }
 
-// Quantize a block of 32 held four elements a lane by eight consecutive lanes
-// (mask: those lanes), and store it at (chunk, slot).  The code is floor(x/d +
-// 1/2) + 8, decided exactly: (q +- 1/2) * d has at most 13 significant bits,
-// so comparing x with it in fp32 settles what the approximate quotient
-// cannot.  A block with a NaN or an infinity reads back as NaN.
-__device__ __forceinline__ void kv_store4(uint8_t *chunk, bool is_v, int hs, int slot, int e4, const float (&x)[4],
-                                          unsigned mask)
+// Quantize a block of 32 held eight elements a lane by four consecutive lanes
+// (mask: those lanes): this lane's codes (element j in nibble j), the scale.
+// The code is floor(x/d + 1/2) + 8, decided exactly: q * d has at most 12
+// significant bits and a last place above x's, so r = x - q d is exact in
+// fp32.  q comes from an approximate quotient; where every |r| <= |d| / 2 it
+// is the nearest code (the next one up at + |d| / 2), and else (beside a border,
+// or a scale that is saturated or subnormal) the lane decides its eight one by
+// one.  A block with
+// a NaN or an infinity reads back as NaN.
+__device__ __forceinline__ uint32_t kv_quant8(const float (&x)[8], unsigned mask, uint16_t *scale)
 {
-    float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-    // NaN and infinity: x - x is 0 for every finite x
-    const float z = (x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]);
+    float hi = x[0], lo = x[0], z = 0.f;   // z: 0 * x is 0 for every finite x
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        hi = fmaxf(hi, x[j]);
+        lo = fminf(lo, x[j]);
+        z = fmaf(x[j], 0.f, z);
+    }
     const bool bad = __any_sync(mask, !(z == 0.f)) != 0;
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
+    for (int o = 1; o < 4; o <<= 1) {
         hi = fmaxf(hi, __shfl_xor_sync(mask, hi, o));
         lo = fminf(lo, __shfl_xor_sync(mask, lo, o));
     }
     const float m = hi >= -lo ? hi : lo;
-    float d = __bfloat162float(__float2bfloat16_rn(m * -0.125f));
-    const __half dh = __float2half_rn(fminf(fmaxf(d, -8160.f), 8160.f));
-    d = __half2float(dh);
-    unsigned codes = 0x8888u;
-    if (!bad && d != 0.f) {
-        const float da = fabsf(d), inv = 1.f / da;
-        codes = 0u;
+    const __half dh = __float2half_rn(fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(m * -0.125f)), -8160.f), 8160.f));
+    const float d = __half2float(dh), da = fabsf(d), half = 0.5f * da;
+    *scale = bad ? 0x7fff : __half_as_ushort(dh);
+    if (bad || d == 0.f) return 0x88888888u;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(da));
+    const float sign = d < 0.f ? -1.f : 1.f;
+    constexpr float BIG = 12582912.f;   // 1.5 * 2^23: a sum with it rounds to an integer
+    float sum[2] = {0.f, 0.f}, off = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float xs = d < 0.f ? -x[j] : x[j];
-            float q = floorf(fminf(fmaxf(xs * inv, -8.f), 7.f) + 0.5f);
-            if (xs >= (q + 0.5f) * da) q += 1.f;
-            else if (xs < (q - 0.5f) * da) q -= 1.f;
-            const int code = (int)fminf(fmaxf(q, -8.f), 7.f) + 8;
-            codes |= (unsigned)code << (4 * j);
+    for (int j = 7; j >= 0; j--) {
+        const float xs = x[j] * sign, q = fmaf(xs, inv, BIG) - BIG, r = fmaf(-q, da, xs);
+        off = fmaxf(off, fabsf(r));
+        sum[j >> 2] = fmaf(sum[j >> 2], 16.f, fminf(r >= half ? q + 1.f : q, 7.f));   // four codes (16 bits of x have many ties)
+    }
+    if (off > half || fabsf(m) * inv > 8.4f) {
+        sum[0] = sum[1] = 0.f;
+#pragma unroll 1
+        for (int j = 7; j >= 0; j--) {
+            float xj = x[0];
+#pragma unroll
+            for (int k = 1; k < 8; k++) xj = k == j ? x[k] : xj;
+            const float xs = xj * sign;
+            float q = fmaf(fminf(fmaxf(xs * inv, -9.f), 9.f), 1.f, BIG) - BIG;
+            const float r = fmaf(-q, da, xs);
+            q = r >= half ? q + 1.f : r < -half ? q - 1.f : q;
+            q = fminf(fmaxf(q, -8.f), 7.f);
+            if (j >= 4) sum[1] = fmaf(sum[1], 16.f, q);
+            else sum[0] = fmaf(sum[0], 16.f, q);
         }
     }
-    *reinterpret_cast<uint16_t *>(chunk + kv_code_off(is_v, hs, slot, e4)) = (uint16_t)codes;
-    if ((e4 & 7) == 0)
-        *reinterpret_cast<__half *>(chunk + kv_scale_off(is_v, hs, slot, e4 >> 3)) = bad ? __ushort_as_half(0x7fff) : dh;
+    // + 8 for every code: the codes are the low 16 bits of an integer above 2^23
+    return (__float_as_uint(sum[0] + (34952.f + 8388608.f)) & 0xffffu) | __float_as_uint(sum[1] + (34952.f + 8388608.f)) << 16;
+}
+// ... and where a row's eight e8 go (K: one word; V: half of two words)
+__device__ __forceinline__ void kv_store_codes8(uint8_t *chunk, bool is_v, int hs, int slot, int e8, uint32_t codes, uint16_t scale)
+{
+    uint8_t *p = chunk + kv_code_off(is_v, hs, slot, 2 * e8);
+    if (is_v) {
+        *reinterpret_cast<uint16_t *>(p) = (uint16_t)codes;
+        *reinterpret_cast<uint16_t *>(p + (hs >> 3)) = (uint16_t)(codes >> 16);   // the next g: 4 * HB bytes on
+    } else {
+        *reinterpret_cast<uint32_t *>(p) = codes;
+    }
+    if ((e8 & 3) == 0) *reinterpret_cast<uint16_t *>(chunk + kv_scale_off(is_v, hs, slot, e8 >> 2)) = scale;
+}
+// V of the two tokens of a pair (slot even): whole words
+__device__ __forceinline__ void kv_store_pair8(uint8_t *chunk, int hs, int slot, int e8, uint32_t c0, uint32_t c1, uint16_t s0, uint16_t s1)
+{
+    uint8_t *p = chunk + kv_code_off(true, hs, slot, 2 * e8);
+    *reinterpret_cast<uint32_t *>(p) = __byte_perm(c0, c1, 0x5410);
+    *reinterpret_cast<uint32_t *>(p + (hs >> 3)) = __byte_perm(c0, c1, 0x7632);
+    if ((e8 & 3) == 0) *reinterpret_cast<uint32_t *>(chunk + kv_scale_off(true, hs, slot, e8 >> 2)) = s0 | (uint32_t)s1 << 16;
+}
+
+// The codes of eight elements of a stored row (element j in nibble j), and their scale.
+__device__ __forceinline__ uint32_t kv_codes8(const uint8_t *chunk, bool is_v, int hs, int slot, int e8)
+{
+    const uint8_t *p = chunk + kv_code_off(is_v, hs, slot, 2 * e8);
+    return is_v ? *reinterpret_cast<const uint16_t *>(p) | (uint32_t)*reinterpret_cast<const uint16_t *>(p + (hs >> 3)) << 16
+                : *reinterpret_cast<const uint32_t *>(p);
+}
+__device__ __forceinline__ __half kv_scale8(const uint8_t *chunk, bool is_v, int hs, int slot, int e8)
+{
+    return *reinterpret_cast<const __half *>(chunk + kv_scale_off(is_v, hs, slot, e8 >> 2));
 }
 
 // four elements 4*e4 .. of a stored row
