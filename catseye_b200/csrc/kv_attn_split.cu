@@ -124,7 +124,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
     const KvMagic magic = kv_magic();
 
     int ri, kvh, entry = 0, at = 0, steps = 0;   // STREAM: entry = run * tiles + tile; steps at .. of it come next
-    long long tile, left = 0, total = 0, begin = 0;
+    long long tile, left = 0, total = 0, begin = 0, end = 0, ctas = 1;   // ctas: those that have a stretch
     bool beyond = false;   // STREAM: some run has more row tiles than the launch counted on
     if constexpr (STREAM) {
         long long *pre = reinterpret_cast<long long *>(smem);   // steps before each entry; then the warps' sums
@@ -158,8 +158,12 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
             __syncthreads();
         }
         beyond = __syncthreads_or(beyond) != 0;
-        begin = total * blockIdx.x / gridDim.x;
-        left = total * (blockIdx.x + 1) / gridDim.x - begin;
+        ctas = max(1ll, min((long long)gridDim.x, total));   // a step each at least: no CTA between two of a unit's is idle
+        if (blockIdx.x < ctas) {
+            begin = total * blockIdx.x / ctas;
+            end = total * (blockIdx.x + 1) / ctas;
+            left = end - begin;
+        }
         int hi = entries;   // the entry that holds step `begin`: the last with pre <= begin
         while (hi - entry > 1) {
             const int mid = (entry + hi) / 2;
@@ -562,9 +566,9 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 }
             }
             if (tid == 0) {
-                const long long start = total * (blockIdx.x + 1) / gridDim.x - left - now - at;   // the unit's first step
-                const int owner = (int)(((start + 1) * gridDim.x - 1) / total);
-                const int last = (int)(((start + steps) * gridDim.x - 1) / total);
+                const long long start = end - left - now - at;   // the unit's first step
+                const int owner = (int)(((start + 1) * ctas - 1) / total);
+                const int last = (int)(((start + steps) * ctas - 1) / total);
                 wk.split[2 * blockIdx.x + (at == 0)] = make_int4(entry, kvh, owner, last - owner + 1);
             }
         } else if (STREAM || C == 1) {
@@ -615,7 +619,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
 
 // The units that lie in several CTAs' stretches.  Block i looks at CTA i's two:
 // as the k-th of a unit's P CTAs it joins rows k, k + P, ...: a warp a row, or,
-// past eight parts, the row its warps share, every eighth part each.
+// past eight parts, one after the other, its warps taking every eighth part.
 template <int ROWS>
 __global__ void __launch_bounds__(256, 4) k_kv_attn_join(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork wk)
 {
@@ -628,38 +632,36 @@ __global__ void __launch_bounds__(256, 4) k_kv_attn_join(const __grid_constant__
         if (sp.w == 0) continue;
         const int owner = sp.z, P = sp.w, k0 = (int)blockIdx.x - owner;
         const bool shared = P > 8;
-        const int r = shared ? k0 : k0 + P * y;
-        if (shared ? r >= ROWS : false) continue;
         const KvRun run = a.runs[sp.x / a.tiles];
         const int2 span = kv_run_rows(run, a.q.rows, nullptr);
-        const long long rr = (long long)(sp.x % a.tiles) * ROWS + r;
-        const bool real = r < ROWS && rr < (long long)(span.y - span.x) * a.mul;
-        float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float mp, float lp, const float4 &v) {
-            const float mn = fmaxf(m, mp);
-            const float f = m == -INFINITY ? 0.f : kv_exp2(m - mn), g = mp == -INFINITY ? 0.f : kv_exp2(mp - mn);
-            m = mn;
-            l = l * f + lp * g;
-            acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
-        };
-        if (real) {
+        const long long r0 = (long long)(sp.x % a.tiles) * ROWS;
+        const int used = (int)min((long long)ROWS, (long long)(span.y - span.x) * a.mul - r0);
+        for (int r = shared ? k0 : k0 + P * y; r < used; r += shared ? P : 8 * P) {
+            float m = -INFINITY, l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            auto add = [&](float mp, float lp, const float4 &v) {
+                const float mn = fmaxf(m, mp);
+                const float f = m == -INFINITY ? 0.f : kv_exp2(m - mn), g = mp == -INFINITY ? 0.f : kv_exp2(mp - mn);
+                m = mn;
+                l = l * f + lp * g;
+                acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
+            };
 #pragma unroll 4
             for (int k = shared ? y : 0; k < P; k += shared ? 8 : 1) {
                 const float *p = wk.part + (size_t)(2 * (owner + k) + (k == 0)) * sp_part(ROWS, hs);
                 const float4 v = 4 * x < hs ? *reinterpret_cast<const float4 *>(p + r * hs + 4 * x) : make_float4(0.f, 0.f, 0.f, 0.f);
                 add(p[ROWS * hs + r], p[ROWS * hs + ROWS + r], v);
             }
+            if (shared) {
+                __syncthreads();   // the row before is done with them
+                so[y][x] = acc;
+                if (x == 0) sm[y] = make_float2(m, l);
+                __syncthreads();
+                if (y > 0) continue;
+                for (int k = 1; k < 8; k++) add(sm[k].x, sm[k].y, so[k][x]);
+            }
+            if (4 * x < hs) finish4(a, run, span, sp.y, r0 + r, x, acc, l);
         }
-        if (shared) {
-            __syncthreads();   // the slot before is done with them
-            so[y][x] = acc;
-            if (x == 0) sm[y] = make_float2(m, l);
-            __syncthreads();
-            if (y > 0) continue;
-            for (int k = 1; k < 8; k++) add(sm[k].x, sm[k].y, so[k][x]);
-        }
-        if (real && 4 * x < hs) finish4(a, run, span, sp.y, rr, x, acc, l);
     }
 }
 

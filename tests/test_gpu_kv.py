@@ -299,6 +299,99 @@ def test_prompt_attention(dtype, hs, n_kv, mul, new, lens):
     check_attention(c, 0, q, out, runs, mul, untouched=3)
 
 
+# A context of LONG tokens is planned as equal stretches over the whole GPU
+# and a second kernel that joins them, whatever the runs' true lengths are.
+LONG = 1_000_000
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hs,n_kv,mul", [(32, 2, 1), (64, 1, 3), (96, 2, 4), (128, 2, 1), (128, 1, 8), (128, 1, 20)])
+@pytest.mark.parametrize("lens", DECODE + [[5000, 1, 700]])
+def test_decode_attention_in_stretches(dtype, hs, n_kv, mul, lens):
+    c = make(lens, n_kv, hs)
+    fill(c, lens)
+    q, out, runs = attend(c, 1, [1] * len(lens), lens, mul, dtype, hints=(1, LONG))
+    check_attention(c, 1, q, out, runs, mul, untouched=3)
+    assert _lib.load().cats_gpu_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hint", [1, 3, 100])
+@pytest.mark.parametrize("new,lens", [([2], [2]), ([33, 0, 1, 7], [33, 40, 150, 71]), ([1, 90, 20], [400, 90, 1000])])
+def test_rows_in_stretches(dtype, hint, new, lens):
+    """Runs of more and of fewer rows than the hint says, beside empty ones."""
+    c = make(lens, 2, 64)
+    fill(c, lens)
+    q, out, runs = attend(c, 0, new, lens, 2, dtype, hints=(hint, LONG))
+    check_attention(c, 0, q, out, runs, 2, untouched=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_stretches_with_holes_and_what_is_masked(dtype):
+    """Missing pages, rows before position 0, a batch of empty runs, NaN behind the mask: in stretches as in one piece."""
+    lens = [700, 300]
+    c = make(lens, 1, 64)
+    fill(c, lens)
+    dead = randn(64, 1, 64, seed=1)
+    dead[:] = math.nan
+    c.append(0, dead, dead, runs_of([(0, 20, 0, 680), (0, 1, 1, 299)]), 20)   # rows 680.. and 299 are NaN
+    q = randn(30, 2, 64, seed=3).to(dtype)
+    for runs in ([(0, 10, 0, 670), (10, 1, 1, 298), (11, 0, 1, 0)], [(0, 12, 1, -5), (12, 4, 0, 0)],
+                 [(0, 0, 0, 0), (3, 0, 1, 5)]):
+        got = torch.full_like(q, 3)
+        c.attention(0, got, q, runs_of(runs), 1, LONG)
+        check_attention(c, 0, q, got, runs, 2, untouched=3)
+    assert _lib.load().cats_gpu_device_error() == 0
+    c.table[0, 3] = -1
+    piece, stretch = torch.full_like(q, 3), torch.full_like(q, 3)
+    c.attention(0, piece, q, runs_of([(0, 4, 0, 600)]), 4, 700)
+    c.attention(0, stretch, q, runs_of([(0, 4, 0, 600)]), 4, LONG)
+    assert torch.isfinite(stretch).all() and (piece.float() - stretch.float()).abs().max() < 2**-8
+    torch.cuda.synchronize()
+    assert _lib.load().cats_gpu_device_error() == 0x40
+
+
+@pytest.mark.parametrize("rows,hint", [(1, LONG), (64, 2000), (1, 2000)])
+def test_captured_replayed_and_on_two_streams(rows, hint):
+    """One captured call replayed after its inputs moved on; two streams at once: each the answer of a call alone."""
+    lens = [2000, 900]
+    c = make(lens, 2, 128)
+    fill(c, lens)
+    runs = runs_of([(0, rows, 0, 2000 - rows), (rows, rows, 1, 900 - rows)])
+    qs = [randn(2 * rows, 8, 128, seed=20 + i).half() for i in range(6)]
+    alone = []
+    for q in qs:
+        alone.append(torch.empty_like(q))
+        c.attention(0, alone[-1], q, runs, rows, hint)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    got = [torch.empty_like(q) for q in qs]
+    for i, q in enumerate(qs):
+        c.attention(0, got[i], q, runs, rows, hint, stream=side[i % 2].cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(alone, got))
+    graphs, ins, outs = [], [], []
+    for s in side:
+        ins.append(qs[0].clone())
+        outs.append(torch.empty_like(qs[0]))
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=s, capture_error_mode="thread_local"):
+            c.attention(0, outs[-1], ins[-1], runs, rows, hint, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for i in range(0, 6, 2):                          # both graphs in flight together
+        for j in range(2):
+            ins[j].copy_(qs[i + j])
+        torch.cuda.synchronize()
+        for j in range(2):
+            with torch.cuda.stream(side[j]):
+                graphs[j].replay()
+                graphs[j].replay()
+        torch.cuda.synchronize()
+        for j in range(2):
+            assert torch.equal(outs[j], alone[i + j])
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [1, 40])
 def test_rows_before_position_zero_see_nothing(dtype, rows):
