@@ -74,6 +74,15 @@ SIGNATURES = {
     "cats_gpu_llm_batch_enqueue": (_i, [_vp]),
     "cats_gpu_llm_batch_enqueue_decode": (_i, [_vp, _i]),
     "cats_gpu_llm_time_product": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
+    "cats_gpu_llm_score_batch": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp]),
+    "cats_gpu_llm_cache_q4": (_i, [_vp, _i, _i]),
+    "cats_gpu_llm_cache_fork": (_i, [_vp, _i, _i, _i]),
+    "cats_gpu_llm_cache_truncate": (_i, [_vp, _i, _i]),
+    "cats_gpu_llm_cache_compact": (_i, [_vp, _ip]),
+    "cats_gpu_llm_cache_read": (_i, [_vp, _i, _i, _i, _vp, _vp]),
+    "cats_gpu_llm_cache_to_dense": (_i, [_vp, _i, _i]),
+    "cats_gpu_llm_cache_length": (_i, [_vp, _i]),
+    "cats_gpu_llm_cache_free_pages": (_i, [_vp]),
     "cats_gpu_llm_set_engine": (_i, [_vp, _i]),
     "cats_gpu_tp_unique_id_bytes": (_sz, []),
     "cats_gpu_tp_unique_id": (_i, [_vp, _sz]),

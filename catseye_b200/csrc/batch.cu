@@ -26,9 +26,12 @@
 // token (:1765-1770, sample_argmax :1944-1956).  With tensor parallelism the
 // wo and w2 products go to a delta buffer that is sum-allreduced and added,
 // and the classifier slices are allgathered, as in the decode graph.
+#include "kv_attn.cuh"
+#include "kv_model.cuh"
 #include "llm.cuh"
 #include "mv_device.cuh"
 #include "qgemm.cuh"
+#include "score.cuh"
 #include <algorithm>
 #include <cstring>
 #include <vector>
@@ -42,6 +45,13 @@ constexpr int AT_NQ = 64;          // query rows per CTA: tokens x the query hea
 constexpr int AT_MAXHS = 128;
 
 // ------------------------------------------------------------- small kernels
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 // A product's element i: y[i], or, for a K split the product left to its
 // reader (SplitOut), the sum of the partials in split order, the arithmetic
 // of the split-sum kernel.
@@ -173,6 +183,55 @@ __global__ void k_rope_kv(PartSrc y, int T, const BatchTok *__restrict__ bt, flo
     }
 }
 
+// The same for the paged Q4_0 cache: q as fp16 (the attention's operand), k
+// and v quantized into their pages.  Eight elements (four pairs) a thread, so
+// four neighbours hold a block of 32.
+__global__ void __launch_bounds__(256) k_rope_kv_paged(PartSrc y, int T, const BatchTok *__restrict__ bt,
+                                                       __half *__restrict__ q, const __grid_constant__ KvView c,
+                                                       int q_dim, int kv_dim, int seq_len)
+{
+    const int qkv = q_dim + 2 * kv_dim, cols = qkv / 8;
+    const unsigned mask = 0xfu << (threadIdx.x & 28);
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < (long long)T * cols; i += gridDim.x * 256LL) {
+        const int t = (int)(i / cols), r0 = 8 * (int)(i % cols);
+        const BatchTok b = bt[t];
+        const float4 lo = y.ld4((size_t)t * qkv + r0), hi = y.ld4((size_t)t * qkv + r0 + 4);
+        float x[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const bool is_q = r0 < q_dim, is_v = r0 >= q_dim + kv_dim;
+        const int idx = is_q ? r0 : is_v ? r0 - q_dim - kv_dim : r0 - q_dim;
+        if (!is_v) {
+#pragma unroll
+            for (int p = 0; p < 8; p += 2) rope_pair(x[p], x[p + 1], idx + p, c.hs, b.pos);
+        }
+        if (is_q) {
+            *reinterpret_cast<uint4 *>(q + (size_t)t * q_dim + r0) =
+                make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(x[4], x[5]), pack_f16x2(x[6], x[7]));
+            continue;
+        }
+        const bool here = b.pos >= 0 && b.pos < seq_len;
+        if (!here && idx == 0 && c.err) atomicOr(c.err, CATS_DEVERR_POS_RANGE);   // no cache write
+        const int page = here ? c.page(b.seq, b.pos / KV_PAGE) : -1;
+        uint16_t scale;
+        const uint32_t codes = kv_quant8(x, mask, &scale);
+        if (page >= 0)
+            kv_store_codes8(c.chunk(page, idx / c.hs), is_v, c.hs, b.pos % KV_PAGE, idx % c.hs / 8, codes, scale);
+    }
+}
+
+// fp16 rows [T][n] -> x16
+__global__ void k_x16_half(const __half *__restrict__ x, __half *__restrict__ x16, int T, int Tpad, int n)
+{
+    const long long total = (long long)(n / 64) * T * 8;
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const int c = (int)(i & 7), t = (int)((i >> 3) % T), kb = (int)((i >> 3) / T);
+        const __half *src = x + (size_t)t * n + kb * 64 + x16_src_off(c);
+        const uint2 a = *reinterpret_cast<const uint2 *>(src), b = *reinterpret_cast<const uint2 *>(src + 16);
+        *reinterpret_cast<uint4 *>(x16 + x16_chunk(kb, c, t, Tpad)) =
+            make_uint4(__byte_perm(a.x, a.y, 0x5410), __byte_perm(a.x, a.y, 0x7632), __byte_perm(b.x, b.y, 0x5410),
+                       __byte_perm(b.x, b.y, 0x7632));
+    }
+}
+
 // SwiGLU of the interleaved [w1;w3] product (row 2i = w1_i x, 2i+1 = w3_i x):
 // h_i = silu(w1_i x) * (w3_i x) (:1744-1752), written as fp16 into x16.
 __global__ void k_swiglu_x16(PartSrc y, int T, int hidden, __half *__restrict__ x16, int Tpad)
@@ -242,13 +301,15 @@ __global__ void __launch_bounds__(256) k_logits_argmax(PartSrc lg, int T, int vo
 
 // The generate loop's advance: every token's argmax becomes its next input
 // at the next position; the ids are logged per step.
-__global__ void k_batch_advance(BatchTok *bt, const int *next, int T, int *log, int log_cap, int *step)
+// (runs: the paged cache's batch, a run a token; null without one)
+__global__ void k_batch_advance(BatchTok *bt, const int *next, int T, int *log, int log_cap, int *step, KvRun *runs)
 {
     const int s = *step;
     for (int t = threadIdx.x; t < T; t += blockDim.x) {
         const int nx = next[t];
         bt[t].token = nx;
         bt[t].pos += 1;
+        if (runs) runs[t].pos += 1;
         if (log && s < log_cap) log[(size_t)s * T + t] = nx;
     }
     __syncthreads();
@@ -480,13 +541,6 @@ constexpr int MA_SV = MA_HS + 4;   // V row stride (floats): 32-bit fragment loa
 
 __host__ __device__ constexpr size_t ma_smem_bytes() { return (size_t)2 * MA_KC * (MA_SK + MA_SV) * 4; }
 
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1)
 {
@@ -703,7 +757,7 @@ static void free_batch(LlmModel *m)
     m->bt_graph = nullptr;
     m->bt_graph_T = 0;
     void *dp[] = {m->bt_tok, m->bt_blocks, m->bt_x, m->bt_delta, m->bt_y, m->bt_q, m->bt_xb, m->bt_lg, m->bt_logits,
-                  m->bt_x16, m->bt_ws, m->bt_next, m->bt_step, m->bt_log};
+                  m->bt_x16, m->bt_ws, m->bt_next, m->bt_step, m->bt_log, m->bt_score};
     for (void *p : dp) if (p) cudaFree(p);
     if (m->bt_tok_host) cudaFreeHost(m->bt_tok_host);
     if (m->bt_blocks_host) cudaFreeHost(m->bt_blocks_host);
@@ -711,6 +765,7 @@ static void free_batch(LlmModel *m)
     m->bt_q = nullptr; m->bt_xb = nullptr; m->bt_lg = nullptr; m->bt_logits = nullptr; m->bt_x16 = nullptr;
     m->bt_ws = nullptr; m->bt_ws_bytes = 0;
     m->bt_next = nullptr; m->bt_step = nullptr; m->bt_log = nullptr; m->bt_log_cap = 0;
+    m->bt_score = nullptr; m->bt_score_bytes = 0;
     m->bt_tok_host = nullptr; m->bt_blocks_host = nullptr;
     m->bt_cap = 0;
 }
@@ -925,6 +980,24 @@ static cudaError_t residual_product(LlmModel *m, const DevWeight &W, int T, cuda
     return cudaGetLastError();
 }
 
+// The step's middle on the paged cache: RoPE, k and v into their pages, the
+// attention over them, its output as the next product's operand.  A captured
+// greedy step (advance) is planned for the longest context it may reach.
+static cudaError_t paged_attention(LlmModel *m, int l, const PartSrc &y, int T, int Tpad, bool advance, cudaStream_t st)
+{
+    const LlmPaged *p = m->paged;
+    const KvView view = llm_paged_view(m, l);
+    const long long eights = (long long)T * (m->q_dim + 2 * m->kv_dim) / 8;
+    k_rope_kv_paged<<<grid_for(eights, 256), 256, 0, st>>>(y, T, m->bt_tok, p->q16, view, m->q_dim, m->kv_dim, m->c.seq_len);
+    cudaError_t e = cudaGetLastError();
+    if (e) return e;
+    const KvBatch b{p->runs, p->n_runs, p->max_rows, advance ? m->c.seq_len : p->max_len};
+    if ((e = launch_kv_attention(view, KV_F16, KvRows{p->o16, m->q_dim, T, 1}, KvRows{p->q16, m->q_dim, T, 1}, m->heads_loc, b, st)))
+        return e;
+    k_x16_half<<<grid_for((long long)T * m->q_dim / 8, 256), 256, 0, st>>>(p->o16, m->bt_x16, T, Tpad, m->q_dim);
+    return cudaGetLastError();
+}
+
 cudaError_t llm_batch_enqueue(LlmModel *m, int T, int nblocks, bool advance, int *log, int log_cap)
 {
     const LlmConfig &c = m->c;
@@ -944,13 +1017,17 @@ cudaError_t llm_batch_enqueue(LlmModel *m, int T, int nblocks, bool advance, int
         if ((e = cudaGetLastError())) return e;
         if ((e = launch_qgemm_x16(m->qkv[l].L, m->qkv[l].ptr, m->bt_x16, m->bt_y, T, false, m->bt_ws,
                                     m->bt_ws_bytes, m->err, st, &so))) return e;
-        const long long np = nqkv / 2;
-        k_rope_kv<<<grid_for(np, 256), 256, 0, st>>>(part_src(m->bt_y, so, nqkv), T, m->bt_tok, m->bt_q, m->kcache,
-                                                     m->vcache, seq_stride, (size_t)l * c.seq_len * m->kv_dim,
-                                                     m->q_dim, m->kv_dim, m->head_size, c.seq_len, m->n_seqs, m->err);
-        if ((e = cudaGetLastError())) return e;
-        if ((e = launch_attn_batch(m, l, nblocks, m->bt_max_rows, st))) return e;
-        if ((e = launch_x16(m->bt_xb, m->bt_x16, T, m->q_dim, st))) return e;
+        if (m->paged) {
+            if ((e = paged_attention(m, l, part_src(m->bt_y, so, nqkv), T, Tpad, advance, st))) return e;
+        } else {
+            const long long np = nqkv / 2;
+            k_rope_kv<<<grid_for(np, 256), 256, 0, st>>>(part_src(m->bt_y, so, nqkv), T, m->bt_tok, m->bt_q, m->kcache,
+                                                         m->vcache, seq_stride, (size_t)l * c.seq_len * m->kv_dim,
+                                                         m->q_dim, m->kv_dim, m->head_size, c.seq_len, m->n_seqs, m->err);
+            if ((e = cudaGetLastError())) return e;
+            if ((e = launch_attn_batch(m, l, nblocks, m->bt_max_rows, st))) return e;
+            if ((e = launch_x16(m->bt_xb, m->bt_x16, T, m->q_dim, st))) return e;
+        }
         if ((e = residual_product(m, m->wo[l], T, st, &pend))) return e;
         k_rmsnorm_x16<<<T, 256, 0, st>>>(m->bt_x, m->rms_ffn + (size_t)l * c.dim, m->bt_x16, c.dim, Tpad,
                                          part_src(m->bt_x, pend, nd));
@@ -977,26 +1054,31 @@ cudaError_t llm_batch_enqueue(LlmModel *m, int T, int nblocks, bool advance, int
                                        c.tp_size, m->bt_logits, m->bt_next, m->err);
     if ((e = cudaGetLastError())) return e;
     if (advance) {
-        k_batch_advance<<<1, 256, 0, st>>>(m->bt_tok, m->bt_next, T, log, log_cap, m->bt_step);
+        k_batch_advance<<<1, 256, 0, st>>>(m->bt_tok, m->bt_next, T, log, log_cap, m->bt_step,
+                                               m->paged ? m->paged->runs : nullptr);
         if ((e = cudaGetLastError())) return e;
     }
     return cudaSuccess;
 }
 
+int llm_batch_seqs(const LlmModel *m) { return m->paged ? m->paged->pages.n_seqs() : m->n_seqs; }
+
 // Validate and upload a batch (tokens, positions, sequences); returns the
 // number of attention blocks through *nblocks.
-int llm_batch_set(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, int *nblocks)
+int llm_batch_set(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, int *nblocks, int ahead)
 {
     const LlmConfig &c = m->c;
     if (T <= 0 || T > m->bt_cap || !tokens || !pos) return E_ARG;
     for (int t = 0; t < T; t++) {
         const int s = seqs ? seqs[t] : 0;
-        if (tokens[t] < 0 || tokens[t] >= c.vocab || pos[t] < 0 || pos[t] >= c.seq_len || s < 0 || s >= m->n_seqs)
+        if (tokens[t] < 0 || tokens[t] >= c.vocab || pos[t] < 0 || pos[t] >= c.seq_len || s < 0 || s >= llm_batch_seqs(m))
             return E_ARG;
     }
     // the pinned staging may still be the source of an earlier copy
     if (cudaStreamSynchronize(m->stream) != cudaSuccess) return E_CUDA;
     for (int t = 0; t < T; t++) m->bt_tok_host[t] = BatchTok{tokens[t], pos[t], seqs ? seqs[t] : 0, 0};
+    if (m->paged)
+        if (int rc = llm_paged_set(m, T, ahead)) return rc;
     const int nb = make_blocks(m, m->bt_tok_host, T, m->bt_blocks_host);
     int most = 0;
     for (int b = 0; b < nb; b++) most = std::max(most, m->bt_blocks_host[b].y);
@@ -1031,6 +1113,10 @@ cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps)
     // one token; one step is captured once into a graph and replayed
     if (steps <= 0) return cudaSuccess;
     cudaError_t e;
+    if (m->paged) {
+        const int rc = llm_paged_extend(m, T, steps, false);
+        if (rc) return rc == E_NOMEM ? cudaErrorMemoryAllocation : rc == E_ARG ? cudaErrorInvalidValue : cudaErrorUnknown;
+    }
     if (m->bt_log_cap < steps * T) {
         if (m->bt_log) cudaFree(m->bt_log);
         m->bt_log = nullptr;
@@ -1057,11 +1143,42 @@ cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps)
     return cudaSuccess;
 }
 
+int llm_score_batch(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, const int *targets, int k,
+                    float *logprob, float *entropy, int *top_ids, float *top_logprob)
+{
+    int nb = 0;
+    int rc = llm_batch_set(m, tokens, pos, seqs, T, &nb);   // (waits for the stream: the buffer below is free)
+    if (rc) return rc;
+    const size_t n = T, bytes = n * 4 * (3 + 2 * (size_t)k);
+    if (m->bt_score_bytes < bytes) {
+        if (m->bt_score) cudaFree(m->bt_score);
+        m->bt_score = nullptr;
+        m->bt_score_bytes = 0;
+        if (cudaMalloc(&m->bt_score, bytes) != cudaSuccess) {
+            cudaGetLastError();
+            return E_NOMEM;
+        }
+        m->bt_score_bytes = bytes;
+    }
+    int *d_targets = reinterpret_cast<int *>(m->bt_score), *d_ids = d_targets + n;
+    float *d_lp = reinterpret_cast<float *>(d_ids + n * k), *d_h = d_lp + n, *d_top = d_h + n;
+    const ScoreArgs a{m->bt_logits, d_targets, targets ? d_lp : nullptr, entropy ? d_h : nullptr, d_ids, d_top,
+                      m->c.vocab, T, m->c.vocab, k, m->err};
+    if ((targets && cudaMemcpyAsync(d_targets, targets, n * 4, cudaMemcpyHostToDevice, m->stream)) ||
+        llm_batch_enqueue(m, T, nb, false, nullptr, 0) || launch_logprobs(a, KV_F32, m->stream) ||
+        (targets && cudaMemcpyAsync(logprob, d_lp, n * 4, cudaMemcpyDeviceToHost, m->stream)) ||
+        (entropy && cudaMemcpyAsync(entropy, d_h, n * 4, cudaMemcpyDeviceToHost, m->stream)) ||
+        (k && (cudaMemcpyAsync(top_ids, d_ids, n * k * 4, cudaMemcpyDeviceToHost, m->stream) ||
+               cudaMemcpyAsync(top_logprob, d_top, n * k * 4, cudaMemcpyDeviceToHost, m->stream))))
+        return E_CUDA;
+    return cudaStreamSynchronize(m->stream) == cudaSuccess ? E_OK : E_CUDA;
+}
+
 int llm_generate_batch(LlmModel *m, int T, int steps, int *tokens_host)
 {
     if (steps <= 0) return E_OK;
     cudaError_t e = llm_batch_decode_enqueue(m, T, steps);
-    if (e) return e == cudaErrorMemoryAllocation ? E_NOMEM : E_CUDA;
+    if (e) return e == cudaErrorMemoryAllocation ? E_NOMEM : e == cudaErrorInvalidValue ? E_ARG : E_CUDA;
     if (tokens_host &&
         cudaMemcpyAsync(tokens_host, m->bt_log, (size_t)steps * T * 4, cudaMemcpyDeviceToHost, m->stream))
         return E_CUDA;

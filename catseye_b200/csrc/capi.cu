@@ -8,12 +8,16 @@
 #include "loader.cuh"
 #include "conv.cuh"
 #include "kquant.cuh"
+#include "kv_model.cuh"
 #include "llm.cuh"
+#include "score.cuh"
 #include "qgemm.cuh"
 #include "sgemm.cuh"
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <functional>
+#include <new>
 #include <vector>
 #include <mutex>
 #include <unordered_map>
@@ -793,6 +797,7 @@ static int batch_ready(cats_gpu_llm *h, const char *what)
     if (!batch_supported(&h->m)) return fail(CATS_ERR_UNSUPPORTED, what);
     if (h->m.bt_cap == 0) return fail(CATS_ERR_ARG, what);   // cats_gpu_llm_batch_reserve first
     if (h->m.c.tp_size > 1 && !h->m.comm_ctx) return fail(CATS_ERR_ARG, what);
+    if (h->m.paged) h->bt_T = 0;   // another call's pages: the batch set before is not enqueued again
     return CATS_OK;
 }
 
@@ -831,6 +836,8 @@ int cats_gpu_llm_batch_enqueue(cats_gpu_llm *h)
 {
     const char *what = "cats_gpu_llm_batch_enqueue";
     if (!h || h->bt_T <= 0) return fail(CATS_ERR_ARG, what);
+    if (h->m.paged && h->m.paged->advanced > 0)
+        if (int rc = llm_paged_extend(&h->m, h->bt_T, 1, true)) return fail(rc, what);
     return check(llm_batch_enqueue(&h->m, h->bt_T, h->bt_nb, false, nullptr, 0), what);
 }
 
@@ -838,7 +845,11 @@ int cats_gpu_llm_batch_enqueue_decode(cats_gpu_llm *h, int steps)
 {
     const char *what = "cats_gpu_llm_batch_enqueue_decode";
     if (!h || h->bt_T <= 0 || steps < 0 || h->bt_nb != h->bt_T) return fail(CATS_ERR_ARG, what);
-    return check(llm_batch_decode_enqueue(&h->m, h->bt_T, steps), what);
+    const cudaError_t e = llm_batch_decode_enqueue(&h->m, h->bt_T, steps);
+    // (the paged cache: no room, or past the context)
+    if (h->m.paged && (e == cudaErrorMemoryAllocation || e == cudaErrorInvalidValue))
+        return fail(e == cudaErrorMemoryAllocation ? CATS_ERR_NOMEM : CATS_ERR_ARG, what);
+    return check(e, what);
 }
 
 int cats_gpu_llm_time_product(cats_gpu_llm *h, int kind, int T, int reps, float *ms_per_launch,
@@ -866,18 +877,84 @@ int cats_gpu_llm_generate_batch(cats_gpu_llm *h, const int *tokens, const int *p
                                 int *tokens_host)
 {
     const char *what = "cats_gpu_llm_generate_batch";
-    if (!h || !tokens || !pos || n <= 0 || steps < 0 || n > h->m.n_seqs) return fail(CATS_ERR_ARG, what);
+    if (!h || !tokens || !pos || n <= 0 || steps < 0 || n > llm_batch_seqs(&h->m)) return fail(CATS_ERR_ARG, what);
     if (int rc = batch_ready(h, what)) return rc;
     for (int i = 0; i < n; i++)
         if (pos[i] < 0 || pos[i] + steps > h->m.c.seq_len) return fail(CATS_ERR_ARG, what);
     std::vector<int> seqs(n);
     for (int i = 0; i < n; i++) seqs[i] = i;
     int nb = 0;
-    if (int rc = llm_batch_set(&h->m, tokens, pos, seqs.data(), n, &nb)) return fail(rc, what);
+    if (int rc = llm_batch_set(&h->m, tokens, pos, seqs.data(), n, &nb, steps)) return fail(rc, what);
     h->bt_T = 0;
     if (int rc = llm_generate_batch(&h->m, n, steps, tokens_host)) return fail(rc, what);
     return device_status(h, what);
 }
+
+int cats_gpu_llm_score_batch(cats_gpu_llm *h, const int *tokens, const int *pos, const int *seqs, int T,
+                             const int *targets, int k, float *logprob, float *entropy, int *top_ids, float *top_logprob)
+{
+    const char *what = "cats_gpu_llm_score_batch";
+    if (!h || k < 0 || (targets && !logprob) || (k > 0 && (!top_ids || !top_logprob))) return fail(CATS_ERR_ARG, what);
+    if (k > SCORE_MAX_K) return fail(CATS_ERR_UNSUPPORTED, what);
+    if (int rc = batch_ready(h, what)) return rc;
+    for (int t = 0; targets && t < T; t++)
+        if (targets[t] >= h->m.c.vocab) return fail(CATS_ERR_ARG, what);
+    if (int rc = llm_score_batch(&h->m, tokens, pos, seqs, T, targets, k, logprob, entropy, top_ids, top_logprob))
+        return fail(rc, what);
+    h->bt_T = 0;
+    return device_status(h, what);
+}
+
+int cats_gpu_llm_cache_q4(cats_gpu_llm *h, int n_pages, int n_seqs)
+{
+    const char *what = "cats_gpu_llm_cache_q4";
+    if (!h || n_pages < 0 || (n_pages > 0 && n_seqs <= 0)) return fail(CATS_ERR_ARG, what);
+    if (!h->m.weights_ready) return fail(CATS_ERR_ARG, what);
+    int rc = llm_cache_q4(&h->m, n_pages, n_seqs);
+    h->bt_T = 0;
+    return rc ? fail(rc, what) : CATS_OK;
+}
+
+// The paged cache's entry points: a model that has one, and no exception out.
+static int paged_call(cats_gpu_llm *h, const char *what, const std::function<int(LlmModel *)> &f)
+{
+    if (!h || !h->m.paged) return fail(CATS_ERR_ARG, what);
+    h->bt_T = 0;   // a batch's positions may not be its own any more
+    try {
+        const int rc = f(&h->m);
+        return rc ? fail(rc, what) : CATS_OK;
+    } catch (const std::bad_alloc &) {
+        return fail(CATS_ERR_NOMEM, what);
+    }
+}
+
+int cats_gpu_llm_cache_fork(cats_gpu_llm *h, int src, int dst, int len)
+{
+    return paged_call(h, "cats_gpu_llm_cache_fork", [&](LlmModel *m) { return llm_cache_fork(m, src, dst, len); });
+}
+int cats_gpu_llm_cache_truncate(cats_gpu_llm *h, int seq, int len)
+{
+    return paged_call(h, "cats_gpu_llm_cache_truncate", [&](LlmModel *m) { return llm_cache_truncate(m, seq, len); });
+}
+int cats_gpu_llm_cache_compact(cats_gpu_llm *h, int *moved)
+{
+    return paged_call(h, "cats_gpu_llm_cache_compact", [&](LlmModel *m) { return llm_cache_compact(m, moved); });
+}
+int cats_gpu_llm_cache_read(cats_gpu_llm *h, int layer, int seq, int n, float *k, float *v)
+{
+    const char *what = "cats_gpu_llm_cache_read";
+    if (!k || !v) return fail(CATS_ERR_ARG, what);
+    return paged_call(h, what, [&](LlmModel *m) { return llm_cache_read(m, layer, seq, n, k, v); });
+}
+int cats_gpu_llm_cache_to_dense(cats_gpu_llm *h, int seq, int n)
+{
+    return paged_call(h, "cats_gpu_llm_cache_to_dense", [&](LlmModel *m) { return llm_cache_to_dense(m, seq, n); });
+}
+int cats_gpu_llm_cache_length(cats_gpu_llm *h, int seq)
+{
+    return h && h->m.paged && h->m.paged->pages.seq_ok(seq) ? h->m.paged->pages.length(seq) : -1;
+}
+int cats_gpu_llm_cache_free_pages(cats_gpu_llm *h) { return h && h->m.paged ? h->m.paged->pages.free_count() : -1; }
 
 int cats_gpu_llm_synchronize(cats_gpu_llm *h)
 {

@@ -11,6 +11,7 @@
 //   w2    : quantize -> matvec -> residual add into x                   (:1754-1761)
 // then the classifier (final rmsnorm + matvec + greedy argmax, :1765-1770)
 // and a one-thread kernel that feeds the argmax back as the next token.
+#include "kv_model.cuh"
 #include "llm.cuh"
 #include "mv_device.cuh"
 #include <algorithm>
@@ -326,6 +327,7 @@ void llm_free(LlmModel *m)
     m->exec = nullptr;
     m->graph = nullptr;
     llm_batch_free(m);
+    llm_paged_free(m);
     tp_release(m);   // after the graphs that hold its NCCL calls
     for (auto &w : m->qkv) free_w(w);
     for (auto &w : m->wo) free_w(w);

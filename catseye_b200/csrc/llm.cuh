@@ -35,6 +35,8 @@ typedef void (*AllreduceFn)(void *ctx, float *buf, size_t count, cudaStream_t st
 typedef void (*ArgmaxReduceFn)(void *ctx, unsigned long long *key, cudaStream_t st);
 typedef void (*AllgatherFn)(void *ctx, float *buf, size_t count_per_rank, int rank, cudaStream_t st);
 
+struct LlmPaged;   // the batched step's paged Q4_0 cache (kv_model.cuh)
+
 struct LlmModel {
     LlmConfig c{};
     int q_dim = 0, kv_dim = 0, head_size = 0, hidden_loc = 0, vocab_loc = 0, vocab_off = 0;
@@ -87,6 +89,9 @@ struct LlmModel {
     cudaGraph_t bt_graph = nullptr;
     cudaGraphExec_t bt_exec = nullptr;
     int bt_graph_T = 0;
+    LlmPaged *paged = nullptr;            // set: the batched step keeps its K/V there, not in kcache / vcache
+    uint8_t *bt_score = nullptr;          // log probabilities of a scored batch
+    size_t bt_score_bytes = 0;
     // tensor parallel hooks (NCCL, tp.cu), null when tp_size == 1
     AllreduceFn allreduce = nullptr;
     ArgmaxReduceFn argmax_reduce = nullptr;
@@ -168,10 +173,15 @@ cudaError_t llm_time_matvec(LlmModel *m, int kind, int reps, float *ms_per_launc
 bool batch_supported(const LlmModel *m);
 int llm_batch_reserve(LlmModel *m, int cap, int n_seqs);
 void llm_batch_free(LlmModel *m);
-int llm_batch_set(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, int *nblocks);
+int llm_batch_seqs(const LlmModel *m);   // sequences a batch may name
+int llm_batch_set(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, int *nblocks, int ahead = 1);
 cudaError_t llm_batch_enqueue(LlmModel *m, int T, int nblocks, bool advance, int *log, int log_cap);
 int llm_forward_batch(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, int *next_host,
                       float *logits_host);
+// llm_forward_batch, then each token's log probability of targets[t], the
+// entropy and the k likeliest ids with their log probabilities (host arrays).
+int llm_score_batch(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, const int *targets, int k,
+                    float *logprob, float *entropy, int *top_ids, float *top_logprob);
 int llm_generate_batch(LlmModel *m, int T, int steps, int *tokens_host);
 cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps);
 // Device time of one kind of batched product (0 qkv, 1 wo, 2 w13, 3 w2,

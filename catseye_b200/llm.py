@@ -160,6 +160,63 @@ class GpuLLM:
                                                         C.c_void_p(out.ctypes.data)), "generate_batch")
         return out[:steps]
 
+    def score_batch(self, tokens, pos, targets=None, k=0, seqs=None):
+        """One batched step's scores: (log probability of targets[t] after
+        token t or None, entropy, ids of the k likeliest next tokens [T, k],
+        their log probabilities [T, k])."""
+        tokens, pos = np.ascontiguousarray(tokens, np.int32), np.ascontiguousarray(pos, np.int32)
+        T = tokens.size
+        if pos.size != T or (seqs is not None and np.size(seqs) != T) or (targets is not None and np.size(targets) != T):
+            raise ValueError("tokens, pos, seqs and targets must have the same length")
+        arr = [None if a is None else np.ascontiguousarray(a, np.int32) for a in (seqs, targets)]
+        ptr = [None if a is None else C.c_void_p(a.ctypes.data) for a in arr]
+        lp = None if targets is None else np.zeros(T, np.float32)
+        h = np.zeros(T, np.float32)
+        ids, top = np.zeros((T, max(k, 0)), np.int32), np.zeros((T, max(k, 0)), np.float32)
+        _lib.check(self.lib.cats_gpu_llm_score_batch(
+            self.h, C.c_void_p(tokens.ctypes.data), C.c_void_p(pos.ctypes.data), ptr[0], T, ptr[1], k,
+            None if lp is None else C.c_void_p(lp.ctypes.data), C.c_void_p(h.ctypes.data), C.c_void_p(ids.ctypes.data),
+            C.c_void_p(top.ctypes.data)), "score_batch")
+        return lp, h, ids, top
+
+    # ---- paged Q4_0 cache of the batched step
+    def cache_q4(self, n_pages, n_seqs=1):
+        """Keep the batched step's K/V in n_pages pages of 64 tokens in Q4_0
+        blocks, shared by n_seqs sequences; 0 pages: back to the dense cache."""
+        _lib.check(self.lib.cats_gpu_llm_cache_q4(self.h, n_pages, n_seqs), "cache_q4")
+
+    def cache_fork(self, src, dst, length):
+        """dst becomes the first `length` tokens of src (pages shared until written)."""
+        _lib.check(self.lib.cats_gpu_llm_cache_fork(self.h, src, dst, length), "cache_fork")
+
+    def cache_truncate(self, seq, length=0):
+        """Keep a sequence's first `length` tokens."""
+        _lib.check(self.lib.cats_gpu_llm_cache_truncate(self.h, seq, length), "cache_truncate")
+
+    def cache_compact(self):
+        """Move the used pages to the front of the pool; returns how many moved."""
+        moved = C.c_int()
+        _lib.check(self.lib.cats_gpu_llm_cache_compact(self.h, C.byref(moved)), "cache_compact")
+        return moved.value
+
+    def cache_read(self, layer, seq, n, kv_dim=None):
+        """K and V [n, kv_dim] that the cache holds for a sequence's first n tokens."""
+        k, v = (np.zeros((n, kv_dim or self.cfg.kv_dim), np.float32) for _ in range(2))
+        _lib.check(self.lib.cats_gpu_llm_cache_read(self.h, layer, seq, n, C.c_void_p(k.ctypes.data),
+                                                    C.c_void_p(v.ctypes.data)), "cache_read")
+        return k, v
+
+    def cache_to_dense(self, seq, n):
+        """Copy a sequence's first n tokens into the single-token engines' cache."""
+        _lib.check(self.lib.cats_gpu_llm_cache_to_dense(self.h, seq, n), "cache_to_dense")
+
+    def cache_length(self, seq):
+        return self.lib.cats_gpu_llm_cache_length(self.h, seq)
+
+    @property
+    def cache_free_pages(self):
+        return self.lib.cats_gpu_llm_cache_free_pages(self.h)
+
     def batch_set(self, tokens, pos, seqs=None):
         """Upload a batch for batch_enqueue (timing)."""
         tokens = np.ascontiguousarray(tokens, np.int32)

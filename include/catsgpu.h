@@ -284,6 +284,40 @@ int cats_gpu_llm_batch_enqueue(cats_gpu_llm *m);
 int cats_gpu_llm_batch_enqueue_decode(cats_gpu_llm *m, int steps);
 int cats_gpu_llm_time_product(cats_gpu_llm *m, int kind, int T, int reps, float *ms_per_launch,
                               double *flop_per_launch, double *weight_bytes_per_launch);
+/* Scoring: cats_gpu_llm_forward_batch, then for every token the log
+ * probability of targets[t] (the next token, say; negative: none, 0), the
+ * entropy of its distribution in nats, and the k <= 32 likeliest next tokens
+ * with their log probabilities, [T][k] (cats_gpu_logprobs_dev on the step's
+ * logits, which stay on the device).  targets with logprob, entropy, and the
+ * top_ arrays with k = 0 may be NULL.  Host pointers. */
+int cats_gpu_llm_score_batch(cats_gpu_llm *m, const int *tokens, const int *pos, const int *seqs, int T,
+                             const int *targets, int k, float *logprob, float *entropy, int *top_ids,
+                             float *top_logprob);
+/* The batched step on a paged KV cache in Q4_0 blocks (4.5 bits a value, a
+ * seventh of the fp32 cache; cats_gpu_kv_* below has the format): n_pages
+ * pages of CATS_KV_PAGE tokens, taken as sequences grow, shared by n_seqs
+ * sequences (0 .. n_seqs - 1, empty at first).  cats_gpu_llm_forward_batch,
+ * _score_batch, _generate_batch and _batch_set then read and write it; n_pages
+ * 0 goes back to the dense cache.  head_size must be a multiple of 32 up to
+ * 128 (else CATS_ERR_UNSUPPORTED).  A step's positions may rewrite a sequence
+ * or extend it, without a gap and each once (else CATS_ERR_ARG); too few free
+ * pages: CATS_ERR_NOMEM, the cache as it was.  Queries and attention output
+ * are fp16.  The single-token engines keep their own dense cache:
+ * _cache_to_dense copies a sequence's first n tokens into it.
+ * _cache_fork: dst becomes the first len tokens of src, sharing its pages;
+ * pages are copied when one of their sequences writes.  _cache_truncate: keep
+ * len tokens (0 frees the sequence).  _cache_compact: used pages move to the
+ * front of the pool (*moved of them; may be NULL).  _cache_read: K and V [n]
+ * [local kv heads * head_size] of a sequence's first n tokens.  _cache_length
+ * and _cache_free_pages: -1 without a paged cache. */
+int cats_gpu_llm_cache_q4(cats_gpu_llm *m, int n_pages, int n_seqs);
+int cats_gpu_llm_cache_fork(cats_gpu_llm *m, int src, int dst, int len);
+int cats_gpu_llm_cache_truncate(cats_gpu_llm *m, int seq, int len);
+int cats_gpu_llm_cache_compact(cats_gpu_llm *m, int *moved);
+int cats_gpu_llm_cache_read(cats_gpu_llm *m, int layer, int seq, int n, float *k, float *v);
+int cats_gpu_llm_cache_to_dense(cats_gpu_llm *m, int seq, int n);
+int cats_gpu_llm_cache_length(cats_gpu_llm *m, int seq);
+int cats_gpu_llm_cache_free_pages(cats_gpu_llm *m);
 /* Asynchronous form for timing: enqueue `steps` greedy steps on the model's stream. */
 int cats_gpu_llm_enqueue(cats_gpu_llm *m, int steps);
 int cats_gpu_llm_set_position(cats_gpu_llm *m, int token, int pos);
