@@ -134,8 +134,32 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
     a.n_heads = n_heads;
     a.mul = n_heads / c.n_kv;
     a.scale_log2 = 1.4426950408889634f / sqrtf((float)c.hs);
-    if (kv_attn_tile_takes(a, b.max_rows)) return launch_kv_attn_tile(a, b.max_rows, st);
-    return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
+    a.q_lo = 0;
+    a.q_hi = INT_MAX;
+    // The tile kernel reads the cache once per 256 query rows, in one CTA; the
+    // split kernel once per 16 (fp32: 8), in as many CTAs as there is work for.
+    // 128 tokens cost the one 2.5 us (fp32: 3.6) a CTA, whatever its rows, and
+    // the other some 1 / 75 us a unit over the whole GPU, so the tile kernel is
+    // for calls with 3200 query rows and more for each wave of its CTAs.
+    // Measured, tile / split, heads of 128: 16 runs of 4 rows x 64 heads after 1000
+    // tokens 35 / 55 us (fp16), 55 / 61 us (fp32); 64 rows of 32 heads after 8000
+    // tokens 164 / 84 us, 238 / 111 us; fp32, 2048 rows of 32 heads 203 / 1335 us.
+    const long long q_run = (long long)std::max(b.max_rows, 1) * a.mul;
+    const long long rows = std::min((long long)b.n_runs * std::max(b.max_rows, 1), (long long)q.rows);
+    const int per = kv_attn_tile_rows(a);
+    const long long ctas = std::min(b.n_runs * ((q_run + per - 1) / per), rows * a.mul / per + b.n_runs) * c.n_kv;
+    const int sms = 148;
+    if (!kv_attn_tile_takes(a) || q_run < 32 || rows * n_heads < 3200 * ((ctas + sms - 1) / sms))
+        return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
+    // Where most runs are short (decode steps beside a prompt) they keep to the
+    // split kernel: below 32 query rows a run costs less there even on a full GPU.
+    if (2 * rows < (long long)b.n_runs * b.max_rows) {
+        a.q_hi = a.q_lo = 32;
+        const cudaError_t e = launch_kv_attn_split(a, (a.q_hi + a.mul - 1) / a.mul, b.max_len, st);
+        if (e) return e;
+        a.q_hi = INT_MAX;
+    }
+    return launch_kv_attn_tile(a, b.max_rows, st);
 }
 
 // ------------------------------------------------------------- page copies

@@ -13,6 +13,7 @@ struct KvAttn {
     const KvRun *runs;
     int type, n_runs, n_heads, mul, tiles;   // tiles: row tiles per run in the grid
     float scale_log2;                        // log2(e) / sqrt(head size)
+    int q_lo, q_hi;                          // runs with q_lo <= query rows of a kv head < q_hi are this launch's
 };
 
 // The four pairs of halves of a code word: nibble i of each 16-bit side, (code
@@ -233,7 +234,8 @@ static __device__ __noinline__ float4 kv_plain_row4(const KvAttn &a, int seq, in
     return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-bool kv_attn_tile_takes(const KvAttn &a, int max_rows);
+int kv_attn_tile_rows(const KvAttn &a);   // query rows that a CTA of the tile kernel takes
+bool kv_attn_tile_takes(const KvAttn &a);
 cudaError_t launch_kv_attn_tile(const KvAttn &a, int max_rows, cudaStream_t st);
 cudaError_t launch_kv_attn_split(const KvAttn &a, int max_rows, int max_len, cudaStream_t st);
 

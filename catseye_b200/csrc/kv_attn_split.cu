@@ -78,7 +78,7 @@ __device__ __forceinline__ void finish4(const KvAttn &a, const KvRun &run, const
 __device__ __forceinline__ int steps_of(const KvAttn &a, const KvRun &run, const int2 &span, long long tile, int rows)
 {
     const long long n_q = (long long)(span.y - span.x) * a.mul;
-    if (tile * rows >= n_q) return 0;
+    if (tile * rows >= n_q || n_q >= a.q_hi) return 0;
     const int last = span.x + (int)((min(n_q, (tile + 1) * rows) - 1) / a.mul);
     const long long halves = min(((long long)run.pos + last) / SP_TOK + 1, 2ll * a.c.max_pages);
     return max(1, (int)((halves + SP_WARPS - 1) / SP_WARPS));
@@ -138,7 +138,8 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 const KvRun r = a.runs[i / a.tiles];
                 const int2 sp = kv_run_rows(r, a.q.rows, blockIdx.x == 0 ? a.c.err : nullptr);
                 v = (long long)steps_of(a, r, sp, i % a.tiles, ROWS) * a.c.n_kv;
-                beyond |= (long long)(sp.y - sp.x) * a.mul > (long long)a.tiles * ROWS;
+                const long long n_q = (long long)(sp.y - sp.x) * a.mul;
+                beyond |= n_q > (long long)a.tiles * ROWS && n_q < a.q_hi;
             }
             long long x = v;
 #pragma unroll
@@ -218,8 +219,8 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                     for (ri = 0; ri < a.n_runs && !found; ri++) {
                         run = a.runs[ri];
                         span = kv_run_rows(run, a.q.rows, nullptr);
-                        const long long over =
-                            max(0ll, ((long long)(span.y - span.x) * a.mul + ROWS - 1) / ROWS - a.tiles) * a.c.n_kv;
+                        const long long n_q = (long long)(span.y - span.x) * a.mul;
+                        const long long over = n_q < a.q_hi ? max(0ll, (n_q + ROWS - 1) / ROWS - a.tiles) * a.c.n_kv : 0;
                         if (i < over) {
                             found = true;
                             tile = a.tiles + i / a.c.n_kv;
@@ -237,7 +238,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
             span = kv_run_rows(run, a.q.rows, rank == 0 ? a.c.err : nullptr);
         }
         const long long n_q = (long long)(span.y - span.x) * a.mul;   // query rows of this kv head
-        if (!STREAM && tile * ROWS >= n_q) break;
+        if (!STREAM && (tile * ROWS >= n_q || n_q >= a.q_hi)) break;
         // The query row of column `col` of column tile t: fp32 rows take two
         // columns, their halves.
         const int used = (int)min((long long)ROWS, n_q - tile * ROWS);

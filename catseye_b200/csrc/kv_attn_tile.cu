@@ -1,5 +1,5 @@
 // kv_attn_tile.cu — attention over the paged Q4_0 cache for many query rows
-// (prompts), 16-bit rows, on the 5th-generation tensor cores.
+// (prompts) on the 5th-generation tensor cores.
 //
 // A CTA takes 256 query rows of a kv head (tokens x the query heads that share
 // it) as two tiles of 128, and goes through the sequence 128 tokens at a time:
@@ -8,18 +8,25 @@
 //   O_i += P_i V       A = P in TMEM, B = V in shared memory, O in TMEM
 // with the running maximum m and sum of a softmax per row.  The two tiles take
 // turns: while one's probabilities are computed the other's products run.
+// fp32 rows: q and p are two fp16 halves each (22 bits), two products each into
+// the same accumulator; O holds one tile of tokens and is added to R in TMEM,
+// which at heads of 128 leaves room for one tile of rows.
 //
 // Roles: warps 0-3 and 4-7 the rows of the two tiles (they also bring Q in and
-// store O), warps 8-15 dequantize the cache's codes into the products' operand
-// layout (128-byte swizzle, two stages), warp 16 issues the products, warp 17
+// store O), warps 8-11 dequantize the cache's codes into the products' operand
+// layout (128-byte swizzle, two stages), warp 12 issues the products, warp 13
 // brings the codes to shared memory with bulk copies, three half tiles ahead.
 // (Codes loaded to registers a tile ahead made each proxy fence wait for them.)  The
 // codes are read once per 256 rows; the values (code - 8) * scale are exact in
 // fp16 (kv.cuh), so the products' operands are the cache's values.
 //
-// Bound by the exponentials and the tensor cores alike: a 128 x 128 tile costs
-// 1024 cycles of both (16 exponentials a cycle; 2 x 512 cycles of products).
-// So the accumulator is not rescaled for every new maximum: m is only moved
+// Bound by a tile's chain: 128 tokens take a row's thread some 2900 cycles (its
+// exponentials alone 1024, sixteen a cycle and SM) and then the products 1000,
+// which the other tile's rows hide only in part.  4096 rows of 32 heads of 128
+// (bf16, causal): 225 us, 611 TFLOP/s; 64 tokens at a time with S twice 260 us,
+// two threads a row 313 us, eight dequantizing warps 249 us, S loaded a piece
+// ahead 250 us: all of them more code, and the roles share one instruction
+// cache.  The accumulator is not rescaled for every new maximum: m is only moved
 // when a row's maximum passes it by 2^8, which happens once or twice a row.
 //
 // Every wait is bounded; TMEM is freed on every path.
@@ -30,19 +37,23 @@
 
 namespace cats {
 
-constexpr int TI_ROWS = 256, TI_KV = 128;
+constexpr int TI_KV = 128;
+// tiles of 128 query rows a CTA takes: two, or what TMEM has room for beside R
+__host__ __device__ constexpr int ti_q_tiles(int hs, bool f32) { return f32 && hs == 128 ? 1 : 2; }
 constexpr int TI_SOFT = 8, TI_DEQ = 4, TI_MMA_WARP = TI_SOFT + TI_DEQ, TI_LOAD_WARP = TI_MMA_WARP + 1,
               TI_THREADS = (TI_LOAD_WARP + 1) * 32;
 constexpr float TI_P_BITS = 7.f, TI_LAG = 8.f;   // probabilities are held times 2^7 and may reach 2^15
 
-// shared memory, from a 1024-byte boundary: Q [2][HS/64][128 rows][128 B], K the
-// same per stage, V [2 pages][HS rows][128 B] per stage, three buffers of raw
-// codes (K and V of a tile by turns), barriers
-template <int HS> struct TileSmem {
+// shared memory, from a 1024-byte boundary: Q [2][HS/64][128 rows][128 B] (fp32
+// rows: both halves of each tile), K the same per stage, V [2 pages][HS rows]
+// [128 B] per stage, three buffers of raw codes (K and V of a tile by turns),
+// barriers
+template <int HS, bool F32> struct TileSmem {
     static constexpr int SLICE = 128 * 128;                  // 128 rows of 64 halves
-    static constexpr int Q_TILE = HS / 64 * SLICE, K_STAGE = HS / 64 * SLICE, V_PAGE = HS * 128, V_STAGE = 2 * V_PAGE;
+    static constexpr int QT = ti_q_tiles(HS, F32);
+    static constexpr int Q_HALF = HS / 64 * SLICE, Q_TILE = (F32 ? 2 : 1) * Q_HALF, K_STAGE = HS / 64 * SLICE, V_PAGE = HS * 128, V_STAGE = 2 * V_PAGE;
     static constexpr int RAW_UNIT = 72 * HS;                 // K or V of two pages: codes, then scales
-    static constexpr int K = 2 * Q_TILE, V = K + 2 * K_STAGE, RAW = V + 2 * V_STAGE, BAR = RAW + 3 * RAW_UNIT;
+    static constexpr int K = QT * Q_TILE, V = K + 2 * K_STAGE, RAW = V + 2 * V_STAGE, BAR = RAW + 3 * RAW_UNIT;
     static constexpr int BYTES = BAR + 256 + 1024;           // + the alignment's slack
 };
 
@@ -120,10 +131,10 @@ __device__ __forceinline__ void ti_wait_ld() { asm volatile("tcgen05.wait::ld.sy
 __device__ __forceinline__ void ti_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A row's maximum has moved: its accumulator (o_cols columns, 0: none yet) and
-// the probabilities of this tile so far (done pieces of 16 columns) follow by
+// the probabilities of this tile so far (done pieces of 32 tokens) follow by
 // al.  Out of line: it runs once or twice a row, and the loop around it has to
 // fit the instruction cache.
-__device__ __noinline__ void ti_rescale(uint32_t O, int o_cols, uint32_t P, int done, float al)
+template <bool F32> __device__ __noinline__ void ti_rescale(uint32_t O, int o_cols, uint32_t P, int done, float al)
 {
     uint32_t v[16];
 #pragma unroll 1
@@ -137,22 +148,57 @@ __device__ __noinline__ void ti_rescale(uint32_t O, int o_cols, uint32_t P, int 
     ti_wait_st();
 #pragma unroll 1
     for (int ch = 0; ch < done; ch++) {
-        ti_ld16(v, P + 16 * ch);
+        const uint32_t at = P + (F32 ? 32 : 16) * ch;
+        uint32_t rest[16];
+        ti_ld16(v, at);
+        if (F32) ti_ld16(rest, at + 16);
         ti_wait_ld();
 #pragma unroll
         for (int k = 0; k < 16; k++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
-            v[k] = kv_pack(f.x * al, f.y * al);
+            float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+            if (F32) {
+                const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&rest[k]));
+                f = make_float2((f.x + g.x) * al, (f.y + g.y) * al);
+                v[k] = kv_pack(f.x, f.y);
+                rest[k] = kv_pack(kv_rest(f.x), kv_rest(f.y));
+            } else {
+                v[k] = kv_pack(f.x * al, f.y * al);
+            }
         }
-        ti_st16(P + 16 * ch, v);
+        ti_st16(at, v);
+        if (F32) ti_st16(at + 16, rest);
     }
 }
 
-template <int HS>
+// R += O (more: R has something), rounded
+__device__ __noinline__ void ti_fold(uint32_t O, uint32_t R, int cols, bool more)
+{
+#pragma unroll 1
+    for (int ch = 0; ch < cols; ch += 32) {
+        uint32_t v[2][16], x[2][16];
+        ti_ld16(v[0], O + ch);
+        ti_ld16(v[1], O + ch + 16);
+        if (more) {
+            ti_ld16(x[0], R + ch);
+            ti_ld16(x[1], R + ch + 16);
+        }
+        ti_wait_ld();
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+                if (more) v[h][k] = __float_as_uint(__uint_as_float(v[h][k]) + __uint_as_float(x[h][k]));
+            ti_st16(R + ch + 16 * h, v[h]);
+        }
+    }
+    ti_wait_st();
+}
+
+template <int HS, bool F32>
 __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_constant__ KvAttn a)
 {
-    using L = TileSmem<HS>;
-    constexpr int HB = HS / 32;
+    using L = TileSmem<HS, F32>;
+    constexpr int HB = HS / 32, QT = L::QT, ROWS = 128 * QT;
     extern __shared__ uint8_t raw_smem[];
     uint8_t *sm = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
     uint64_t *bar = reinterpret_cast<uint64_t *>(sm + L::BAR);
@@ -163,7 +209,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
-        mbar_init(&bar[B_Q], TI_SOFT);
+        mbar_init(&bar[B_Q], 4 * QT);
         for (int s = 0; s < 2; s++) {
             mbar_init(&bar[B_KF + s], TI_DEQ);
             mbar_init(&bar[B_KE + s], 1);
@@ -187,7 +233,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;   // S_0, S_1 (128 columns each; P_i over the first 64 of S_i), O_0, O_1
+        // S_0, S_1 (128 columns each; P_i over S_i), O_0, O_1; fp32 rows: R_0, R_1 too
+    const uint32_t tmem = *slot;
+    constexpr int O_AT = 256, O_STEP = F32 ? HS : 128, R_AT = O_AT + QT * O_STEP;
+    static_assert(!F32 || R_AT + QT * HS <= 512, "");
 
     const int kvh = blockIdx.x;
     const KvRun run = a.runs[blockIdx.z];
@@ -200,17 +249,17 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     uint32_t kv_it = 0, q_it = 0, s_it[2] = {0, 0}, o_it[2] = {0, 0};
 
     // the longest tiles (the last ones) of every head first
-    const long long mine = n_q > 0 ? (n_q + TI_ROWS - 1) / TI_ROWS : 0;
+    const long long mine = n_q >= max(a.q_lo, 1) ? (n_q + ROWS - 1) / ROWS : 0;
     for (long long back = blockIdx.y; back < mine; back += a.tiles) {
         const long long tile = mine - 1 - back;
         // per Q tile: KV tiles, the first position that some row does not see
         int n[2], low[2], top = -1;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const long long r0 = tile * TI_ROWS + 128 * i, r1 = min(n_q, r0 + 128) - 1;
+            const long long r0 = tile * ROWS + 128 * i, r1 = min(n_q, r0 + 128) - 1;
             n[i] = 0;
             low[i] = -1;
-            if (r0 < n_q && seq_ok) {
+            if (i < QT && r0 < n_q && seq_ok) {
                 const long long p0 = (long long)run.pos + span.x + r0 / a.mul, p1 = (long long)run.pos + span.x + r1 / a.mul;
                 const long long t = min(p1, cap - 1);
                 n[i] = t < 0 ? 0 : (int)(t / TI_KV) + 1;
@@ -220,16 +269,41 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
         }
         const int tiles = max(n[0], n[1]);
 
-        if (warp < TI_SOFT) {
+        if (warp < 4 * QT) {
             // ------------------------------------------------ rows
             const int i = warp >> 2, r = tid & 127;
-            const long long rr = tile * TI_ROWS + 128 * i + r;
+            const long long rr = tile * ROWS + 128 * i + r;
             const bool real = rr < n_q;
             const int tok = span.x + (real ? (int)(rr / a.mul) : 0), head = kvh * a.mul + (real ? (int)(rr % a.mul) : 0);
             const int lim = real ? kv_limit(a.c, run, tok) : -1;
             const size_t at = (size_t)(run.first + tok) * a.q.ld + (size_t)head * HS;
             float sc, kf;
-            {
+            if constexpr (F32) {   // two halves, 22 bits of a value; the row is read twice
+                float amax = 0.f;
+#pragma unroll 4
+                for (int ci = 0; ci < HS / 8 && real; ci++) {
+                    float x[8];
+                    kv_load_row<8>(a.q, KV_F32, at + 8 * ci, x);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(x[e]));
+                }
+                sc = kv_row_scale(amax);
+                kf = a.scale_log2 / sc;
+#pragma unroll 2
+                for (int ci = 0; ci < HS / 8; ci++) {
+                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (real) kv_load_row<8>(a.q, KV_F32, at + 8 * ci, x);
+                    uint32_t h[4], rest[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        h[u] = kv_pack(sc * x[u], sc * x[u + 4]);
+                        rest[u] = kv_pack(kv_rest(sc * x[u]), kv_rest(sc * x[u + 4]));
+                    }
+                    uint8_t *dst = sm + i * L::Q_TILE + (ci >> 3) * L::SLICE + sw128(r, ci & 7);
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(dst + L::Q_HALF) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                }
+            } else {
                 uint2 x[HS / 4];   // the row, all its loads in flight at once
                 const uint16_t *p = static_cast<const uint16_t *>(a.q.p) + at;
 #pragma unroll
@@ -262,10 +336,23 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar[B_Q]);
 
-            const uint32_t lanes = (uint32_t)(warp & 3) << 21, S = tmem + lanes + 128 * i, O = tmem + lanes + 256 + 128 * i;
+            const uint32_t lanes = (uint32_t)(warp & 3) << 21, S = tmem + lanes + 128 * i, O = tmem + lanes + O_AT + O_STEP * i,
+                           R = tmem + lanes + R_AT + O_STEP * i;
             float m = -INFINITY, l = 0.f;
             bool ok = true;
+            // fp32 rows: the tensor cores cut their running sums off instead of
+            // rounding them, some 2^-25 of the sum an instruction, always towards zero.
+            // So O holds one tile of tokens and is then added, rounded, to R.  (2.1e-6 off
+            // after 1200 tokens with one accumulator throughout, 5e-7 with R.)
+            const size_t to = (size_t)(run.first + tok) * a.out.ld + (size_t)head * HS;
             for (int j = 0; j < n[i]; j++) {
+                if (F32 && j > 0) {   // while the products for S run
+                    ok = ti_wait(&bar[B_O + i], o_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    ti_fold(O, R, HS, j > 1);
+                }
                 ok = ti_wait(&bar[B_S + i], s_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
@@ -299,7 +386,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                         sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
                         if (far) m = mn;
                         // (the products so far are complete: S came after them)
-                        ti_rescale(O, j > 0 ? HS : 0, S, ch, al);
+                        ti_rescale<F32>(F32 ? R : O, j > 0 ? HS : 0, S, ch, al);
                     }
                     const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
 #pragma unroll
@@ -308,8 +395,15 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                         sum[k & 2] += e0;
                         sum[(k & 2) + 1] += e1;
                         w[k >> 1] = kv_pack(e0, e1);
+                        if (F32) v[k >> 1] = kv_pack(kv_rest(e0), kv_rest(e1));
                     }
-                    ti_st16(S + 16 * ch, w);
+                    // fp32 rows: over the piece of S it comes from, both halves
+                    ti_st16(S + (F32 ? 32 : 16) * ch, w);
+                    if (F32) {
+#pragma unroll
+                        for (int k = 0; k < 16; k++) w[k] = v[k];
+                        ti_st16(S + 32 * ch + 16, w);
+                    }
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 ti_wait_st();
@@ -321,16 +415,16 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 ok = ti_wait(&bar[B_O + i], o_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
+                if (F32) ti_fold(O, R, HS, n[i] > 1);
             }
             const float inv = !ok || *abort_s ? NAN : l == 0.f ? 0.f : 1.f / l;
-            const size_t to = (size_t)(run.first + tok) * a.out.ld + (size_t)head * HS;
 #pragma unroll 1
             for (int ch = 0; ch < HS; ch += 32) {
                 uint32_t v[32];
 #pragma unroll
                 for (int k = 0; k < 32; k++) v[k] = 0u;
                 if (n[i] > 0) {
-                    ti_ld32(v, O + ch);
+                    ti_ld32(v, (F32 ? R : O) + ch);
                     ti_wait_ld();
                 }
                 if (real) {
@@ -346,6 +440,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 }
             }
             tc_fence_before();
+        } else if (warp < TI_SOFT) {   // (a CTA of one tile has four warps less)
         } else if (warp < TI_MMA_WARP) {
             // ------------------------------------------------ the cache's codes to operands
             const int w = warp - TI_SOFT;
@@ -361,7 +456,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 return (int)(u % 3) * L::RAW_UNIT;
             };
             auto stage_free = [&](int b, uint32_t it) {
-                ok = ti_wait(&bar[b + (it & 1)], (it >> 1) + 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
+                ok = ti_wait(&bar[b + it % 2], it / 2 + 1, abort_s, a.c.err, CATS_DEVERR_MBAR_EMPTY);
                 ok = __all_sync(0xffffffffu, ok);
             };
             // Where this lane reads and writes; what a loop adds is constant.  K: token 32w +
@@ -382,7 +477,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             };
             for (int j = 0; j < tiles && ok; j++) {
                 const uint32_t it = kv_it + j, u0 = 2 * it;
-                const int st = it & 1, p0 = j * TI_KV;
+                const int st = it % 2, p0 = j * TI_KV;
                 // ---- K: warp w takes tokens 32w .. 32w + 31 of the tile
                 int raw = raw_unit(u0);
                 if (!ok) break;
@@ -487,18 +582,20 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                            v_d = umma_desc_sw128(smem_u32(sm + L::V));   // + bytes / 16
             bool ok = true;
             auto qk = [&](int i, uint32_t it) {
-                const uint64_t qi = q_d + i * (L::Q_TILE / 16), ks = k_d + (it & 1) * (L::K_STAGE / 16);
+                const uint64_t qi = q_d + i * (L::Q_TILE / 16), ks = k_d + it % 2 * (L::K_STAGE / 16);
                 if (ti_elect()) {
 #pragma unroll
-                    for (int k = 0; k < HS / 16; k++)
-                        ti_mma_ss(tmem + 128 * i, qi + ((k >> 2) * L::SLICE + (k & 3) * 32) / 16,
-                                  ks + ((k >> 2) * L::SLICE + (k & 3) * 32) / 16, id_qk, k > 0);
+                    for (int h = F32; h >= 0; h--)   // (the rests first: they are the smaller)
+#pragma unroll
+                        for (int k = 0; k < HS / 16; k++)
+                            ti_mma_ss(tmem + 128 * i, qi + (h * L::Q_HALF + (k >> 2) * L::SLICE + (k & 3) * 32) / 16,
+                                      ks + ((k >> 2) * L::SLICE + (k & 3) * 32) / 16, id_qk, h < F32 || k > 0);
                     ti_commit(&bar[B_S + i]);
                 }
                 __syncwarp();
             };
             auto k_full = [&](uint32_t it) {
-                if (ok) ok = ti_wait(&bar[B_KF + (it & 1)], it >> 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                if (ok) ok = ti_wait(&bar[B_KF + it % 2], it / 2, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after();
             };
@@ -507,14 +604,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 k_full(kv_it);
                 for (int i = 0; i < 2 && ok; i++)
                     if (n[i] > 0) qk(i, kv_it);
-                if (ok && ti_elect()) ti_commit(&bar[B_KE + (kv_it & 1)]);
+                if (ok && ti_elect()) ti_commit(&bar[B_KE + kv_it % 2]);
                 __syncwarp();
             }
             for (int j = 0; j < tiles && ok; j++) {
                 const uint32_t it = kv_it + j;
-                ok = ti_wait(&bar[B_VF + (it & 1)], it >> 1, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
+                ok = ti_wait(&bar[B_VF + it % 2], it / 2, abort_s, a.c.err, CATS_DEVERR_MBAR_FULL);
                 if (j + 1 < tiles) k_full(it + 1);
-                const uint64_t vs = v_d + (it & 1) * (L::V_STAGE / 16);
+                const uint64_t vs = v_d + it % 2 * (L::V_STAGE / 16);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     if (j >= n[i] || !ok) continue;
@@ -524,18 +621,21 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     tc_fence_after();
                     if (ti_elect()) {
 #pragma unroll
-                        for (int k = 0; k < TI_KV / 16; k++)
-                            ti_mma_ts(tmem + 256 + 128 * i, tmem + 128 * i + 8 * k, vs + ((k >> 2) * L::V_PAGE + (k & 3) * 32) / 16, id_pv,
-                                      j > 0 || k > 0);
-                        if (j + 1 == n[i]) ti_commit(&bar[B_O + i]);
+                        for (int k = 0; k < TI_KV / 16; k++) {
+                            const uint64_t vk = vs + ((k >> 2) * L::V_PAGE + (k & 3) * 32) / 16;
+                            const uint32_t o = tmem + O_AT + O_STEP * i, p = tmem + 128 * i + (F32 ? 32 * (k >> 1) + 8 * (k & 1) : 8 * k);
+                            ti_mma_ts(o, p, vk, id_pv, (!F32 && j > 0) || k > 0);
+                            if (F32) ti_mma_ts(o, p + 16, vk, id_pv, 1);
+                        }
+                        if (F32 || j + 1 == n[i]) ti_commit(&bar[B_O + i]);
                     }
                     __syncwarp();
                     if (j + 1 < n[i]) qk(i, it + 1);
                 }
                 if (!ok) break;
                 if (ti_elect()) {
-                    ti_commit(&bar[B_VE + (it & 1)]);
-                    if (j + 1 < tiles) ti_commit(&bar[B_KE + ((it + 1) & 1)]);
+                    ti_commit(&bar[B_VE + it % 2]);
+                    if (j + 1 < tiles) ti_commit(&bar[B_KE + (it + 1) % 2]);
                 }
                 __syncwarp();
             }
@@ -554,30 +654,30 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-template <int HS> static cudaError_t launch_tile(const KvAttn &a, dim3 grid, cudaStream_t st)
+template <int HS, bool F32> static cudaError_t launch_tile(const KvAttn &a, dim3 grid, cudaStream_t st)
 {
     static unsigned long long done = 0;
-    const int smem = TileSmem<HS>::BYTES;
+    const int smem = TileSmem<HS, F32>::BYTES;
     cudaError_t e = once_per_device(
-        done, [&] { return cudaFuncSetAttribute(k_kv_attn_tile<HS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+        done, [&] { return cudaFuncSetAttribute(k_kv_attn_tile<HS, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     if (e) return e;
-    k_kv_attn_tile<HS><<<grid, TI_THREADS, smem, st>>>(a);
+    k_kv_attn_tile<HS, F32><<<grid, TI_THREADS, smem, st>>>(a);
     return cudaGetLastError();
 }
 
-bool kv_attn_tile_takes(const KvAttn &a, int max_rows)
-{
-    return a.type != KV_F32 && (a.c.hs == 64 || a.c.hs == 128) && a.n_runs <= 65535 &&
-           (long long)max_rows * a.mul >= 64;
-}
+int kv_attn_tile_rows(const KvAttn &a) { return 128 * ti_q_tiles(a.c.hs, a.type == KV_F32); }
+
+bool kv_attn_tile_takes(const KvAttn &a) { return (a.c.hs == 64 || a.c.hs == 128) && a.n_runs <= 65535; }
 
 cudaError_t launch_kv_attn_tile(const KvAttn &a0, int max_rows, cudaStream_t st)
 {
     KvAttn a = a0;
     const long long q = (long long)std::max(max_rows, 1) * a.mul;
-    a.tiles = (int)std::min<long long>((q + TI_ROWS - 1) / TI_ROWS, 65535);
+    const int rows = kv_attn_tile_rows(a);
+    a.tiles = (int)std::min<long long>((q + rows - 1) / rows, 65535);
     const dim3 grid((unsigned)a.c.n_kv, (unsigned)a.tiles, (unsigned)a.n_runs);
-    return a.c.hs == 64 ? launch_tile<64>(a, grid, st) : launch_tile<128>(a, grid, st);
+    if (a.type == KV_F32) return a.c.hs == 64 ? launch_tile<64, true>(a, grid, st) : launch_tile<128, true>(a, grid, st);
+    return a.c.hs == 64 ? launch_tile<64, false>(a, grid, st) : launch_tile<128, false>(a, grid, st);
 }
 
 } // namespace cats

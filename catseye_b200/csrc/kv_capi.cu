@@ -130,7 +130,7 @@ int cats_gpu_kv_attention_dev(const cats_gpu_kv *c, int layer, void *out, const 
     KvView view;
     KvRows rq, ro;
     if (rows == 0 || n_runs == 0) return CATS_OK;
-    if (!tabled(c) || !view_of(c, layer, &view) || !runs || n_runs < 0 || max_rows < 0 || max_len < 0 ||
+    if (!tabled(c) || !view_of(c, layer, &view) || !runs || n_runs < 0 || max_rows < 0 || max_len < 0 || out == q ||
         n_heads <= 0 || n_heads % c->n_kv_heads ||
         !rows_ok(q, type, ld_q, rows, (long long)n_heads * c->head_size, &rq) ||
         !rows_ok(out, type, ld_out, rows, (long long)n_heads * c->head_size, &ro))

@@ -327,6 +327,47 @@ def test_rows_in_stretches(dtype, hint, new, lens):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("new,lens", [([700], [1800]), ([300, 1, 0, 2, 1, 1, 5], [900, 1300, 10, 200, 64, 1, 517]),
+                                      ([250, 250, 249], [250, 1250, 513])])
+def test_long_prompts(dtype, hs, new, lens):
+    """Rows for several tiles over several tiles of tokens; prompts beside single tokens."""
+    c = make(lens, 4, hs)
+    fill(c, lens)
+    q, out, runs = attend(c, 1, new, lens, 4, dtype)
+    check_attention(c, 1, q, out, runs, 4, untouched=3)
+    assert _lib.load().cats_gpu_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_prompts_with_holes_and_nan(dtype):
+    """A NaN value row seen by the last rows only, one that is not seen, a page
+    that is missing, maxima that move late, rows before position 0."""
+    lens = [900, 1400]
+    c = make(lens, 4, 64)
+    fill(c, lens)
+    x = randn(64, 4, 64, seed=1)
+    c.append(0, x * 8, x, runs_of([(0, 64, 0, 800)]), 64)             # large keys late in the sequence
+    nan = torch.full_like(x, math.nan)
+    c.append(0, x, nan, runs_of([(0, 1, 0, 100), (0, 1, 1, 1390)]), 1)
+    q = randn(820, 16, 64, seed=3).to(dtype)
+    out = torch.full_like(q, 3)
+    runs = [(0, 400, 0, -320), (400, 400, 1, 1000), (800, 20, 0, 880)]
+    c.attention(0, out, q, runs_of(runs), 400, 1400)
+    o = out.double().cpu().numpy()
+    assert (o[:320] == 0).all() and np.isfinite(o[:400]).all() and np.isfinite(o[400:790]).all()
+    assert np.isnan(o[790:800]).all() and np.isnan(o[800:]).all()
+    check_attention(c, 0, q, out, [(0, 400, 0, -320), (400, 390, 1, 1000)], 4)
+    plain = torch.full_like(q, 3)
+    c.table[1, 9] = -1
+    c.attention(0, out, q, runs_of(runs[1:2]), 400, 1400)
+    c.attention(0, plain, q, runs_of(runs[1:2]), 1, 1400)             # the other kernel, by its hint
+    torch.cuda.synchronize()
+    assert _lib.load().cats_gpu_device_error() == 0x40
+    assert (out[400:790].float() - plain[400:790].float()).abs().max() < (2**-16 if dtype == torch.float32 else 2**-7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_stretches_with_holes_and_what_is_masked(dtype):
     """Missing pages, rows before position 0, a batch of empty runs, NaN behind the mask: in stretches as in one piece."""
     lens = [700, 300]
