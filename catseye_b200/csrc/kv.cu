@@ -40,12 +40,26 @@ __global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvVi
                 const size_t at = (size_t)(run.first + r0) * t.ld + (size_t)head * c.hs + 8 * e8;
                 const int slot = (int)(2 * pair & (KV_PAGE - 1));
                 float x[2][8];
-                if constexpr (APPEND) {
+                uint32_t w[2][4];
+                if constexpr (APPEND) {   // (does not wait for the table)
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
+                        const size_t from = at + (u ? t.ld : 0);
+                        if constexpr (type == KV_F32) {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) x[u][j] = 0.f;
-                        if (in[u]) kv_load_row<8>(t, type, at + (u ? t.ld : 0), x[u]);   // (does not wait for the table)
+                            for (int j = 0; j < 8; j++) x[u][j] = 0.f;
+                            if (in[u]) kv_load_row<8>(t, type, from, x[u]);
+                        } else {
+                            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
+                            const uint16_t *p = static_cast<const uint16_t *>(t.p) + from;
+                            if (in[u] && t.vec) {
+                                const uint2 a = *reinterpret_cast<const uint2 *>(p), b = *reinterpret_cast<const uint2 *>(p + 4);
+                                w[u][0] = a.x; w[u][1] = a.y; w[u][2] = b.x; w[u][3] = b.y;
+                            } else if (in[u]) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) w[u][j] = p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
+                            }
+                        }
                     }
                 }
                 const int page = c.page(run.seq, pair < 0 ? -1 : (int)min(pair / (KV_PAGE / 2), (long long)INT_MAX));
@@ -55,7 +69,10 @@ __global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvVi
                     uint32_t codes[2];
                     uint16_t scale[2];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) codes[u] = kv_quant8(x[u], mask, &scale[u]);
+                    for (int u = 0; u < 2; u++) {
+                        if constexpr (type == KV_F32) codes[u] = kv_quant8(x[u], mask, &scale[u]);
+                        else codes[u] = kv_quant8_half<type>(w[u], mask, &scale[u]);
+                    }
                     if (is_v && in[0] && in[1]) {
                         kv_store_pair8(ch, c.hs, slot, e8, codes[0], codes[1], scale[0], scale[1]);
                         continue;
@@ -73,16 +90,46 @@ __global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvVi
                             uint32_t h[4];
                             kv_dequant(kv_codes8(ch, is_v, c.hs, slot + u, e8),
                                        __half2half2(kv_scale8(ch, is_v, c.hs, slot + u, e8)), magic, h);
+                            if constexpr (type == KV_F16) {   // the values as they are
+                                w[u][0] = __byte_perm(h[0], h[1], 0x5410);
+                                w[u][1] = __byte_perm(h[2], h[3], 0x5410);
+                                w[u][2] = __byte_perm(h[0], h[1], 0x7632);
+                                w[u][3] = __byte_perm(h[2], h[3], 0x7632);
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-                                x[u][j] = f.x;
-                                x[u][j + 4] = f.y;
+                                for (int j = 0; j < 4; j++) {
+                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+                                    x[u][j] = f.x;
+                                    x[u][j + 4] = f.y;
+                                }
                             }
+                        } else if constexpr (type == KV_F16) {
+                            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
                         }
                         const size_t to = at + (u ? t.ld : 0);
-                        kv_store_row4(t, type, to, make_float4(x[u][0], x[u][1], x[u][2], x[u][3]));
-                        kv_store_row4(t, type, to + 4, make_float4(x[u][4], x[u][5], x[u][6], x[u][7]));
+                        if constexpr (type == KV_F32) {
+                            kv_store_row4(t, type, to, make_float4(x[u][0], x[u][1], x[u][2], x[u][3]));
+                            kv_store_row4(t, type, to + 4, make_float4(x[u][4], x[u][5], x[u][6], x[u][7]));
+                        } else {
+                            if constexpr (type == KV_BF16) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    const __nv_bfloat162 b = __floats2bfloat162_rn(x[u][2 * j], x[u][2 * j + 1]);
+                                    w[u][j] = *reinterpret_cast<const uint32_t *>(&b);
+                                }
+                            }
+                            uint16_t *p = static_cast<uint16_t *>(t.p) + to;
+                            if (t.vec) {
+                                *reinterpret_cast<uint2 *>(p) = make_uint2(w[u][0], w[u][1]);
+                                *reinterpret_cast<uint2 *>(p + 4) = make_uint2(w[u][2], w[u][3]);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    p[2 * j] = (uint16_t)w[u][j];
+                                    p[2 * j + 1] = (uint16_t)(w[u][j] >> 16);
+                                }
+                            }
+                        }
                     }
                 }
             }

@@ -23,6 +23,7 @@
 #pragma once
 #include "common.cuh"
 #include <cuda_bf16.h>
+#include <type_traits>
 
 namespace cats {
 
@@ -150,6 +151,47 @@ __device__ __forceinline__ uint32_t kv_quant8(const float (&x)[8], unsigned mask
     // + 8 for every code: the codes are the low 16 bits of an integer above 2^23
     return (__float_as_uint(sum[0] + (34952.f + 8388608.f)) & 0xffffu) | __float_as_uint(sum[1] + (34952.f + 8388608.f)) << 16;
 }
+// The same block of fp16 or bf16 values, eight a lane as they lie in memory (w).
+// The border that x / d is nearest to, x / d itself or half a code from it, is
+// decided without a remainder: x has p <= 11 significant bits and d 8, so where
+// x / d is not on a border it is at least (1 - 2^-12) 2^-(p + 2) >= 0.999 2^-13
+// away.  So y = x / d + 8.5 + 2^-14, whose floor is the code, may be off by up to
+// 2^-14 - 2^-25 either way: 2^-20 from the reciprocal (2^-23 of 8.5), 2^-21 from
+// the saturated sixteenth, 2^-16 from the factor that keeps 16 below itself,
+// 2^-17 from the sum with 128, in all 2.5e-5 of 6.1e-5.  The floor is then the third byte
+// of 128 + y.
+template <int TYPE> __device__ __forceinline__ uint32_t kv_quant8_half(const uint32_t (&w)[4], unsigned mask, uint16_t *scale)
+{
+    using T2 = std::conditional_t<TYPE == KV_F16, __half2, __nv_bfloat162>;
+    auto two = [](uint32_t v) { return *reinterpret_cast<const T2 *>(&v); };
+    auto word = [](T2 v) { return *reinterpret_cast<const uint32_t *>(&v); };
+    auto low = [](uint32_t v) { return TYPE == KV_F16 ? __half2float(__ushort_as_half((uint16_t)v)) : __uint_as_float(v << 16); };
+    auto high = [](uint32_t v) { return TYPE == KV_F16 ? __half2float(__ushort_as_half((uint16_t)(v >> 16))) : __uint_as_float(v & 0xffff0000u); };
+    const uint32_t hi = word(__hmax2_nan(__hmax2_nan(two(w[0]), two(w[1])), __hmax2_nan(two(w[2]), two(w[3]))));
+    const uint32_t lo = word(__hmin2_nan(__hmin2_nan(two(w[0]), two(w[1])), __hmin2_nan(two(w[2]), two(w[3])))) ^ 0x80008000u;
+    uint32_t top = word(__hmax2_nan(two(__byte_perm(hi, lo, 0x5410)), two(__byte_perm(hi, lo, 0x7632))));   // (largest, minus the smallest)
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) top = word(__hmax2_nan(two(top), two(__shfl_xor_sync(mask, top, o))));
+    const float above = low(top), below = high(top), m = above >= below ? above : -below;
+    const bool bad = !(above < INFINITY && below < INFINITY);
+    const __half dh = __float2half_rn(fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(m * -0.125f)), -8160.f), 8160.f));
+    const float d = __half2float(dh);
+    *scale = bad ? 0x7fff : __half_as_ushort(dh);
+    if (bad || d == 0.f) return 0x88888888u;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+    inv *= 0.0625f;
+    uint32_t y[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float x = j & 1 ? high(w[j >> 1]) : low(w[j >> 1]);
+        y[j] = __float_as_uint(fmaf(__saturatef(fmaf(x, inv, (8.5f + 0x1p-14f) / 16.f)), 16.f - 0x1p-16f, 128.f));
+    }
+    const uint32_t even = __byte_perm(__byte_perm(y[0], y[2], 0x0062), __byte_perm(y[4], y[6], 0x0062), 0x5410) & 0x0f0f0f0fu;
+    const uint32_t odd = __byte_perm(__byte_perm(y[1], y[3], 0x0062), __byte_perm(y[5], y[7], 0x0062), 0x5410) & 0x0f0f0f0fu;
+    return even | odd << 4;
+}
+
 // ... and where a row's eight e8 go (K: one word; V: half of two words)
 __device__ __forceinline__ void kv_store_codes8(uint8_t *chunk, bool is_v, int hs, int slot, int e8, uint32_t codes, uint16_t scale)
 {

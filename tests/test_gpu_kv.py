@@ -120,7 +120,8 @@ def test_append_and_read_hold_the_definition(dtype, hs, n_kv):
     assert _lib.load().cats_gpu_device_error() == 0
 
 
-def test_quantizer_at_its_borders():
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantizer_at_its_borders(dtype):
     """Values next to and on the borders between codes, blocks of zeros, of one
     sign, of both extremes, tiny, subnormal, saturating, and non-finite ones."""
     d = np.float32(0.40625)
@@ -146,16 +147,38 @@ def test_quantizer_at_its_borders():
         b = base.copy()
         b[rng.integers(32)] = bad
         rows.append(b)
-    x = torch.tensor(np.array(rows, np.float32), device="cuda")[:, None]          # [n, 1, 32]
+    x = torch.tensor(np.array(rows, np.float32), device="cuda").to(dtype)[:, None]          # [n, 1, 32]
     n = x.shape[0]
     c = make([n], 1, 32, layers=1)
     run = runs_of([(0, n, 0, 0)])
     c.append(0, x, x, run, n)
     k, v = torch.empty_like(x), torch.empty_like(x)
     c.read(0, k, v, run, n)
-    want = blocks(x.cpu().numpy())
-    assert np.array_equal(k.cpu().numpy(), want, equal_nan=True)
-    assert np.array_equal(v.cpu().numpy(), want, equal_nan=True)
+    want = torch.from_numpy(blocks(x.double().cpu().numpy())).to(dtype).double().numpy()
+    assert np.array_equal(k.double().cpu().numpy(), want, equal_nan=True)
+    assert np.array_equal(v.double().cpu().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_quantizer_on_every_16_bit_value(dtype, sign):
+    """Every finite value in blocks of every significand a scale can have, at
+    scales that make it small, large, out of range and subnormal."""
+    every = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    every = every[torch.isfinite(every.float())]
+    for top in [sign * 8 * s * (128 + i) / 128 for i in range(0, 128, 5 if sign < 0 else 3) for s in (1.0,)] + \
+            [sign * 2.0 ** e for e in (-24, -16, -14, 9, 13, 15)]:
+        x = every[(every.abs() <= abs(torch.tensor(top).to(dtype).float())) & (every.abs() >= abs(top) * 2.0**-6)]
+        x = torch.nn.functional.pad(x, (0, -x.numel() % 31)).view(-1, 31)
+        x = torch.cat([torch.full((len(x), 1), top, dtype=dtype), x], 1)[:, None].cuda()    # [n, 1, 32]
+        n = x.shape[0]
+        c = make([n], 1, 32, layers=1)
+        run = runs_of([(0, n, 0, 0)])
+        c.append(0, x, x.flip(2), run, n)
+        k, v = torch.empty_like(x), torch.empty_like(x)
+        c.read(0, k, v, run, n)
+        assert torch.equal(k.cpu(), torch.from_numpy(blocks(x.double().cpu().numpy())).to(dtype)), top
+        assert torch.equal(v.cpu(), torch.from_numpy(blocks(x.flip(2).double().cpu().numpy())).to(dtype)), top
 
 
 @pytest.mark.parametrize("dtype", TYPES)
