@@ -10,13 +10,116 @@ namespace cats {
 // A thread takes eight elements (a word of K codes) of the two tokens of a
 // pair (whose V codes share words): four neighbours hold a block of 32.
 // APPEND: rows -> blocks; else blocks -> rows.  Rows of k (side 0) and v (side
-// 1) of the runs: grid.x over a row's eights, grid.y over the pairs, grid.z
-// over the runs.  What a thread's column is, is settled once; then it goes
-// down the pairs.
+// 1) of the runs: grid.x over a row's eights, grid.y over eights of tokens,
+// grid.z over the runs.  What a thread's column is, is settled once, what its
+// page is once in eight tokens.
 //
 // Bound by HBM for long prompts: in 2 * hs * size, out 2 * hs * 4.5 bits a
-// token and head.
-template <int type, bool APPEND>
+// token and head, if the instructions let it: some twenty an element with a
+// page and 64-bit offsets for every pair.
+constexpr int KV_EIGHT = 8;   // tokens of a thread's turn
+
+// eight elements of a row, as they lie (TYPE 16 bits) or as floats
+template <int TYPE> struct Eight {
+    using T = std::conditional_t<TYPE == KV_F32, float, uint16_t>;
+    alignas(16) uint32_t w[TYPE == KV_F32 ? 8 : 4];
+};
+template <int TYPE> __device__ __forceinline__ Eight<TYPE> load_eight(const char *row)   // aligned to four elements
+{
+    Eight<TYPE> r;
+    using V = std::conditional_t<TYPE == KV_F32, uint4, uint2>;
+    reinterpret_cast<V *>(r.w)[0] = reinterpret_cast<const V *>(row)[0];
+    reinterpret_cast<V *>(r.w)[1] = reinterpret_cast<const V *>(row)[1];
+    return r;
+}
+template <int TYPE> __device__ __forceinline__ void store_eight(char *row, const Eight<TYPE> &r)
+{
+    using V = std::conditional_t<TYPE == KV_F32, uint4, uint2>;
+    reinterpret_cast<V *>(row)[0] = reinterpret_cast<const V *>(r.w)[0];
+    reinterpret_cast<V *>(row)[1] = reinterpret_cast<const V *>(r.w)[1];
+}
+template <int TYPE> __device__ __forceinline__ Eight<TYPE> load_eight(const KvRows &t, size_t at, bool in)
+{
+    Eight<TYPE> r;
+    constexpr int N = sizeof(r.w) / 4;
+#pragma unroll
+    for (int j = 0; j < N; j++) r.w[j] = 0u;
+    if (!in) return r;
+    if (t.vec) {
+        r = load_eight<TYPE>(static_cast<const char *>(t.p) + at * sizeof(typename Eight<TYPE>::T));
+    } else if constexpr (TYPE == KV_F32) {
+        const uint32_t *p = static_cast<const uint32_t *>(t.p) + at;
+#pragma unroll
+        for (int j = 0; j < 8; j++) r.w[j] = p[j];
+    } else {
+        const uint16_t *p = static_cast<const uint16_t *>(t.p) + at;
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.w[j] = p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
+    }
+    return r;
+}
+template <int TYPE> __device__ __forceinline__ void store_eight(const KvRows &t, size_t at, const Eight<TYPE> &r)
+{
+    if (t.vec) {
+        store_eight<TYPE>(static_cast<char *>(t.p) + at * sizeof(typename Eight<TYPE>::T), r);
+    } else if constexpr (TYPE == KV_F32) {
+        uint32_t *p = static_cast<uint32_t *>(t.p) + at;
+#pragma unroll
+        for (int j = 0; j < 8; j++) p[j] = r.w[j];
+    } else {
+        uint16_t *p = static_cast<uint16_t *>(t.p) + at;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            p[2 * j] = (uint16_t)r.w[j];
+            p[2 * j + 1] = (uint16_t)(r.w[j] >> 16);
+        }
+    }
+}
+template <int TYPE> __device__ __forceinline__ uint32_t quant_eight(const Eight<TYPE> &r, unsigned mask, uint16_t *scale)
+{
+    if constexpr (TYPE == KV_F32) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = __uint_as_float(r.w[j]);
+        return kv_quant8(x, mask, scale);
+    } else {
+        return kv_quant8_half<TYPE>(r.w, mask, scale);
+    }
+}
+template <int TYPE> __device__ __forceinline__ Eight<TYPE> dequant_eight(uint32_t codes, uint32_t scale, const KvMagic &magic)
+{
+    const __half2 d = __half2half2(__ushort_as_half((uint16_t)scale));
+    uint32_t h[4];   // elements j and j + 4
+    kv_dequant(codes, d, magic, h);
+    Eight<TYPE> r;
+    if constexpr (TYPE == KV_F16) {   // the values as they are
+        r.w[0] = __byte_perm(h[0], h[1], 0x5410);
+        r.w[1] = __byte_perm(h[2], h[3], 0x5410);
+        r.w[2] = __byte_perm(h[0], h[1], 0x7632);
+        r.w[3] = __byte_perm(h[2], h[3], 0x7632);
+    } else {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
+            x[j] = f.x;
+            x[j + 4] = f.y;
+        }
+        if constexpr (TYPE == KV_F32) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) r.w[j] = __float_as_uint(x[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                r.w[j] = *reinterpret_cast<const uint32_t *>(&b);
+            }
+        }
+    }
+    return r;
+}
+
+template <int TYPE, bool APPEND>
 __global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvView c, const __grid_constant__ KvRows k,
                                                     const __grid_constant__ KvRows v, const KvRun *__restrict__ runs,
                                                     int n_runs)
@@ -28,108 +131,106 @@ __global__ void __launch_bounds__(256, 4) k_kv_rows(const __grid_constant__ KvVi
         const bool is_v = col >= per_side;
         const int e1 = is_v ? col - per_side : col, head = e1 / per_head, e8 = e1 - head * per_head;
         const KvRows &t = is_v ? v : k;
+        const int word2 = is_v ? c.hs >> 3 : c.hs >> 1, scale2 = is_v ? 2 : c.hs >> 4;
+        const uint32_t mix0 = is_v ? 0x5410 : 0x3210, mix1 = is_v ? 0x7632 : 0x7654;
         for (int ri = blockIdx.z; ri < n_runs; ri += gridDim.z) {
             const KvRun run = runs[ri];
             const int2 span = kv_run_rows(run, k.rows, c.err);
             if (span.x >= span.y) continue;
             const long long end = (long long)run.pos + span.y;
-            for (long long pair = (((long long)run.pos + span.x) >> 1) + blockIdx.y; 2 * pair < end; pair += gridDim.y) {
-                // tokens 2 pair, 2 pair + 1: in the run?
-                const long long r0 = 2 * pair - run.pos;
-                const bool in[2] = {r0 >= span.x, r0 + 1 < span.y};
-                const size_t at = (size_t)(run.first + r0) * t.ld + (size_t)head * c.hs + 8 * e8;
-                const int slot = (int)(2 * pair & (KV_PAGE - 1));
-                float x[2][8];
-                uint32_t w[2][4];
-                if constexpr (APPEND) {   // (does not wait for the table)
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const size_t from = at + (u ? t.ld : 0);
-                        if constexpr (type == KV_F32) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) x[u][j] = 0.f;
-                            if (in[u]) kv_load_row<8>(t, type, from, x[u]);
-                        } else {
-                            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
-                            const uint16_t *p = static_cast<const uint16_t *>(t.p) + from;
-                            if (in[u] && t.vec) {
-                                const uint2 a = *reinterpret_cast<const uint2 *>(p), b = *reinterpret_cast<const uint2 *>(p + 4);
-                                w[u][0] = a.x; w[u][1] = a.y; w[u][2] = b.x; w[u][3] = b.y;
-                            } else if (in[u]) {
-#pragma unroll
-                                for (int j = 0; j < 4; j++) w[u][j] = p[2 * j] | (uint32_t)p[2 * j + 1] << 16;
-                            }
-                        }
-                    }
-                }
-                const int page = c.page(run.seq, pair < 0 ? -1 : (int)min(pair / (KV_PAGE / 2), (long long)INT_MAX));
+            for (long long turn = (((long long)run.pos + span.x) >> 3) + blockIdx.y; KV_EIGHT * turn < end; turn += gridDim.y) {
+                const int page = c.page(run.seq, turn < 0 ? -1 : (int)min(turn / (KV_PAGE / KV_EIGHT), (long long)INT_MAX));
+                if (APPEND && page < 0) continue;
                 uint8_t *ch = c.chunk(max(page, 0), head);
-                if constexpr (APPEND) {
-                    if (page < 0) continue;
-                    uint32_t codes[2];
-                    uint16_t scale[2];
+                const int slot0 = (int)(KV_EIGHT * turn & (KV_PAGE - 1)), r0 = (int)(KV_EIGHT * turn - run.pos);   // (within eight of the rows)
+                const size_t at0 = (size_t)((long long)run.first + r0) * t.ld + (size_t)head * c.hs + 8 * e8;
+                if (t.vec && r0 >= span.x && r0 + KV_EIGHT <= span.y) {
+                    // Whole turns of aligned rows.  A pair's two words and scales are `word2` and
+                    // `scale2` apart, pairs hs and hs / 8 bytes; V's words mix the two tokens.
+                    uint8_t *code = ch + kv_code_off(is_v, c.hs, slot0, 2 * e8), *scale = ch + kv_scale_off(is_v, c.hs, slot0, e8 >> 2);
+                    const char *row = static_cast<const char *>(t.p) + at0 * sizeof(typename Eight<TYPE>::T);
+                    const size_t step = t.ld * sizeof(typename Eight<TYPE>::T);
+#pragma unroll 1
+                    for (int j = 0; j < KV_EIGHT; j += 4, row += 4 * step, code += 2 * c.hs, scale += c.hs >> 2) {
+                        if constexpr (APPEND) {
+                            Eight<TYPE> x[4];
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        if constexpr (type == KV_F32) codes[u] = kv_quant8(x[u], mask, &scale[u]);
-                        else codes[u] = kv_quant8_half<type>(w[u], mask, &scale[u]);
-                    }
-                    if (is_v && in[0] && in[1]) {
-                        kv_store_pair8(ch, c.hs, slot, e8, codes[0], codes[1], scale[0], scale[1]);
-                        continue;
-                    }
+                            for (int u = 0; u < 4; u++) x[u] = load_eight<TYPE>(row + u * step);
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
-                        if (in[u]) kv_store_codes8(ch, is_v, c.hs, slot + u, e8, codes[u], scale[u]);
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        if (!in[u]) continue;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) x[u][j] = 0.f;
-                        if (page >= 0) {
-                            uint32_t h[4];
-                            kv_dequant(kv_codes8(ch, is_v, c.hs, slot + u, e8),
-                                       __half2half2(kv_scale8(ch, is_v, c.hs, slot + u, e8)), magic, h);
-                            if constexpr (type == KV_F16) {   // the values as they are
-                                w[u][0] = __byte_perm(h[0], h[1], 0x5410);
-                                w[u][1] = __byte_perm(h[2], h[3], 0x5410);
-                                w[u][2] = __byte_perm(h[0], h[1], 0x7632);
-                                w[u][3] = __byte_perm(h[2], h[3], 0x7632);
-                            } else {
-#pragma unroll
-                                for (int j = 0; j < 4; j++) {
-                                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[j]));
-                                    x[u][j] = f.x;
-                                    x[u][j + 4] = f.y;
-                                }
+                            for (int u = 0; u < 2; u++) {
+                                uint16_t s0, s1;
+                                const uint32_t c0 = quant_eight<TYPE>(x[2 * u], mask, &s0), c1 = quant_eight<TYPE>(x[2 * u + 1], mask, &s1);
+                                *reinterpret_cast<uint32_t *>(code + u * c.hs) = __byte_perm(c0, c1, mix0);
+                                *reinterpret_cast<uint32_t *>(code + u * c.hs + word2) = __byte_perm(c0, c1, mix1);
+                                if (e8 & 3) continue;
+                                *reinterpret_cast<uint16_t *>(scale + u * (c.hs >> 3)) = s0;
+                                *reinterpret_cast<uint16_t *>(scale + u * (c.hs >> 3) + scale2) = s1;
                             }
-                        } else if constexpr (type == KV_F16) {
-                            w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0u;
-                        }
-                        const size_t to = at + (u ? t.ld : 0);
-                        if constexpr (type == KV_F32) {
-                            kv_store_row4(t, type, to, make_float4(x[u][0], x[u][1], x[u][2], x[u][3]));
-                            kv_store_row4(t, type, to + 4, make_float4(x[u][4], x[u][5], x[u][6], x[u][7]));
                         } else {
-                            if constexpr (type == KV_BF16) {
+                            uint32_t w[4] = {0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u}, s[4] = {0u, 0u, 0u, 0u};
+                            if (page >= 0) {
 #pragma unroll
-                                for (int j = 0; j < 4; j++) {
-                                    const __nv_bfloat162 b = __floats2bfloat162_rn(x[u][2 * j], x[u][2 * j + 1]);
-                                    w[u][j] = *reinterpret_cast<const uint32_t *>(&b);
+                                for (int u = 0; u < 4; u++) {
+                                    w[u] = *reinterpret_cast<const uint32_t *>(code + (u >> 1) * c.hs + (u & 1 ? word2 : 0));
+                                    s[u] = *reinterpret_cast<const uint16_t *>(scale + (u >> 1) * (c.hs >> 3) + (u & 1 ? scale2 : 0));
                                 }
                             }
-                            uint16_t *p = static_cast<uint16_t *>(t.p) + to;
-                            if (t.vec) {
-                                *reinterpret_cast<uint2 *>(p) = make_uint2(w[u][0], w[u][1]);
-                                *reinterpret_cast<uint2 *>(p + 4) = make_uint2(w[u][2], w[u][3]);
+#pragma unroll
+                            for (int u = 0; u < 4; u++)
+                                store_eight<TYPE>(const_cast<char *>(row) + u * step,
+                                                  dequant_eight<TYPE>(__byte_perm(w[u & 2], w[u | 1], u & 1 ? mix1 : mix0), s[u], magic));
+                        }
+                    }
+                    continue;
+                }
+#pragma unroll 1
+                for (int j = 0; j < KV_EIGHT; j += 4) {   // two pairs' loads in flight
+                    bool in[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) in[u] = r0 + j + u >= span.x && r0 + j + u < span.y;
+                    const size_t at = at0 + j * t.ld;
+                    if constexpr (APPEND) {
+                        Eight<TYPE> x[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) x[u] = load_eight<TYPE>(t, at + u * t.ld, in[u]);
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            if (!in[u] && !in[u + 1]) continue;
+                            uint16_t s0, s1;
+                            const uint32_t c0 = quant_eight<TYPE>(x[u], mask, &s0), c1 = quant_eight<TYPE>(x[u + 1], mask, &s1);
+                            const int slot = slot0 + j + u;
+                            if (is_v && in[u] && in[u + 1]) {
+                                kv_store_pair8(ch, c.hs, slot, e8, c0, c1, s0, s1);
+                                continue;
+                            }
+                            if (in[u]) kv_store_codes8(ch, is_v, c.hs, slot, e8, c0, s0);
+                            if (in[u + 1]) kv_store_codes8(ch, is_v, c.hs, slot + 1, e8, c1, s1);
+                        }
+                    } else {
+                        // (a pair's codes lie together: both are read where one is wanted)
+                        uint32_t codes[4], scale[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u += 2) {
+                            codes[u] = codes[u + 1] = 0x88888888u;
+                            scale[u] = scale[u + 1] = 0u;
+                            if (page < 0 || !(in[u] || in[u + 1])) continue;
+                            const int slot = slot0 + j + u;
+                            if (is_v) {
+                                const uint2 w = kv_pair8(ch, c.hs, slot, e8, scale[u]);
+                                codes[u] = w.x;
+                                codes[u + 1] = w.y;
+                                scale[u + 1] = scale[u] >> 16;
                             } else {
 #pragma unroll
-                                for (int j = 0; j < 4; j++) {
-                                    p[2 * j] = (uint16_t)w[u][j];
-                                    p[2 * j + 1] = (uint16_t)(w[u][j] >> 16);
+                                for (int h = 0; h < 2; h++) {
+                                    codes[u + h] = kv_codes8(ch, false, c.hs, slot + h, e8);
+                                    scale[u + h] = __half_as_ushort(kv_scale8(ch, false, c.hs, slot + h, e8));
                                 }
                             }
                         }
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            if (in[u]) store_eight<TYPE>(t, at + u * t.ld, dequant_eight<TYPE>(codes[u], scale[u], magic));
                     }
                 }
             }
@@ -143,7 +244,7 @@ static cudaError_t launch_rows(const KvView &c, int type, const KvRows &k, const
 {
     const int cols = (int)std::min<long long>(((long long)c.n_kv * (c.hs / 4) + 255) / 256, 1024);
     // some eight CTAs an SM in all, each going down its rows
-    const int runs = std::min(b.n_runs, 32768), rows = std::max(b.max_rows, 1) / 2 + 1;   // pairs
+    const int runs = std::min(b.n_runs, 32768), rows = std::max(b.max_rows, 1) / KV_EIGHT + 1;
     const long long down = std::max<long long>(1, 148ll * 16 / std::max<long long>(1, (long long)cols * runs));
     const dim3 grid((unsigned)cols, (unsigned)std::min<long long>(rows, std::min<long long>(down, 65535)), (unsigned)runs);
     switch (type) {

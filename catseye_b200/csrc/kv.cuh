@@ -177,7 +177,6 @@ template <int TYPE> __device__ __forceinline__ uint32_t kv_quant8_half(const uin
     const __half dh = __float2half_rn(fminf(fmaxf(__bfloat162float(__float2bfloat16_rn(m * -0.125f)), -8160.f), 8160.f));
     const float d = __half2float(dh);
     *scale = bad ? 0x7fff : __half_as_ushort(dh);
-    if (bad || d == 0.f) return 0x88888888u;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
     inv *= 0.0625f;
@@ -189,7 +188,7 @@ template <int TYPE> __device__ __forceinline__ uint32_t kv_quant8_half(const uin
     }
     const uint32_t even = __byte_perm(__byte_perm(y[0], y[2], 0x0062), __byte_perm(y[4], y[6], 0x0062), 0x5410) & 0x0f0f0f0fu;
     const uint32_t odd = __byte_perm(__byte_perm(y[1], y[3], 0x0062), __byte_perm(y[5], y[7], 0x0062), 0x5410) & 0x0f0f0f0fu;
-    return even | odd << 4;
+    return bad || d == 0.f ? 0x88888888u : even | odd << 4;
 }
 
 // ... and where a row's eight e8 go (K: one word; V: half of two words)
@@ -223,6 +222,15 @@ __device__ __forceinline__ uint32_t kv_codes8(const uint8_t *chunk, bool is_v, i
 __device__ __forceinline__ __half kv_scale8(const uint8_t *chunk, bool is_v, int hs, int slot, int e8)
 {
     return *reinterpret_cast<const __half *>(chunk + kv_scale_off(is_v, hs, slot, e8 >> 2));
+}
+
+// V of the two tokens of a pair: their codes, and both scales
+__device__ __forceinline__ uint2 kv_pair8(const uint8_t *chunk, int hs, int slot, int e8, uint32_t &scales)
+{
+    const uint8_t *p = chunk + kv_code_off(true, hs, slot, 2 * e8);
+    const uint32_t a = *reinterpret_cast<const uint32_t *>(p), b = *reinterpret_cast<const uint32_t *>(p + (hs >> 3));
+    scales = *reinterpret_cast<const uint32_t *>(chunk + kv_scale_off(true, hs, slot, e8 >> 2));
+    return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 }
 
 // four elements 4*e4 .. of a stored row
