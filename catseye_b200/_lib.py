@@ -169,6 +169,8 @@ def load(path=None):
 
 def check(rc, what="catsgpu"):
     """Raise on a non-zero status (or a sticky error after a void call)."""
+    if rc == 0:
+        return 0
     lib = load()
     if rc is None:
         rc = lib.cats_gpu_last_error()

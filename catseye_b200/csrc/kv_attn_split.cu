@@ -2,29 +2,39 @@
 // single tokens of many sequences, short runs.
 //
 // What it must read is the cache: 144 bytes a token and kv head of size 128
-// (4.5 bits a value), so it is bound by HBM while the arithmetic keeps up.  All
-// query rows that share a kv head go through it together (rows of the tensor
-// cores' 16-row tiles: the `mul` query heads of a token, of several tokens for
-// a run), and the long axis is split: a warp takes whole pages, the warps of a
-// CTA and the CTAs of a cluster interleave theirs, and each keeps its own
-// running maximum, sum and weighted values (one pass over the data).  They are
-// joined once at the end, through shared memory in the CTA and through the
-// cluster's distributed shared memory across CTAs: no workspace in global
-// memory, no second launch, the same order every time.
+// (4.5 bits a value).  The long axis is split: a warp takes half pages (32
+// tokens), the warps of a CTA interleave theirs, and each keeps its own running
+// maximum, sum and weighted values (one pass over the data), joined once at the
+// end.
 //
-// A page's chunk of one kv head is contiguous, so lane 0 of a warp brings it
-// to shared memory with one bulk copy into the warp's own ring of two; the
-// warp waits only for its own copies, and no CTA barrier runs until the end.
-// From there a lane reads the codes it feeds to m16n8k16 directly (kv.cuh's
-// order is the fragments'), and dequantizes them exactly in fp16.
+// Products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16): tokens, then
+// the head's elements, are the 16 rows, the query rows that share a kv head
+// the 8 columns, two such tiles where there are more.  So one query fills an
+// eighth of an instruction, not a sixteenth, a dequantized fragment serves all
+// columns, and what a lane's codes are is settled by kv.cuh's order.  P becomes
+// the second product's operand by an 8 x 8 transpose in the warp.  fp32 rows: q
+// and p are two fp16 halves in neighbouring columns (22 bits, no second product).
 //
-// fp32 rows: q and p are split into two fp16 halves, which take rows 0-7 and
-// 8-15 of the same instruction (22 bits, no second product).  fp16 and bf16
-// rows use the 16 rows for 16 queries, or 8 when that is enough.
+// Two ways to share the work.  Few half pages: a cluster of up to 8 CTAs a
+// (row tile, kv head), joined through distributed shared memory, one launch.
+// Many: equal stretches of all units' half pages, one for each of the SMs' CTA
+// slots, whatever the lengths; a second small kernel joins the units that lie
+// in several.  That kernel and the scan over the runs cost some 14 us, so it
+// takes four half pages a warp: one sequence of 131072 tokens (64 heads, 8 kv
+// heads of 128) 120 us in clusters, 51 in stretches; 16 of 2048 tokens (32 kv
+// heads, fp32) 64 and 54.
+//
+// Each warp keeps three half pages in its own ring: two under way while one is
+// used, 16 bytes a lane and copy; no CTA barrier runs until the end.  (Bulk
+// copies issued by one lane cost that warp 90 cycles each.)
+//
+// Bound by the issue of the dequantization: some 1350 instructions a half page
+// pair (9216 bytes), 64% of what a copy reaches of HBM (4.2 TB/s) once it runs.
 #include "kv_attn.cuh"
 #include <algorithm>
 #include <climits>
 #include <cooperative_groups.h>
+#include <mutex>
 #include <type_traits>
 
 namespace cats {
@@ -103,7 +113,7 @@ __host__ __device__ constexpr int sp_part(int rows, int hs) { return rows * (hs 
 constexpr int SP_MAX_ENTRIES = 1024;   // row tiles whose lengths a streamed CTA scans
 
 __host__ __device__ constexpr int sp_rows(bool split, int nt) { return (split ? 4 : 8) * nt; }
-__host__ __device__ constexpr int sp_resident(int nt) { return nt == 1 ? 4 : 3; }   // CTAs an SM
+__host__ __device__ constexpr int sp_resident(int nt) { return nt == 1 ? 4 : 3; }   // CTAs an SM (registers: 128, 168)
 
 template <bool SPLIT, int NT, int HB, bool STREAM>
 __global__ void __launch_bounds__(SP_WARPS * 32, sp_resident(NT))
@@ -673,6 +683,8 @@ __global__ void __launch_bounds__(256, 4) k_kv_attn_join(const __grid_constant__
 static cudaMemPool_t work_pool()
 {
     static cudaMemPool_t pools[64] = {};
+    static std::mutex lock;
+    std::lock_guard<std::mutex> hold(lock);
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
     if (!pools[dev]) {
@@ -762,8 +774,8 @@ cudaError_t launch_kv_attn_split(const KvAttn &a0, int max_rows, int max_len, cu
     a.tiles = (int)std::min<long long>((q + rows - 1) / rows, 1 << 16);
     const long long units = (long long)a.n_runs * a.c.n_kv * a.tiles, halves = std::max(1, max_len / SP_TOK + (max_len % SP_TOK != 0));
     if (units > (1ll << 26)) return cudaErrorInvalidValue;
-    // Many pages: streamed, one CTA for each of the SMs' slots.  Else a cluster a
-    // unit, up to 8 CTAs while each warp has half a page.
+    // Many half pages: streamed, one CTA for each of the SMs' slots.  Else a cluster a
+    // unit, up to 8 CTAs while each warp has a half page.
     const bool stream = (long long)a.n_runs * a.tiles <= SP_MAX_ENTRIES && units * halves >= 4ll * slots * SP_WARPS;
     int C = 1;
     while (!stream && C < 8 && units * C < slots && C * 2 * SP_WARPS <= halves) C *= 2;

@@ -184,14 +184,18 @@ __global__ void __launch_bounds__(SC_THREADS, 4) k_logprobs(const __grid_constan
     auto bound_of = [&] {
         sh.top[warp][lane] = sort32(mx, lane);
         __syncthreads();
-        float m[SC_WARPS];
+        if (warp < 2) {   // two halves, then one: the others wait
+            float m[SC_WARPS / 2];
 #pragma unroll
-        for (int w = 0; w < SC_WARPS; w++) m[w] = sh.top[w][lane];
+            for (int w = 0; w < SC_WARPS / 2; w++) m[w] = sh.top[2 * w + warp][lane];
 #pragma unroll
-        for (int n = SC_WARPS / 2; n; n >>= 1)
+            for (int n = SC_WARPS / 4; n; n >>= 1)
 #pragma unroll
-            for (int w = 0; w < n; w++) m[w] = merge32(m[w], m[w + n], lane);
-        return __shfl_sync(0xffffffffu, m[0], k - 1);
+                for (int w = 0; w < n; w++) m[w] = merge32(m[w], m[w + n], lane);
+            sh.top[warp][lane] = m[0];   // (the lists read are this warp's alone)
+        }
+        __syncthreads();
+        return __shfl_sync(0xffffffffu, merge32(sh.top[0][lane], sh.top[1][lane], lane), k - 1);
     };
     auto gather = [&](float bound) {
         if (mx >= bound) {
@@ -248,7 +252,8 @@ __global__ void __launch_bounds__(SC_THREADS, 4) k_logprobs(const __grid_constan
         if (k > 0) {
             if (chunk == 0) bound = bound_of();
             gather(bound);
-            if (chunk > 0 && (chunk & (chunk + 1)) == 0 && c0 + step < span) {
+            // after 4, 16, 64 .. chunks
+            if ((chunk & (chunk + 1)) == 0 && ((chunk + 1) & 0x55555554) && c0 + step < span) {
                 __syncthreads();
                 const int got = sh.count;
                 over |= got > SC_LIST + k;

@@ -40,16 +40,18 @@ def _type(t):
 
 def _rows(t, heads, hs, device, what):
     """Row stride of a tensor [rows][heads][hs] whose rows are whole."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hs:
-        raise ValueError(f"{what}: shape [rows, {heads}, {hs}] is wanted, not {list(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hs:
+        raise ValueError(f"{what}: shape [rows, {heads}, {hs}] is wanted, not {list(shape)}")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the cache on {device}")
     s0, s1, s2 = t.stride()
     if (s2 != 1 and hs > 1) or (s1 != hs and heads > 1):
         raise ValueError(f"{what}: the values of a row must be contiguous")
-    if t.shape[0] <= 1:
-        return heads * hs
-    if s0 < heads * hs:
+    width = heads * hs
+    if shape[0] <= 1:
+        return width
+    if s0 < width:
         raise ValueError(f"{what}: rows overlap")
     return s0
 
@@ -68,7 +70,7 @@ class Cache:
         if not pool.is_cuda or table.device != pool.device:
             raise ValueError("pool and table must be on the same CUDA device")
         self._lib = _lib.check_device(pool.device)
-        self.pool, self.table = pool, table
+        self.pool, self.table, self._dev, self._i32 = pool, table, pool.device, torch.int32
         self.n_pages, self.n_layers, self.n_kv_heads = pool.shape[:3]
         self.head_size = pool.shape[3] // 72
         self._c = _lib.KvC(pool.data_ptr(), table.data_ptr(), *pool.shape[:3], self.head_size, *table.shape)
@@ -83,14 +85,15 @@ class Cache:
                    torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device))
 
     def _batch(self, runs):
-        if runs.dim() != 2 or runs.shape[1] != 4 or not runs.is_contiguous() or str(runs.dtype) != "torch.int32":
+        shape = runs.shape
+        if len(shape) != 2 or shape[1] != 4 or not runs.is_contiguous() or runs.dtype != self._i32:
             raise ValueError("runs: a contiguous int32 tensor [n, 4] is wanted")
-        if runs.device != self.pool.device:
-            raise ValueError(f"runs are on {runs.device}, the cache on {self.pool.device}")
-        return runs.data_ptr(), runs.shape[0]
+        if runs.device != self._dev:
+            raise ValueError(f"runs are on {runs.device}, the cache on {self._dev}")
+        return runs.data_ptr(), shape[0]
 
     def _kv(self, fn, layer, k, v, runs, max_rows, stream):
-        dev = self.pool.device
+        dev = self._dev
         ld_k = _rows(k, self.n_kv_heads, self.head_size, dev, "k")
         ld_v = _rows(v, self.n_kv_heads, self.head_size, dev, "v")
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
@@ -114,7 +117,7 @@ class Cache:
         heads = q.shape[1] if q.dim() == 3 else 0
         if heads == 0 or heads % self.n_kv_heads:
             raise ValueError(f"q: [rows, heads, head_size] with heads a multiple of {self.n_kv_heads} is wanted")
-        dev = self.pool.device
+        dev = self._dev
         ld_q = _rows(q, heads, self.head_size, dev, "q")
         ld_o = _rows(out, heads, self.head_size, dev, "out")
         if q.dtype != out.dtype or q.shape[0] != out.shape[0]:

@@ -66,7 +66,7 @@ class GpuLLM:
             _lib.check(None, "cats_gpu_llm_create")
             raise _lib.CatsGpuError("cats_gpu_llm_create failed")
         self._logits = np.zeros(cfg.vocab, dtype=np.float32)
-        self._view, self._view_ptr = None, None
+        self._view, self._view_ptr, self._tp_size = None, None, tp_size
 
     @classmethod
     def load(cls, path, tp_rank=0, tp_size=1, seq_len=0):
@@ -84,7 +84,7 @@ class GpuLLM:
             _lib.check(None, "cats_gpu_llm_load")
             raise _lib.CatsGpuError("cats_gpu_llm_load failed")
         self._logits = np.zeros(self.cfg.vocab, dtype=np.float32)
-        self._view, self._view_ptr = None, None
+        self._view, self._view_ptr, self._tp_size = None, None, tp_size
         return self
 
     def set_weights(self, mw):
@@ -199,9 +199,10 @@ class GpuLLM:
         _lib.check(self.lib.cats_gpu_llm_cache_compact(self.h, C.byref(moved)), "cache_compact")
         return moved.value
 
-    def cache_read(self, layer, seq, n, kv_dim=None):
-        """K and V [n, kv_dim] that the cache holds for a sequence's first n tokens."""
-        k, v = (np.zeros((n, kv_dim or self.cfg.kv_dim), np.float32) for _ in range(2))
+    def cache_read(self, layer, seq, n):
+        """K and V [n, kv_dim] that the cache holds for a sequence's first n
+        tokens (a tensor-parallel rank: of its kv heads)."""
+        k, v = (np.zeros((n, self.cfg.kv_dim // self._tp_size), np.float32) for _ in range(2))
         _lib.check(self.lib.cats_gpu_llm_cache_read(self.h, layer, seq, n, C.c_void_p(k.ctypes.data),
                                                     C.c_void_p(v.ctypes.data)), "cache_read")
         return k, v

@@ -33,5 +33,5 @@ def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
         logits.data_ptr(), _type(logits), rows, vocab, ld, targets.data_ptr() if targets is not None else None, k,
         p if targets is not None else None, p + 4 * rows if entropy else None, ids.data_ptr() if k else None,
         p + 8 * rows if k else None, stream), "logprobs")
-    return (f[:rows] if targets is not None else None, f[rows:2 * rows] if entropy else None, ids,
-            f[2 * rows:].view(rows, k))
+    lp, h, top = f.split((rows, rows, rows * k))
+    return lp if targets is not None else None, h if entropy else None, ids, top.view(rows, k)

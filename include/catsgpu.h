@@ -392,7 +392,8 @@ int cats_gpu_kv_read_dev(const cats_gpu_kv *c, int layer, void *k, void *v, int 
  * a kv head (llm/catseye_llm.h:1677-1723).  A row at a negative position sees
  * nothing and gets zeros.  Sums and softmax statistics are fp32; fp32 rows
  * enter the tensor cores as two fp16 halves each of q and of the
- * probabilities, other types as one. */
+ * probabilities, other types as one.  out and q share no memory (the same
+ * pointer: CATS_ERR_ARG). */
 int cats_gpu_kv_attention_dev(const cats_gpu_kv *c, int layer, void *out, const void *q, int type, int n_heads,
                               long long ld_out, long long ld_q, int rows, const int *runs, int n_runs, int max_rows,
                               int max_len, void *stream);
