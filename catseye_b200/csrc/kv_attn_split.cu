@@ -694,8 +694,13 @@ static cudaMemPool_t work_pool()
         pr.location.id = dev;
         uint64_t keep = UINT64_MAX;
         cudaMemPool_t p = nullptr;
-        if (cudaMemPoolCreate(&p, &pr) != cudaSuccess ||
-            cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep) != cudaSuccess) {
+        // (the first call of all may be a captured one: this is not part of it)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        const bool made = cudaMemPoolCreate(&p, &pr) == cudaSuccess &&
+                          cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep) == cudaSuccess;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!made) {
             cudaGetLastError();
             return nullptr;
         }

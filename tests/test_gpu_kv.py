@@ -14,7 +14,10 @@ once to fp16 (2^-11 max |v|, twice as the normaliser is not rounded alike),
 bf16 query rows lie exactly in fp16's range after scaling, and the output is
 rounded by half a step."""
 import math
+import os
 import random
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -454,6 +457,34 @@ def test_captured_replayed_and_on_two_streams(rows, hint):
         torch.cuda.synchronize()
         for j in range(2):
             assert torch.equal(outs[j], alone[i + j])
+
+
+FIRST = """
+import torch
+from catseye_b200 import kv
+c = kv.Cache.empty(40, 1, 2, 64, 1, 40)
+c.table.copy_(torch.arange(40, dtype=torch.int32)[None])
+x = torch.randn(2000, 2, 64, device="cuda")
+c.append(0, x, x, torch.tensor([[0, 2000, 0, 0]], dtype=torch.int32, device="cuda"), 2000)
+q, out, want = (torch.randn(1, 8, 64, device="cuda") for _ in range(3))
+run = torch.tensor([[0, 1, 0, 1999]], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=torch.cuda.Stream(), capture_error_mode="thread_local"):
+    c.attention(0, out, q, run, 1, 1_000_000, stream=torch.cuda.current_stream().cuda_stream)
+g.replay()
+torch.cuda.synchronize()
+c.attention(0, want, q, run, 1, 1_000_000)
+torch.cuda.synchronize()
+assert torch.equal(out, want)
+"""
+
+
+def test_the_first_call_of_a_process_is_captured():
+    """Nothing the library makes once (attributes, memory pool) asks for an eager call first."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("dtype", TYPES)

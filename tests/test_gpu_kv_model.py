@@ -211,6 +211,23 @@ def test_generation_from_forks(llm, orc):
     m.close()
 
 
+def test_generation_planned_for_a_long_context(llm, orc):
+    """A context long enough for the attention's other division of the work,
+    captured; the first tokens of all are generated ones."""
+    cfg = config(llm, 32, seq_len=32768)
+    _, m = model(llm, orc, cfg, 16, 8)
+    start = np.array([7, 7, 9, 9, 11, 13, 15, 7], np.int32)
+    out = m.generate_batch(start, [0] * 8, 70)
+    assert np.array_equal(out[:, 0], out[:, 1]) and np.array_equal(out[:, 0], out[:, 7]) and np.array_equal(out[:, 2], out[:, 3])
+    for s in (0, 2, 6):
+        fed = np.concatenate([[start[s]], out[:-1, s]])
+        m.cache_truncate(s)
+        _, lg = m.forward_batch(fed, np.arange(70), np.full(70, s), logits=True)
+        for i in range(70):
+            assert lg[i, out[i, s]] >= lg[i].max() - 2 * tol(cfg) * np.linalg.norm(lg[i])
+    m.close()
+
+
 def test_scores_and_dense_hand_over(llm, orc):
     """score_batch against the float64 softmax of the step's logits; the
     sequence copied into the single-token engine's cache goes on there."""
