@@ -14,9 +14,11 @@ namespace cats {
 // grid.z over the runs.  What a thread's column is, is settled once, what its
 // page is once in eight tokens.
 //
-// Bound by HBM for long prompts: in 2 * hs * size, out 2 * hs * 4.5 bits a
-// token and head, if the instructions let it: some twenty an element with a
-// page and 64-bit offsets for every pair.
+// To read and write: 2 * hs * size and 2 * hs * 4.5 bits a token and head.  Bound
+// by issue: 15 instructions an element appended, 9 read back (36 and 20 with a
+// page and 64-bit offsets for every pair, and 16-bit values quantized in fp32).
+// 4096 bf16 rows of 32 heads of 128: appended in 24 us, read back in 18 (86 MB
+// each: 3.6 and 4.7 TB/s); 16 rows of 8 heads 5 us, which is the launch.
 constexpr int KV_EIGHT = 8;   // tokens of a thread's turn
 
 // eight elements of a row, as they lie (TYPE 16 bits) or as floats
@@ -301,7 +303,8 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
         return launch_kv_attn_split(a, b.max_rows, b.max_len, st);
     // Where most runs are short (decode steps beside a prompt) they keep to the
     // split kernel: below 32 query rows a run costs less there even on a full GPU.
-    if (2 * rows < (long long)b.n_runs * b.max_rows) {
+    // (An extra launch costs 5 us: not for batches whose runs average a quarter of the longest.)
+    if (4 * rows < (long long)b.n_runs * b.max_rows) {
         a.q_hi = a.q_lo = 32;
         const cudaError_t e = launch_kv_attn_split(a, (a.q_hi + a.mul - 1) / a.mul, b.max_len, st);
         if (e) return e;
@@ -311,6 +314,7 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
 }
 
 // ------------------------------------------------------------- page copies
+// Bound by HBM: 96 pages of 5.9 MB 180 us, 6.3 TB/s, 96% of a plain copy's rate.
 // The lists travel as the kernel's parameters: no copy of them to the device
 // and nothing to keep alive after the call, captured or not.
 constexpr int KV_COPY_MOVES = 480;
