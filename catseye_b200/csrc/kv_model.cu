@@ -49,13 +49,16 @@ int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs)
     if (n_pages < 0 || n_seqs <= 0) return E_ARG;
     if (!batch_supported(m) || m->head_size % 32 || m->head_size > KV_MAX_HS) return E_UNSUPPORTED;
     const int max_pages = (m->c.seq_len + KV_PAGE - 1) / KV_PAGE;
+    const size_t page_bytes = (size_t)m->c.n_layers * m->kv_heads_loc * 72 * m->head_size;
+    size_t free_mem = 0, all = 0;   // (before the host's lists of so many pages are made)
+    if (cudaMemGetInfo(&free_mem, &all) != cudaSuccess || all / page_bytes < (size_t)n_pages) return E_NOMEM;
     LlmPaged *p = nullptr;
     try {
         p = new LlmPaged(n_pages, n_seqs, max_pages);
     } catch (const std::bad_alloc &) {
         return E_NOMEM;
     }
-    p->page_bytes = (size_t)m->c.n_layers * m->kv_heads_loc * 72 * m->head_size;
+    p->page_bytes = page_bytes;
     const size_t tb = (size_t)n_seqs * max_pages * 4;
     bool ok = cudaMalloc(&p->pool, p->page_bytes * n_pages) == cudaSuccess;
     ok = ok && cudaMalloc(&p->table, tb) == cudaSuccess && cudaMallocHost(&p->table_host, tb) == cudaSuccess;

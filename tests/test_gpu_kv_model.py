@@ -228,6 +228,72 @@ def test_generation_planned_for_a_long_context(llm, orc):
     m.close()
 
 
+def test_any_order_and_larger_batches(llm, orc):
+    """Tokens of two sequences by turns, backwards, and a batch enlarged later:
+    the logits of the grouped batch."""
+    cfg = config(llm, 32)
+    mw, m = model(llm, orc, cfg, 16, 4, cap=40)
+    f = Forward(orc, mw)
+    toks = [prompt(11, 100, cfg.vocab), prompt(12, 100, cfg.vocab)]
+    pos = np.repeat(np.arange(20), 2)
+    seqs = np.tile([0, 1], 20)
+    order = np.concatenate([np.arange(0, 40, 3), np.arange(1, 40, 3)[::-1], np.arange(2, 40, 3)])
+    mixed = np.array([toks[s][p] for s, p in zip(seqs, pos)])
+    _, lg = m.forward_batch(mixed[order], pos[order], seqs[order], logits=True)
+    m.batch_reserve(128, 1)
+    assert m.cache_length(0) == 20
+    _, more = m.forward_batch(np.concatenate([toks[0][20:], toks[1][20:44]]), np.concatenate([np.arange(20, 100), np.arange(20, 44)]),
+                              np.repeat([0, 1], [80, 24]), logits=True)
+    for s, n in ((0, 100), (1, 44)):
+        held = [m.cache_read(l, s, n) for l in range(2)]
+        want, made = f(toks[s][:n], lambda l: held[l])
+        check_cache(made, held)
+        got = {int(p): lg[i] for i, (p, q) in enumerate(zip(pos[order], seqs[order])) if q == s}
+        got.update({20 + i: row for i, row in enumerate(more[:80] if s == 0 else more[80:])})
+        assert max(rel(got[p], want[p]) for p in range(n)) < tol(cfg)
+    m.close()
+
+
+def test_enqueued_batches(llm, orc):
+    """batch_set and its asynchronous steps: positions are made writable ahead
+    of them, a batch is void once another call may have moved its pages, and
+    steps past the context or the pool are refused."""
+    cfg = config(llm, 32)
+    _, m = model(llm, orc, cfg, 6, 3)
+    start = np.array([5, 6], np.int32)
+    want = m.generate_batch(start, [0, 0], 100)
+    for s in (0, 1):
+        m.cache_truncate(s)
+    m.batch_set(start, [0, 0], [0, 1])
+    m.batch_enqueue_decode(60)
+    m.batch_enqueue_decode(40)
+    m.batch_enqueue()                                 # the step at position 100, once more without moving on
+    m.synchronize()
+    assert [m.cache_length(s) for s in range(3)] == [101, 101, 0]
+    _, a = m.forward_batch(want[-1], [100, 100], [0, 1], logits=True)
+    m.cache_truncate(0, 100)
+    m.cache_truncate(1, 100)
+    _, b = m.forward_batch(want[-1], [100, 100], [0, 1], logits=True)
+    assert np.array_equal(a, b)
+    m.batch_set(want[-1], [100, 100], [0, 1])
+    m.cache_fork(0, 2, 70)
+    for call in (m.batch_enqueue, lambda: m.batch_enqueue_decode(1)):
+        with pytest.raises(RuntimeError):
+            call()
+    kept = m.cache_read(0, 2, 70)
+    m.batch_set(want[-1], [100, 100], [0, 1])
+    with pytest.raises(RuntimeError):
+        m.batch_enqueue_decode(300)
+    m.batch_set(want[:5, 0], np.arange(101, 106), np.zeros(5, int))
+    with pytest.raises(RuntimeError):                 # not one token a sequence
+        m.batch_enqueue_decode(1)
+    assert all(np.array_equal(x, y) for x, y in zip(kept, m.cache_read(0, 2, 70)))
+    with pytest.raises(RuntimeError):
+        m.cache_q4(2**31 - 1, 2)
+    assert m.cache_length(2) == 70                    # refused: the cache as it was
+    m.close()
+
+
 def test_scores_and_dense_hand_over(llm, orc):
     """score_batch against the float64 softmax of the step's logits; the
     sequence copied into the single-token engine's cache goes on there."""
