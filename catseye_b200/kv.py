@@ -9,6 +9,7 @@ position of the first row.  stream: a cudaStream_t, or None for the library's
 own, which is ordered with the legacy default stream.
 """
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -36,6 +37,17 @@ def _type(t):
     if got is None:
         raise TypeError(f"float32, float16 or bfloat16 is wanted, not {t.dtype}")
     return got
+
+
+def _ints(x):
+    """(address, length, owner) of host integers as C ints."""
+    if isinstance(x, (list, tuple)):   # a third of the time through numpy
+        a = array("i", x)
+        return a.buffer_info()[0], len(a), a
+    a = np.ascontiguousarray(x, np.int32)
+    if a.ndim != 1:
+        raise ValueError("a list of integers is wanted")
+    return a.ctypes.data, a.size, a
 
 
 def _rows(t, heads, hs, device, what):
@@ -130,11 +142,10 @@ class Cache:
     def copy_pages(self, src, dst, stream=None):
         """Pages dst[i] = pages src[i] (host integers); no page may be written
         twice, nor both read and written."""
-        src, dst = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
-        if src.shape != dst.shape or src.ndim != 1:
+        (src, n, _a), (dst, m, _b) = _ints(src), _ints(dst)
+        if n != m:
             raise ValueError("src and dst must be lists of the same length")
-        _lib.check(self._lib.cats_gpu_kv_copy_pages_dev(self._p, src.ctypes.data, dst.ctypes.data, src.size, stream),
-                   "copy_pages")
+        _lib.check(self._lib.cats_gpu_kv_copy_pages_dev(self._p, src, dst, n, stream), "copy_pages")
 
 
 class Pages:

@@ -25,13 +25,14 @@ def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
         raise ValueError("targets: a contiguous int32 tensor [rows] on the logits' device is wanted")
     if not 0 <= k <= MAX_K:
         raise ValueError(f"k: 0 to {MAX_K} is wanted, not {k}")
-    # one buffer: logprob, entropy, top log probabilities; the ids beside it
-    f = torch.empty(rows * (2 + k), dtype=torch.float32, device=dev)
+    # (four tensors are made in less time than one is cut in three)
+    f32 = torch.float32
+    lp = torch.empty(rows, dtype=f32, device=dev) if targets is not None else None
+    h = torch.empty(rows, dtype=f32, device=dev) if entropy else None
     ids = torch.empty(rows, k, dtype=torch.int32, device=dev)
-    p = f.data_ptr()
+    top = torch.empty(rows, k, dtype=f32, device=dev)
     _lib.check(lib.cats_gpu_logprobs_dev(
         logits.data_ptr(), _type(logits), rows, vocab, ld, targets.data_ptr() if targets is not None else None, k,
-        p if targets is not None else None, p + 4 * rows if entropy else None, ids.data_ptr() if k else None,
-        p + 8 * rows if k else None, stream), "logprobs")
-    lp, h, top = f.split((rows, rows, rows * k))
-    return lp if targets is not None else None, h if entropy else None, ids, top.view(rows, k)
+        lp.data_ptr() if lp is not None else None, h.data_ptr() if entropy else None, ids.data_ptr() if k else None,
+        top.data_ptr() if k else None, stream), "logprobs")
+    return lp, h, ids, top
