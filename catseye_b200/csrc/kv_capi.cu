@@ -86,7 +86,7 @@ int rows_call(const cats_gpu_kv *c, int layer, void *k, void *v, int type, long 
     KvView view;
     KvRows rk, rv;
     if (rows == 0 || n_runs == 0) return CATS_OK;
-    if (!tabled(c) || !view_of(c, layer, &view) || !runs || n_runs < 0 || max_rows < 0 ||
+    if (!tabled(c) || !view_of(c, layer, &view) || !runs || n_runs < 0 || max_rows < 0 || (!append && k == v) ||
         !rows_ok(k, type, ld_k, rows, (long long)c->n_kv_heads * c->head_size, &rk) ||
         !rows_ok(v, type, ld_v, rows, (long long)c->n_kv_heads * c->head_size, &rv))
         return capi_fail(CATS_ERR_ARG, what);

@@ -383,7 +383,7 @@ size_t cats_gpu_kv_page_bytes(int n_layers, int n_kv_heads, int head_size);   /*
 /* k, v: [rows][n_kv_heads * head_size], quantized into the pages of `layer`. */
 int cats_gpu_kv_append_dev(const cats_gpu_kv *c, int layer, const void *k, const void *v, int type, long long ld_k,
                            long long ld_v, int rows, const int *runs, int n_runs, int max_rows, void *stream);
-/* The inverse: the values the cache holds, rounded to `type`. */
+/* The inverse: the values the cache holds, rounded to `type` (k and v apart). */
 int cats_gpu_kv_read_dev(const cats_gpu_kv *c, int layer, void *k, void *v, int type, long long ld_k, long long ld_v,
                          int rows, const int *runs, int n_runs, int max_rows, void *stream);
 /* Causal attention of the rows q [rows][n_heads * head_size] over the cache:

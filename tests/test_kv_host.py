@@ -143,7 +143,7 @@ def _call(name, cache, *args):
 
 
 ROWS = dict(layer=0, k=A, v=A, type=0, ld_k=128, ld_v=128, rows=3, runs=A, n_runs=1, max_rows=3, stream=None)
-ATT = dict(layer=0, out=A, q=A, type=0, n_heads=4, ld_out=256, ld_q=256, rows=3, runs=A, n_runs=1, max_rows=3,
+ATT = dict(layer=0, out=A, q=2 * A, type=0, n_heads=4, ld_out=256, ld_q=256, rows=3, runs=A, n_runs=1, max_rows=3,
            max_len=5, stream=None)
 BAD_CACHE = [dict(pool=0), dict(pool=A + 8), dict(table=0), dict(n_pages=0), dict(n_layers=0), dict(n_kv_heads=0),
              dict(head_size=48), dict(head_size=0), dict(head_size=-32), dict(n_seqs=0), dict(max_pages=0),
@@ -172,6 +172,14 @@ def test_bad_rows_are_refused(change):
                                     dict(runs=0), dict(n_runs=-1), dict(max_rows=-1), dict(max_len=-1)])
 def test_bad_attention_is_refused(change):
     assert _call("cats_gpu_kv_attention_dev", _lib.KvC(**GOOD), *{**ATT, **change}.values()) == 2
+
+
+def test_attention_over_its_own_queries_is_refused():
+    assert _call("cats_gpu_kv_attention_dev", _lib.KvC(**GOOD), *{**ATT, "q": ATT["out"]}.values()) == 2
+
+
+def test_rows_read_into_one_tensor_are_refused():
+    assert _call("cats_gpu_kv_read_dev", _lib.KvC(**GOOD), *ROWS.values()) == 2
 
 
 def test_large_heads_are_unsupported_and_nothing_is_nothing():
