@@ -183,9 +183,11 @@ __global__ void k_rope_kv(PartSrc y, int T, const BatchTok *__restrict__ bt, flo
     }
 }
 
-// The same for the paged Q4_0 cache: q as fp16 (the attention's operand), k
-// and v quantized into their pages.  Eight elements (four pairs) a thread, so
-// four neighbours hold a block of 32.
+// The same for the paged Q4_0 cache: q as fp16, k and v quantized into their
+// pages.  Eight elements (four pairs) a thread, so four neighbours hold a block
+// of 32.  (q's rounding is the one its product's operands had, and halves the
+// attention's rows; the attention's own fp16 output is what the next product
+// would round to.)
 __global__ void __launch_bounds__(256) k_rope_kv_paged(PartSrc y, int T, const BatchTok *__restrict__ bt,
                                                        __half *__restrict__ q, const __grid_constant__ KvView c,
                                                        int q_dim, int kv_dim, int seq_len)
