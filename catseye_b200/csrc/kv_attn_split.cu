@@ -79,7 +79,8 @@ __device__ __forceinline__ void finish4(const KvAttn &a, const KvRun &run, const
     acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     const int tok = span.x + (int)(rr / a.mul), h = kvh * a.mul + (int)(rr % a.mul), row = run.first + tok;
     const float sum = acc.x + acc.y + acc.z + acc.w;
-    if (sum != sum && l == l) acc = kv_plain_row4(a, run.seq, row, h, run.pos + tok, e4);
+    // (a row past the table sees nothing, whatever the others of its tile bring in)
+    if (sum != sum && l == l) acc = kv_plain_row4(a, run.seq, row, h, kv_limit(a.c, run, tok), e4);
     kv_store_row4(a.out, a.type, (size_t)row * a.out.ld + (size_t)h * a.c.hs + 4 * e4, acc);
 }
 
