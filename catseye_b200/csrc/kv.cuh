@@ -233,15 +233,6 @@ __device__ __forceinline__ uint2 kv_pair8(const uint8_t *chunk, int hs, int slot
     return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
 }
 
-// four elements 4*e4 .. of a stored row
-__device__ __forceinline__ float4 kv_load4(const uint8_t *chunk, bool is_v, int hs, int slot, int e4)
-{
-    const unsigned c = *reinterpret_cast<const uint16_t *>(chunk + kv_code_off(is_v, hs, slot, e4));
-    const float d = __half2float(*reinterpret_cast<const __half *>(chunk + kv_scale_off(is_v, hs, slot, e4 >> 3)));
-    return make_float4(d * (float)((int)(c & 15) - 8), d * (float)((int)(c >> 4 & 15) - 8),
-                       d * (float)((int)(c >> 8 & 15) - 8), d * (float)((int)(c >> 12 & 15) - 8));
-}
-
 // Rows of attention or of a cache's tensors: `rows` of them, ld elements apart.
 struct KvRows {
     void *p;

@@ -1,6 +1,6 @@
 // kv_attn.cuh — what the attention kernels over the paged Q4_0 cache share:
 // fragments of cached codes as fp16, the tensor-core instruction, rows of
-// queries, and the plain loop for rows that a NaN in the cache touched.
+// queries, and what keeps a NaN in the cache to the rows that see it.
 #pragma once
 #include "kv.cuh"
 
@@ -195,43 +195,18 @@ __device__ __forceinline__ int kv_limit(const KvView &c, const KvRun &run, int r
     return at < 0 ? -1 : (int)at;
 }
 
-// Elements 4*e4 .. of one row by the plain loop.  The tensor cores multiply a
-// masked position's zero probability with its value too, so a NaN in the cache
-// reaches the rows of its tile that do not see it: those come here (`row` of
-// a, head h, positions 0 .. lim).  What does see a NaN is NaN.
-static __device__ __noinline__ float4 kv_plain_row4(const KvAttn &a, int seq, int row, int h, int lim, int e4)
+// The products multiply a masked position's zero probability with its value
+// too, so a NaN in V would reach the rows of its tile that do not see it.
+// Where some row's mask cuts a tile of tokens, scales that are not finite are
+// taken out before the product, and the first position of each block that holds
+// one is kept (nan_at, shared memory): rows that see it are NaN in that block.
+// `scales` are those of token `at` and the next.
+__device__ __forceinline__ uint32_t kv_finite_scales(uint32_t scales, int at, int *nan_at)
 {
-    const KvView &c = a.c;
-    const int g = h / a.mul, hs = c.hs;
-    const int *table = c.table + (size_t)seq * c.max_pages;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int t = 0; t <= lim; t++) {
-        const int page = table[t / KV_PAGE];
-        if (page < 0 || page >= c.n_pages) continue;
-        const __half d = *reinterpret_cast<const __half *>(c.chunk(page, g) + kv_scale_off(true, hs, t % KV_PAGE, e4 >> 3));
-        if (__hisnan(d)) return make_float4(NAN, NAN, NAN, NAN);
-    }
-    float m = -INFINITY, l = 0.f;
-    for (int t = 0; t <= lim; t++) {
-        const int page = table[t / KV_PAGE];
-        if (page < 0 || page >= c.n_pages) continue;
-        const uint8_t *ch = c.chunk(page, g);
-        float s = 0.f;
-        for (int e = 0; e < hs / 4; e++) {
-            float x[4];
-            kv_load_row<4>(a.q, a.type, (size_t)row * a.q.ld + (size_t)h * hs + 4 * e, x);
-            const float4 k = kv_load4(ch, false, hs, t % KV_PAGE, e);
-            s += x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w;
-        }
-        s *= a.scale_log2;
-        const float mn = fmaxf(m, s), al = m == -INFINITY ? 0.f : exp2f(m - mn), p = exp2f(s - mn);
-        const float4 v = kv_load4(ch, true, hs, t % KV_PAGE, e4);
-        l = l * al + p;
-        o = make_float4(o.x * al + p * v.x, o.y * al + p * v.y, o.z * al + p * v.z, o.w * al + p * v.w);
-        m = mn;
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const uint32_t fine = __hlt2_mask(__habs2(*reinterpret_cast<const __half2 *>(&scales)),
+                                      __half2half2(__ushort_as_half(0x7c00)));
+    if (fine != 0xffffffffu) atomicMin(nan_at, at + ((fine & 0xffffu) != 0));
+    return scales & fine;
 }
 
 int kv_attn_tile_rows(const KvAttn &a);   // query rows that a CTA of the tile kernel takes

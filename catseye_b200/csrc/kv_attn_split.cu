@@ -78,9 +78,6 @@ __device__ __forceinline__ void finish4(const KvAttn &a, const KvRun &run, const
     const float inv = l == 0.f ? 0.f : 1.f / l;
     acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     const int tok = span.x + (int)(rr / a.mul), h = kvh * a.mul + (int)(rr % a.mul), row = run.first + tok;
-    const float sum = acc.x + acc.y + acc.z + acc.w;
-    // (a row past the table sees nothing, whatever the others of its tile bring in)
-    if (sum != sum && l == l) acc = kv_plain_row4(a, run.seq, row, h, kv_limit(a.c, run, tok), e4);
     kv_store_row4(a.out, a.type, (size_t)row * a.out.ld + (size_t)h * a.c.hs + 4 * e4, acc);
 }
 
@@ -124,6 +121,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
     constexpr int ROWS = sp_rows(SPLIT, NT);
     constexpr int NS = SPLIT ? NT : 2 * NT;   // query rows whose scores a lane holds
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int nan_at[WARPS][HB];   // a warp's first position with a NaN in V, by block
     // at the end a warp's rows take its ring, then the CTA's joined rows that of warp 0
     static_assert(ROWS * (HS + 2) * 4 <= SP_STAGES * STAGE, "");
     float *joined = reinterpret_cast<float *>(smem);   // [ROWS][HS], m[ROWS], l[ROWS]
@@ -276,6 +274,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
         // the 32 k + j th
         const int first = (STREAM ? at : rank) * WARPS + warp, step = STREAM ? WARPS : C * WARPS;
         const int mine = first < n_tiles ? (n_tiles - first + step - 1) / step : 0;
+        if (lane < HB) nan_at[warp][lane] = INT_MAX;   // (the last unit's are read: a barrier ago)
         auto look = [&](int i) { return i < mine ? a.c.page(run.seq, (first + i * step) / 2) : -1; };
         int pages = look(lane), ahead = mine > 32 ? look(32 + lane) : -1;   // of i's group of 32, and the next
         // half page i into stage st: every lane brings 16 bytes a copy
@@ -475,11 +474,12 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                     const int pair = 8 * i + 4 * u + c;
                     vw[u] = lds_words<HB>(ch + 16 * HS + (pair * 8 + g) * 4 * HB);
                     vs[u] = lds_words<HB>(ch + 34 * HS + pair * 4 * HB);
-                    if (EDGE) {   // tokens nobody sees may read as NaN
+                    if (EDGE) {   // tokens nobody sees, or not every row
                         const int tk = p0 + 2 * pair;
                         const uint32_t keep = tk + 1 <= top ? 0xffffffffu : tk <= top ? 0xffffu : 0u;
 #pragma unroll
-                        for (int b = 0; b < HB; b++) vs[u].w[b] &= keep;
+                        for (int b = 0; b < HB; b++) vs[u].w[b] = kv_finite_scales(vs[u].w[b] & keep, tk, &nan_at[warp][b]);
+                        __syncwarp();
                     }
                 }
 #pragma unroll
@@ -538,6 +538,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
                 for (int n = 0; n < 4; n++) {
                     const float *d = o[t][2 * b + (n >> 1)] + 2 * (n & 1);
                     f[n] = SPLIT ? d[0] + d[1] : d[e];
+                    if (lim[i] >= nan_at[warp][b]) f[n] = NAN;
                 }
                 *reinterpret_cast<float4 *>(part + r * HS + 32 * b + 4 * g) = make_float4(f[0], f[1], f[2], f[3]);
             }

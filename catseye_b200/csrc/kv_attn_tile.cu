@@ -54,7 +54,7 @@ template <int HS, bool F32> struct TileSmem {
     static constexpr int Q_HALF = HS / 64 * SLICE, Q_TILE = (F32 ? 2 : 1) * Q_HALF, K_STAGE = HS / 64 * SLICE, V_PAGE = HS * 128, V_STAGE = 2 * V_PAGE;
     static constexpr int RAW_UNIT = 72 * HS;                 // K or V of two pages: codes, then scales
     static constexpr int K = QT * Q_TILE, V = K + 2 * K_STAGE, RAW = V + 2 * V_STAGE, BAR = RAW + 3 * RAW_UNIT;
-    static constexpr int BYTES = BAR + 256 + 1024;           // + the alignment's slack
+    static constexpr int BYTES = BAR + 320 + 1024;           // + the alignment's slack
 };
 
 enum TileBar { B_Q, B_KF, B_KE = B_KF + 2, B_VF = B_KE + 2, B_VE = B_VF + 2, B_S = B_VE + 2, B_P = B_S + 2, B_O = B_P + 2, B_RF = B_O + 2, B_RE = B_RF + 3, B_N = B_RE + 3 };
@@ -206,6 +206,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     volatile int *hole = abort_s + 1;   // [4], by KV tile: pages of it that do not exist (bit 0, 1)
     volatile int *present = abort_s + 5;   // [3], by raw buffer: which of its two pages are in it
     uint32_t *slot = const_cast<uint32_t *>(reinterpret_cast<volatile uint32_t *>(abort_s + 8));
+    int *nan_at = reinterpret_cast<int *>(slot + 1);   // [TI_DEQ][HB]: a dequantizing warp's first position with a NaN in V, by block
+    static_assert(B_N * 8 + 9 * 4 + TI_DEQ * HB * 4 <= 320, "");
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
     for (long long back = blockIdx.y; back < mine; back += a.tiles) {
         const long long tile = mine - 1 - back;
         // per Q tile: KV tiles, the first position that some row does not see
-        int n[2], low[2], top = -1;
+        int n[2], low[2], top = -1, floor = INT_MAX;   // floor: what every row sees reaches to
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const long long r0 = tile * ROWS + 128 * i, r1 = min(n_q, r0 + 128) - 1;
@@ -265,6 +267,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 n[i] = t < 0 ? 0 : (int)(t / TI_KV) + 1;
                 low[i] = p1 >= cap ? -1 : (int)max(p0, -1ll);
                 top = max(top, (int)t);
+                floor = min(floor, low[i]);
             }
         }
         const int tiles = max(n[0], n[1]);
@@ -428,13 +431,14 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     ti_wait_ld();
                 }
                 if (real) {
+                    bool nan = false;   // this block of 32 has one that the row sees
+                    for (int d = 0; d < TI_DEQ && n[i] > 0; d++) nan |= lim >= static_cast<volatile int *>(nan_at)[d * HB + (ch >> 5)];
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
                         float4 f = make_float4(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv,
                                                __uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
-                        const float sum = f.x + f.y + f.z + f.w;
                         if (l == 0.f && inv == 0.f) f = make_float4(0.f, 0.f, 0.f, 0.f);
-                        else if (sum != sum && l == l && inv == inv) f = kv_plain_row4(a, run.seq, run.first + tok, head, lim, (ch + k) >> 2);
+                        else if (nan) f = make_float4(NAN, NAN, NAN, NAN);
                         kv_store_row4(a.out, a.type, to + ch + k, f);
                     }
                 }
@@ -471,6 +475,8 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             int v_at[4];
 #pragma unroll
             for (int d = 0; d < 4; d++) v_at[d] = d * 128 + (oct ^ (4 * vg + d)) * 16;
+            if (lane < HB) nan_at[w * HB + lane] = INT_MAX;   // (read behind the barrier that ended the tile before)
+            __syncwarp();
             auto arrive = [&](uint64_t *bp) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bp);
@@ -518,7 +524,9 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                     const int t = p0 + KV_PAGE * vp + 8 * oct + 2 * k;
                     if (p0 + TI_KV - 1 > top) vs[k] &= t + 1 <= top ? 0xffffffffu : t <= top ? 0xffffu : 0u;
                     if (!v_there) vs[k] = 0u;
+                    if (p0 + TI_KV - 1 > floor) vs[k] = kv_finite_scales(vs[k], t, nan_at + w * HB + vb);
                 }
+                __syncwarp();
 #pragma unroll 1
                 for (int u = 0; u < GH; u++) {
                     uint32_t x[4][4];

@@ -1,5 +1,5 @@
 """Attention over the paged Q4_0 cache where a call leaves the ordinary: rows
-behind the table beside values that are NaN."""
+behind the table, values that are NaN."""
 import math
 
 import numpy as np
@@ -39,3 +39,73 @@ def test_rows_past_the_table_beside_a_nan(dtype, mul, hint):
     assert np.isnan(o[1, :, :32]).all() and np.isfinite(o[1, :, 32:]).all()
     assert (o[2:] == 0).all()
     assert _lib.load().cats_gpu_device_error() == 0x40
+
+
+def with_nan(lens, n_kv, hs, at):
+    """Two caches that differ in the value rows named by `at` (sequence, position, head, element) only: NaN there."""
+    clean, dirty = (make(lens, n_kv, hs, layers=1) for _ in range(2))
+    for c in (clean, dirty):
+        fill(c, lens)
+    k, v = kv_rows(lens, n_kv, hs)
+    for s, p, h, e in at:
+        v[sum(lens[:s]) + p, h, e] = math.nan
+    first = np.cumsum([0] + list(lens[:-1]))
+    dirty.append(0, k, v, runs_of([(int(f), n, i, 0) for i, (f, n) in enumerate(zip(first, lens))]), max(lens))
+    return clean, dirty
+
+
+def kv_rows(lens, n_kv, hs):
+    return randn(sum(lens), n_kv, hs, seed=0), randn(sum(lens), n_kv, hs, seed=1)   # as fill() makes them
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hs,mul", [(32, 1), (64, 4), (96, 2), (128, 8), (128, 1)])
+@pytest.mark.parametrize("new,lens,hint", [([300], [700], None), ([700, 1, 9], [700, 150, 400], None), ([1, 3], [400, 300], None),
+                                           ([20, 1, 3], [700, 150, 400], (20, LONG))])
+def test_a_nan_is_only_where_it_is_seen(dtype, hs, mul, new, lens, hint):
+    """NaN in some value rows, first and last of a page, of a tile and of a run:
+    rows that see one are NaN in its block of 32, and all else is, bit for
+    bit, what the cache without them gives."""
+    n_kv = 2
+    at = [(s, p, h, e) for s, n in enumerate(lens)
+          for p, h, e in ((n - 1, 0, 3), (n - new[s], 1, hs - 1), (n - max(new[s] // 2, 1), 0, hs // 2), (128, 1, 0)) if 0 <= p < n]
+    clean, dirty = with_nan(lens, n_kv, hs, at)
+    rows, first, runs = sum(new), 0, []
+    for i, (n, m) in enumerate(zip(new, lens)):
+        runs.append((first, n, i, m - n))
+        first += n
+    q = randn(rows, n_kv * mul, hs, seed=9).to(dtype)
+    want, got = torch.full_like(q, 3), torch.full_like(q, 3)
+    for c, o in ((clean, want), (dirty, got)):
+        c.attention(0, o, q, runs_of(runs), *(hint or (max(new), max(lens))))
+    bad = torch.zeros(rows, n_kv * mul, hs // 32, dtype=torch.bool)
+    for f, n, s, pos in runs:
+        for t, p, h, e in at:
+            if t == s:
+                bad[f + max(p - pos, 0):f + n, h * mul:(h + 1) * mul, e // 32] = True
+    bad = bad.repeat_interleave(32, 2)
+    got, want = got.cpu(), want.cpu()
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
+    assert _lib.load().cats_gpu_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [8000, 5])
+def test_a_nan_does_not_stall_the_batch(dtype, new):
+    """A value row of NaN in every page of a long sequence: the call takes about as long as without."""
+    lens = [8000]
+    clean, dirty = with_nan(lens, 2, 128, [(0, p, h, e) for p in range(7, 8000, 64) for h in (0, 1) for e in (0, 40, 80, 127)])
+    q = randn(new, 8, 128, seed=2).to(dtype)
+    out = torch.empty_like(q)
+    took = []
+    for c in (clean, dirty):
+        each = []
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            c.attention(0, out, q, runs_of([(0, new, 0, 8000 - new)]), new, 8000)
+            b.record()
+            torch.cuda.synchronize()
+            each.append(a.elapsed_time(b))
+        took.append(sorted(each)[2])
+    assert took[1] < 2 * took[0] + 0.05, took
