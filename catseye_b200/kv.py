@@ -5,8 +5,10 @@ runs the operators on them: append, read, attention, copy_pages.  `Pages` is
 the host's bookkeeping: which page holds which tokens of which sequence.
 
 A batch is a CUDA int32 tensor of runs [n][4]: first row, rows, sequence,
-position of the first row.  stream: a cudaStream_t, or None for the library's
-own, which is ordered with the legacy default stream.
+position of the first row.  stream: a cudaStream_t, or None for torch's current
+one (the legacy default: the library's own, which is ordered with it).  A
+call is asynchronous on its stream: what else works on its tensors on another
+is the caller's to order.  Their memory is kept until the call is done with it.
 """
 import ctypes as C
 from array import array
@@ -104,14 +106,21 @@ class Cache:
             raise ValueError(f"runs are on {runs.device}, the cache on {self._dev}")
         return runs.data_ptr(), shape[0]
 
+    def _on(self, stream, *tensors):
+        if stream is None:
+            return _lib.current_stream(self._dev.index)
+        _lib.other_stream(self._dev, stream, (self.pool, self.table, *tensors))
+        return stream
+
     def _kv(self, fn, layer, k, v, runs, max_rows, stream):
         dev = self._dev
         ld_k = _rows(k, self.n_kv_heads, self.head_size, dev, "k")
         ld_v = _rows(v, self.n_kv_heads, self.head_size, dev, "v")
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise ValueError("k and v must have the same type and rows")
-        _lib.check(fn(self._p, layer, k.data_ptr(), v.data_ptr(), _type(k), ld_k, ld_v, k.shape[0], *self._batch(runs),
-                      max_rows, stream), "kv")
+        batch, stream = self._batch(runs), self._on(stream, k, v, runs)
+        _lib.check(fn(self._p, layer, k.data_ptr(), v.data_ptr(), _type(k), ld_k, ld_v, k.shape[0], *batch, max_rows,
+                      stream), "kv")
 
     def append(self, layer, k, v, runs, max_rows, stream=None):
         """Quantize rows k, v [rows, n_kv_heads, head_size] into the pages of `layer`."""
@@ -134,9 +143,10 @@ class Cache:
         ld_o = _rows(out, heads, self.head_size, dev, "out")
         if q.dtype != out.dtype or q.shape[0] != out.shape[0]:
             raise ValueError("q and out must have the same type and rows")
+        batch, stream = self._batch(runs), self._on(stream, q, out, runs)
         _lib.check(self._lib.cats_gpu_kv_attention_dev(self._p, layer, out.data_ptr(), q.data_ptr(), _type(q), heads,
-                                                       ld_o, ld_q, q.shape[0], *self._batch(runs), max_rows, max_len,
-                                                       stream), "kv attention")
+                                                       ld_o, ld_q, q.shape[0], *batch, max_rows, max_len, stream),
+                   "kv attention")
         return out
 
     def copy_pages(self, src, dst, stream=None):
@@ -145,7 +155,7 @@ class Cache:
         (src, n, _a), (dst, m, _b) = _ints(src), _ints(dst)
         if n != m:
             raise ValueError("src and dst must be lists of the same length")
-        _lib.check(self._lib.cats_gpu_kv_copy_pages_dev(self._p, src, dst, n, stream), "copy_pages")
+        _lib.check(self._lib.cats_gpu_kv_copy_pages_dev(self._p, src, dst, n, self._on(stream)), "copy_pages")
 
 
 class Pages:

@@ -10,7 +10,8 @@ def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
     rows may be a wider tensor's): (log softmax at targets [rows] or None,
     entropy [rows] or None, ids of the k <= 32 likeliest [rows, k], their log
     probabilities [rows, k]).  A negative target gives 0; of equal logits the
-    lower id comes first.  stream: a cudaStream_t, or None for the library's."""
+    lower id comes first.  stream: a cudaStream_t, or None for the current one;
+    the results are made on it, and whoever reads them on another waits for it."""
     import torch
     if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: a CUDA tensor [rows, vocab] with contiguous rows is wanted")
@@ -25,6 +26,18 @@ def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
         raise ValueError("targets: a contiguous int32 tensor [rows] on the logits' device is wanted")
     if not 0 <= k <= MAX_K:
         raise ValueError(f"k: 0 to {MAX_K} is wanted, not {k}")
+    if stream is None:
+        stream = _lib.current_stream(dev.index)
+    else:
+        other = _lib.other_stream(dev, stream, (logits, targets))
+        if other is not None:   # the results' memory is that stream's
+            with torch.cuda.stream(other):
+                return _launch(lib, logits, targets, k, entropy, rows, vocab, ld, dev, stream)
+    return _launch(lib, logits, targets, k, entropy, rows, vocab, ld, dev, stream)
+
+
+def _launch(lib, logits, targets, k, entropy, rows, vocab, ld, dev, stream):
+    import torch
     # (four tensors are made in less time than one is cut in three)
     f32 = torch.float32
     lp = torch.empty(rows, dtype=f32, device=dev) if targets is not None else None
