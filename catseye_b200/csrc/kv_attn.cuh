@@ -72,6 +72,14 @@ __device__ __forceinline__ void kv_mma_from(float (&d)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0[0]), "f"(c0[1]), "f"(c0[2]), "f"(c0[3]));
 }
 
+// a += x, b += y, rounded
+__device__ __forceinline__ void kv_add2(float &a, float &b, float x, float y)
+{
+    asm("{\n\t.reg .b64 s, t;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 s, s, t;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
+
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi)
 {
     uint32_t r;

@@ -109,3 +109,33 @@ def test_a_nan_does_not_stall_the_batch(dtype, new):
             each.append(a.elapsed_time(b))
         took.append(sorted(each)[2])
     assert took[1] < 2 * took[0] + 0.05, took
+
+
+@pytest.mark.parametrize("hs", [32, 64, 128])
+@pytest.mark.parametrize("rows,hint", [(1, (1, 1)), (8, (8, 1)), (1, (1, LONG)), (60, (60, 140000)), (300, (300, 140000))])
+def test_long_sums_of_fp32_rows_are_rounded(hs, rows, hint):
+    """131072 values of one sign under nearly flat probabilities, independent of
+    them: what is off is the sums.  A warp adds 32768 tokens, 16 at a time: 2048
+    additions to a sum that grows evenly.  Rounded, each is off by 2^-24 of the
+    sum so far at most, 2^-24 / sqrt(3) rms; over the additions that is
+    sqrt(2048 / 3) 2^-24 / sqrt(3) = 9e-7 of the mean, and the sum of the
+    probabilities as much again: sqrt(2) 9e-7.  What is off in single
+    probabilities (2^-21 each) averages out.  Six such deviations cover some
+    thousand outputs; parts that are joined are off by less.  (Cut off instead of
+    rounded the additions are all off the same way: some 2048 2^-26 = 3e-5.)"""
+    n = 131072
+    c = make([n], 1, hs, layers=1)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = torch.randn(n, 1, hs, generator=g, device="cuda"), torch.rand(n, 1, hs, generator=g, device="cuda") + 0.5
+    runs = runs_of([(0, n, 0, 0)])
+    c.append(0, k, v, runs, n)
+    c.read(0, k, v, runs, n)
+    q = torch.randn(rows, 4, hs, generator=g, device="cuda") * 0.3
+    out = torch.full_like(q, 3)
+    c.attention(0, out, q, runs_of([(0, rows, 0, n - rows)]), *hint)
+    k, v = k[:, 0].double(), v[:, 0].double()
+    hidden = torch.arange(n, device="cuda") > torch.arange(n - rows, n, device="cuda")[:, None]
+    for h in range(4):
+        p = torch.softmax((q[:, h].double() @ k.T / math.sqrt(hs)).masked_fill(hidden, -math.inf), 1)
+        off = (out[:, h].double() / (p @ v) - 1).abs().max()
+        assert off <= 6 * 2**0.5 * 9e-7, off
