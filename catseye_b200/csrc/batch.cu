@@ -1101,6 +1101,7 @@ int llm_forward_batch(LlmModel *m, const int *tokens, const int *pos, const int 
     int rc = llm_batch_set(m, tokens, pos, seqs, T, &nb);
     if (rc) return rc;
     if (llm_batch_enqueue(m, T, nb, false, nullptr, 0) != cudaSuccess) return E_CUDA;
+    if (m->paged) llm_paged_count(m, T, 1, false);
     if (next_host && cudaMemcpyAsync(next_host, m->bt_next, (size_t)T * 4, cudaMemcpyDeviceToHost, m->stream))
         return E_CUDA;
     if (logits_host &&
@@ -1116,7 +1117,7 @@ cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps)
     if (steps <= 0) return cudaSuccess;
     cudaError_t e;
     if (m->paged) {
-        const int rc = llm_paged_extend(m, T, steps, false);
+        const int rc = llm_paged_extend(m, T, steps);
         if (rc) return rc == E_NOMEM ? cudaErrorMemoryAllocation : rc == E_ARG ? cudaErrorInvalidValue : cudaErrorUnknown;
     }
     if (m->bt_log_cap < steps * T) {
@@ -1142,6 +1143,7 @@ cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps)
     }
     for (int s = 0; s < steps; s++)
         if ((e = cudaGraphLaunch(m->bt_exec, m->stream))) return e;
+    if (m->paged) llm_paged_count(m, T, steps, true);
     return cudaSuccess;
 }
 
@@ -1167,7 +1169,10 @@ int llm_score_batch(LlmModel *m, const int *tokens, const int *pos, const int *s
     const ScoreArgs a{m->bt_logits, d_targets, targets ? d_lp : nullptr, entropy ? d_h : nullptr, d_ids, d_top,
                       m->c.vocab, T, m->c.vocab, k, m->err};
     if ((targets && cudaMemcpyAsync(d_targets, targets, n * 4, cudaMemcpyHostToDevice, m->stream)) ||
-        llm_batch_enqueue(m, T, nb, false, nullptr, 0) || launch_logprobs(a, KV_F32, m->stream) ||
+        llm_batch_enqueue(m, T, nb, false, nullptr, 0))
+        return E_CUDA;
+    if (m->paged) llm_paged_count(m, T, 1, false);
+    if (launch_logprobs(a, KV_F32, m->stream) ||
         (targets && cudaMemcpyAsync(logprob, d_lp, n * 4, cudaMemcpyDeviceToHost, m->stream)) ||
         (entropy && cudaMemcpyAsync(entropy, d_h, n * 4, cudaMemcpyDeviceToHost, m->stream)) ||
         (k && (cudaMemcpyAsync(top_ids, d_ids, n * k * 4, cudaMemcpyDeviceToHost, m->stream) ||

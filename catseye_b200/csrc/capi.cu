@@ -837,8 +837,10 @@ int cats_gpu_llm_batch_enqueue(cats_gpu_llm *h)
     const char *what = "cats_gpu_llm_batch_enqueue";
     if (!h || h->bt_T <= 0) return fail(CATS_ERR_ARG, what);
     if (h->m.paged && h->m.paged->advanced > 0)
-        if (int rc = llm_paged_extend(&h->m, h->bt_T, 1, true)) return fail(rc, what);
-    return check(llm_batch_enqueue(&h->m, h->bt_T, h->bt_nb, false, nullptr, 0), what);
+        if (int rc = llm_paged_extend(&h->m, h->bt_T, 1)) return fail(rc, what);
+    if (int rc = check(llm_batch_enqueue(&h->m, h->bt_T, h->bt_nb, false, nullptr, 0), what)) return rc;
+    if (h->m.paged) llm_paged_count(&h->m, h->bt_T, 1, false);
+    return CATS_OK;
 }
 
 int cats_gpu_llm_batch_enqueue_decode(cats_gpu_llm *h, int steps)

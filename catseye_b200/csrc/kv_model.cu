@@ -62,6 +62,8 @@ int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs)
     const size_t tb = (size_t)n_seqs * max_pages * 4;
     bool ok = cudaMalloc(&p->pool, p->page_bytes * n_pages) == cudaSuccess;
     ok = ok && cudaMalloc(&p->table, tb) == cudaSuccess && cudaMallocHost(&p->table_host, tb) == cudaSuccess;
+    ok = ok && cudaMemset(p->table, 0xff, tb) == cudaSuccess;
+    if (ok) memset(p->table_host, 0xff, tb);
     if (!ok) {
         cudaGetLastError();
         std::swap(m->paged, p);   // free the new one, keep what was there
@@ -104,7 +106,8 @@ static int settle(LlmModel *m, const std::vector<int> &src, const std::vector<in
     return cudaMemcpyAsync(p->table, p->table_host, tb, cudaMemcpyHostToDevice, m->stream) == cudaSuccess ? E_OK : E_CUDA;
 }
 
-// Make stretches (sequence, position, count) writable: all of them or none.
+// Make stretches (sequence, position, count) writable, all of them or none; the
+// device's table follows where it changed (table_host is what it holds).
 struct Stretch {
     int seq, pos, n;
 };
@@ -121,22 +124,22 @@ static int write_all(LlmModel *m, std::vector<Stretch> s)
     }
     // The sum of the needs is an upper bound (two stretches may want the same
     // page); past it, try on a copy.
-    const int free0 = pg.free_count();
     long long need = 0;
     for (const Stretch &x : s) need += pg.need(x.seq, x.pos, x.n);
     std::vector<int> src, dst;
     src.reserve(need);
     dst.reserve(need);
-    if (need > free0) {
+    if (need > pg.free_count()) {
         KvPages trial = pg;
         for (const Stretch &x : s)
-            if (int rc = trial.write(x.seq, x.pos, x.n, src, dst)) return rc;
+            if (int rc = trial.reserve(x.seq, x.pos, x.n, src, dst)) return rc;
         pg = std::move(trial);
     } else {
         for (const Stretch &x : s)
-            if (int rc = pg.write(x.seq, x.pos, x.n, src, dst)) return rc;
+            if (int rc = pg.reserve(x.seq, x.pos, x.n, src, dst)) return rc;
     }
-    return pg.free_count() == free0 && src.empty() ? E_OK : settle(m, src, dst);
+    const size_t tb = (size_t)pg.n_seqs() * pg.max_pages() * 4;
+    return src.empty() && !memcmp(m->paged->table_host, pg.table(), tb) ? E_OK : settle(m, src, dst);
 }
 
 static int reserve_rows(LlmModel *m)
@@ -169,11 +172,14 @@ try {
         int n = 1;
         while (t + n < T && tok[t + n].seq == tok[t].seq && tok[t + n].pos == tok[t].pos + n) n++;
         p->runs_host[nr++] = KvRun{t, n, tok[t].seq, tok[t].pos};
-        s.push_back({tok[t].seq, tok[t].pos, std::max(n, ahead)});
+        s.push_back({tok[t].seq, tok[t].pos, ahead ? std::max(n, ahead) : 0});
         rows = std::max(rows, n);
         len = std::max(len, tok[t].pos + n);
         t += n;
     }
+    for (int q : p->set_seqs) p->pages.truncate(q, p->pages.length(q));   // what never ran
+    p->set_seqs.clear();
+    for (const Stretch &x : s) p->set_seqs.push_back(x.seq);
     if (int rc = write_all(m, s)) return rc;
     p->n_runs = nr;
     p->max_rows = rows;
@@ -185,18 +191,23 @@ try {
     return E_NOMEM;
 }
 
-int llm_paged_extend(LlmModel *m, int T, int steps, bool stay)
+int llm_paged_extend(LlmModel *m, int T, int steps)
 try {
     LlmPaged *p = m->paged;
     if (p->n_runs != T) return E_ARG;   // a run of several tokens is not a decode batch
     std::vector<Stretch> s;
     for (int t = 0; t < T; t++) s.push_back({m->bt_tok_host[t].seq, m->bt_tok_host[t].pos + p->advanced, steps});
     if (cudaStreamSynchronize(m->stream) != cudaSuccess) return E_CUDA;
-    if (int rc = write_all(m, s)) return rc;
-    if (!stay) p->advanced += steps;
-    return E_OK;
+    return write_all(m, s);
 } catch (const std::bad_alloc &) {
     return E_NOMEM;
+}
+
+void llm_paged_count(LlmModel *m, int T, int steps, bool move)
+{
+    LlmPaged *p = m->paged;
+    for (int t = 0; t < T; t++) p->pages.count(m->bt_tok_host[t].seq, m->bt_tok_host[t].pos + p->advanced + steps);
+    if (move) p->advanced += steps;
 }
 
 int llm_cache_fork(LlmModel *m, int src, int dst, int len)

@@ -16,6 +16,7 @@ struct LlmPaged {
     int cap = 0;                           // tokens runs / q16 / o16 hold
     int n_runs = 0, max_rows = 0, max_len = 0;
     int advanced = 0;                      // greedy steps enqueued since the batch was set
+    std::vector<int> set_seqs;             // the set batch's sequences
 
     LlmPaged(int n_pages, int n_seqs, int max_pages) : pages(n_pages, n_seqs, max_pages) {}
 };
@@ -26,11 +27,16 @@ struct LlmPaged {
 int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs);
 void llm_paged_free(LlmModel *m);
 // Group the batch in m->bt_tok_host into runs, make their positions writable
-// (from each run's first, at least `ahead`) and upload table and runs.
+// (from each run's first, at least `ahead`; 0: none) and upload table and runs.
+// The sequences' lengths stay: positions count once what writes them is
+// enqueued (llm_paged_count), and the pages of a batch that never ran are free
+// again when the next one is set.
 int llm_paged_set(LlmModel *m, int T, int ahead);
-// The next `steps` positions of a batch of single tokens; stay: the batch
-// does not move on over them.
-int llm_paged_extend(LlmModel *m, int T, int steps, bool stay);
+// Make the next `steps` positions of a batch of single tokens writable.
+int llm_paged_extend(LlmModel *m, int T, int steps);
+// The batch's next `steps` positions a token are enqueued; move: the batch has
+// moved on over them.
+void llm_paged_count(LlmModel *m, int T, int steps, bool move);
 KvView llm_paged_view(const LlmModel *m, int layer);
 int llm_cache_fork(LlmModel *m, int src, int dst, int len);
 int llm_cache_truncate(LlmModel *m, int seq, int len);

@@ -34,8 +34,15 @@ int KvPages::need(int seq, int pos, int n) const
 
 int KvPages::write(int seq, int pos, int n, std::vector<int> &src, std::vector<int> &dst)
 {
-    if (!seq_ok(seq) || pos < 0 || n < 0 || pos > len_[seq] || (long long)pos + n > (long long)max_pages_ * KV_PAGE)
-        return E_ARG;
+    if (!seq_ok(seq) || pos > len_[seq]) return E_ARG;
+    if (int rc = reserve(seq, pos, n, src, dst)) return rc;
+    if (n > 0) count(seq, pos + n);
+    return E_OK;
+}
+
+int KvPages::reserve(int seq, int pos, int n, std::vector<int> &src, std::vector<int> &dst)
+{
+    if (!seq_ok(seq) || pos < 0 || n < 0 || (long long)pos + n > (long long)max_pages_ * KV_PAGE) return E_ARG;
     if (n == 0) return E_OK;
     if (need(seq, pos, n) > free_count()) return E_NOMEM;
     int *t = row(seq);
@@ -49,7 +56,6 @@ int KvPages::write(int seq, int pos, int n, std::vector<int> &src, std::vector<i
         }
         t[i] = p;
     }
-    len_[seq] = std::max(len_[seq], pos + n);
     return E_OK;
 }
 
@@ -71,7 +77,7 @@ int KvPages::truncate(int seq, int len)
 {
     if (!seq_ok(seq) || len < 0 || len > len_[seq]) return E_ARG;
     int *t = row(seq);
-    for (int i = (len + KV_PAGE - 1) / KV_PAGE; i < (len_[seq] + KV_PAGE - 1) / KV_PAGE; i++) {
+    for (int i = (len + KV_PAGE - 1) / KV_PAGE; i < max_pages_ && t[i] >= 0; i++) {
         drop(t[i]);
         t[i] = -1;
     }

@@ -18,9 +18,15 @@ public:
     // to src / dst).  pos may not lie past the sequence's end (E_ARG: the gap
     // would be read).  E_NOMEM, with nothing changed, when too few are free.
     int write(int seq, int pos, int n, std::vector<int> &src, std::vector<int> &dst);
+    // The same without the tokens being there yet: the length stays until count()
+    // says that a sequence holds its first `end` tokens.  (pos may lie behind
+    // other reserved positions.)  truncate() frees what was reserved and not
+    // counted.
+    int reserve(int seq, int pos, int n, std::vector<int> &src, std::vector<int> &dst);
+    void count(int seq, int end) { if (end > len_[seq]) len_[seq] = end; }
     // dst becomes the first len tokens of src, sharing its pages.
     int fork(int src, int dst, int len);
-    // Keep the first len tokens of a sequence; pages nobody holds are free.
+    // Keep the first len tokens of a sequence, and pages for no more; pages nobody holds are free.
     int truncate(int seq, int len);
     // Renumber so that the used pages are 0 .. used - 1 (the copies to make).
     void compact(std::vector<int> &src, std::vector<int> &dst);

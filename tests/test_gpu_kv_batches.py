@@ -1,0 +1,83 @@
+"""The batched step on the paged Q4_0 cache: what its calls leave behind when
+they do not run, run late or run out of room."""
+import numpy as np
+import pytest
+
+from models import prompt
+from test_gpu_kv_model import config, llm, model  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def start(llm, orc, pages=6, seqs=3, n=70, **kw):
+    cfg = config(llm, 32, **kw)
+    _, m = model(llm, orc, cfg, pages, seqs)
+    toks = prompt(10, 200, cfg.vocab)
+    m.forward_batch(toks[:n], np.arange(n), np.zeros(n, int))
+    return m, toks
+
+
+def test_no_steps_leave_no_position(llm, orc):
+    m, toks = start(llm, orc)
+    free = m.cache_free_pages
+    assert m.generate_batch(toks[70:72], [70, 0], 0).shape == (0, 2)
+    assert [m.cache_length(s) for s in range(3)] == [70, 0, 0] and m.cache_free_pages == free
+    with pytest.raises(RuntimeError):
+        m.cache_read(0, 0, 71)
+    with pytest.raises(RuntimeError):                 # a gap, as ever
+        m.generate_batch(toks[70:71], [71], 0)
+    with pytest.raises(RuntimeError):
+        m.forward_batch(toks[71:72], [71], [0])
+    m.close()
+
+
+def test_a_batch_that_never_ran_leaves_no_position(llm, orc):
+    m, toks = start(llm, orc)
+    _, want = m.forward_batch(toks[70:72], [70, 71], [0, 0], logits=True)
+    m.cache_truncate(0, 70)
+    m.batch_set(toks[70:72], [70, 71], [0, 0])
+    assert m.cache_length(0) == 70
+    with pytest.raises(RuntimeError):                 # 70 and 71 were not written
+        m.forward_batch(toks[72:73], [72], [0])
+    with pytest.raises(RuntimeError):
+        m.cache_read(0, 0, 72)
+    with pytest.raises(RuntimeError):
+        m.cache_fork(0, 1, 72)
+    m.batch_set(toks[70:72], [70, 71], [0, 0])
+    m.batch_enqueue()
+    m.synchronize()
+    assert m.cache_length(0) == 72
+    _, got = m.forward_batch(toks[70:72], [70, 71], [0, 0], logits=True)
+    assert np.array_equal(got, want)
+    m.close()
+
+
+def test_pages_of_a_batch_that_never_ran_are_free_for_the_next(llm, orc):
+    m, toks = start(llm, orc, pages=4)                # two pages left
+    m.batch_set(toks[:128], np.arange(128), np.ones(128, int))
+    m.batch_set(toks[:65], np.arange(65), np.full(65, 2))
+    m.batch_enqueue()
+    m.synchronize()
+    assert [m.cache_length(s) for s in range(3)] == [70, 0, 65] and m.cache_free_pages == 0
+    _, a = m.forward_batch(toks[65:68], np.arange(65, 68), np.full(3, 2), logits=True)
+    _, b = m.forward_batch(toks[65:68], np.arange(65, 68), np.zeros(3, int), logits=True)
+    assert np.array_equal(a, b)                       # the same context, in other pages
+    m.close()
+
+
+def test_lengths_follow_the_enqueued_steps(llm, orc):
+    m, toks = start(llm, orc)
+    m.batch_set([toks[70], toks[0]], [70, 0], [0, 1])
+    assert [m.cache_length(s) for s in range(2)] == [70, 0]
+    m.batch_enqueue()
+    assert [m.cache_length(s) for s in range(2)] == [71, 1]
+    m.batch_enqueue_decode(5)
+    assert [m.cache_length(s) for s in range(2)] == [75, 5]
+    m.batch_enqueue()
+    m.batch_enqueue_decode(60)
+    m.synchronize()
+    assert [m.cache_length(s) for s in range(2)] == [135, 65] and m.cache_free_pages == 6 - 3 - 2
+    with pytest.raises(RuntimeError):                 # past the pool: 72 more positions each want two pages
+        m.batch_enqueue_decode(130)
+    assert [m.cache_length(s) for s in range(2)] == [135, 65]
+    m.close()
