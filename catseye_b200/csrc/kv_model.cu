@@ -55,6 +55,7 @@ int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs)
     LlmPaged *p = nullptr;
     try {
         p = new LlmPaged(n_pages, n_seqs, max_pages);
+        p->sent.assign((size_t)n_seqs * max_pages, -1);
     } catch (const std::bad_alloc &) {
         return E_NOMEM;
     }
@@ -63,7 +64,6 @@ int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs)
     bool ok = cudaMalloc(&p->pool, p->page_bytes * n_pages) == cudaSuccess;
     ok = ok && cudaMalloc(&p->table, tb) == cudaSuccess && cudaMallocHost(&p->table_host, tb) == cudaSuccess;
     ok = ok && cudaMemset(p->table, 0xff, tb) == cudaSuccess;
-    if (ok) memset(p->table_host, 0xff, tb);
     if (!ok) {
         cudaGetLastError();
         std::swap(m->paged, p);   // free the new one, keep what was there
@@ -103,15 +103,56 @@ static int settle(LlmModel *m, const std::vector<int> &src, const std::vector<in
         return E_CUDA;
     const size_t tb = (size_t)p->pages.n_seqs() * p->pages.max_pages() * 4;
     memcpy(p->table_host, p->pages.table(), tb);
+    memcpy(p->sent.data(), p->pages.table(), tb);
     return cudaMemcpyAsync(p->table, p->table_host, tb, cudaMemcpyHostToDevice, m->stream) == cudaSuccess ? E_OK : E_CUDA;
 }
 
-// Make stretches (sequence, position, count) writable, all of them or none; the
-// device's table follows where it changed (table_host is what it holds).
+// A few entries of the table, as the kernel's parameters: no staging that an
+// earlier copy may still read, so the host need not wait for the stream.
+constexpr int KV_PATCH = 240;
+struct KvPatch {
+    unsigned long long at[KV_PATCH];
+    int page[KV_PATCH];
+};
+__global__ void k_kv_patch(int *table, int n, const __grid_constant__ KvPatch p)
+{
+    if ((int)threadIdx.x < n) table[p.at[threadIdx.x]] = p.page[threadIdx.x];
+}
+
+// Positions of a sequence to make writable.
 struct Stretch {
     int seq, pos, n;
 };
-static int write_all(LlmModel *m, std::vector<Stretch> s)
+
+// The page copies, and the entries of the stretches that changed, in stream order.
+static int settle_behind(LlmModel *m, const std::vector<Stretch> &s, const std::vector<int> &src, const std::vector<int> &dst)
+{
+    LlmPaged *p = m->paged;
+    if (!src.empty() &&
+        launch_kv_copy(p->pool, p->page_bytes, src.data(), dst.data(), (int)src.size(), m->stream) != cudaSuccess)
+        return E_CUDA;
+    KvPatch patch;
+    int n = 0;
+    auto send = [&] {
+        if (n > 0) k_kv_patch<<<1, 256, 0, m->stream>>>(p->table, n, patch);
+        n = 0;
+        return cudaGetLastError() == cudaSuccess;
+    };
+    for (const Stretch &x : s)
+        for (int i = x.pos / KV_PAGE; x.n > 0 && i <= (x.pos + x.n - 1) / KV_PAGE; i++) {
+            const size_t at = (size_t)x.seq * p->pages.max_pages() + i;
+            if (p->sent[at] == p->pages.table()[at]) continue;
+            patch.at[n] = at;
+            patch.page[n++] = p->sent[at] = p->pages.table()[at];
+            if (n == KV_PATCH && !send()) return E_CUDA;
+        }
+    return send() ? E_OK : E_CUDA;
+}
+
+// Make stretches writable, all of them or none; the
+// device's table follows where it changed.  idle: nothing is enqueued on the
+// stream.
+static int write_all(LlmModel *m, std::vector<Stretch> s, bool idle)
 {
     KvPages &pg = m->paged->pages;
     std::sort(s.begin(), s.end(), [](const Stretch &a, const Stretch &b) { return a.seq != b.seq ? a.seq < b.seq : a.pos < b.pos; });
@@ -138,8 +179,9 @@ static int write_all(LlmModel *m, std::vector<Stretch> s)
         for (const Stretch &x : s)
             if (int rc = pg.reserve(x.seq, x.pos, x.n, src, dst)) return rc;
     }
+    if (!idle) return settle_behind(m, s, src, dst);
     const size_t tb = (size_t)pg.n_seqs() * pg.max_pages() * 4;
-    return src.empty() && !memcmp(m->paged->table_host, pg.table(), tb) ? E_OK : settle(m, src, dst);
+    return src.empty() && !memcmp(m->paged->sent.data(), pg.table(), tb) ? E_OK : settle(m, src, dst);
 }
 
 static int reserve_rows(LlmModel *m)
@@ -180,7 +222,7 @@ try {
     for (int q : p->set_seqs) p->pages.truncate(q, p->pages.length(q));   // what never ran
     p->set_seqs.clear();
     for (const Stretch &x : s) p->set_seqs.push_back(x.seq);
-    if (int rc = write_all(m, s)) return rc;
+    if (int rc = write_all(m, s, true)) return rc;
     p->n_runs = nr;
     p->max_rows = rows;
     p->max_len = len;
@@ -197,8 +239,7 @@ try {
     if (p->n_runs != T) return E_ARG;   // a run of several tokens is not a decode batch
     std::vector<Stretch> s;
     for (int t = 0; t < T; t++) s.push_back({m->bt_tok_host[t].seq, m->bt_tok_host[t].pos + p->advanced, steps});
-    if (cudaStreamSynchronize(m->stream) != cudaSuccess) return E_CUDA;
-    return write_all(m, s);
+    return write_all(m, s, false);
 } catch (const std::bad_alloc &) {
     return E_NOMEM;
 }

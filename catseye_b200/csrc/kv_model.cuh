@@ -10,7 +10,8 @@ struct LlmPaged {
     KvPages pages;
     size_t page_bytes = 0;
     uint8_t *pool = nullptr;               // device
-    int *table = nullptr, *table_host = nullptr;
+    int *table = nullptr, *table_host = nullptr;   // device; pinned staging
+    std::vector<int> sent;                 // what the device's table holds once the stream gets there
     KvRun *runs = nullptr, *runs_host = nullptr;
     __half *q16 = nullptr, *o16 = nullptr; // [cap][q_dim]: queries (RoPE applied) and attention output
     int cap = 0;                           // tokens runs / q16 / o16 hold
@@ -32,7 +33,8 @@ void llm_paged_free(LlmModel *m);
 // enqueued (llm_paged_count), and the pages of a batch that never ran are free
 // again when the next one is set.
 int llm_paged_set(LlmModel *m, int T, int ahead);
-// Make the next `steps` positions of a batch of single tokens writable.
+// Make the next `steps` positions of a batch of single tokens writable, behind
+// what is enqueued (the host does not wait).
 int llm_paged_extend(LlmModel *m, int T, int steps);
 // The batch's next `steps` positions a token are enqueued; move: the batch has
 // moved on over them.

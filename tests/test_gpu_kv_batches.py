@@ -81,3 +81,38 @@ def test_lengths_follow_the_enqueued_steps(llm, orc):
         m.batch_enqueue_decode(130)
     assert [m.cache_length(s) for s in range(2)] == [135, 65]
     m.close()
+
+
+def test_enqueued_steps_do_not_wait_for_the_stream(llm, orc):
+    """Steps enqueued behind work that takes long: the host goes on at once,
+    across page ends and with pages shared until then, and what comes out is what
+    the waiting calls give."""
+    import time
+
+    import torch
+    m, toks = start(llm, orc, pages=16)
+    start_at = np.array([toks[70], toks[71], 9], np.int32)
+    m.cache_fork(0, 1, 70)
+    m.cache_fork(0, 2, 64)
+    want = m.generate_batch(start_at, [70, 70, 64], 130)
+    kept = [m.cache_read(l, s, 190) for l in range(2) for s in range(3)]
+    for s in (1, 2):
+        m.cache_fork(0, s, 70 if s == 1 else 64)
+    m.cache_truncate(0, 70)
+    m.batch_set(start_at, [70, 70, 64], [0, 1, 2])
+    side = torch.cuda.ExternalStream(m.stream)
+    took = []
+    for steps in (30, 30, 70):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(800_000_000)            # some 0.4 s
+        t = time.perf_counter()
+        m.batch_enqueue_decode(steps)
+        took.append(time.perf_counter() - t)
+    m.batch_enqueue()
+    m.synchronize()
+    assert max(took) < 0.2, took
+    assert [m.cache_length(s) for s in range(3)] == [201, 201, 195]
+    again = [m.cache_read(l, s, 190) for l in range(2) for s in range(3)]
+    assert all(np.array_equal(a[i], b[i]) for a, b in zip(kept, again) for i in (0, 1))
+    assert want.shape == (130, 3)
+    m.close()
