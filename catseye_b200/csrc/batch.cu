@@ -1116,10 +1116,6 @@ cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps)
     // one token; one step is captured once into a graph and replayed
     if (steps <= 0) return cudaSuccess;
     cudaError_t e;
-    if (m->paged) {
-        const int rc = llm_paged_extend(m, T, steps);
-        if (rc) return rc == E_NOMEM ? cudaErrorMemoryAllocation : rc == E_ARG ? cudaErrorInvalidValue : cudaErrorUnknown;
-    }
     if (m->bt_log_cap < steps * T) {
         if (m->bt_log) cudaFree(m->bt_log);
         m->bt_log = nullptr;
@@ -1184,8 +1180,10 @@ int llm_score_batch(LlmModel *m, const int *tokens, const int *pos, const int *s
 int llm_generate_batch(LlmModel *m, int T, int steps, int *tokens_host)
 {
     if (steps <= 0) return E_OK;
+    if (m->paged)
+        if (int rc = llm_paged_extend(m, T, steps)) return rc;
     cudaError_t e = llm_batch_decode_enqueue(m, T, steps);
-    if (e) return e == cudaErrorMemoryAllocation ? E_NOMEM : e == cudaErrorInvalidValue ? E_ARG : E_CUDA;
+    if (e) return e == cudaErrorMemoryAllocation ? E_NOMEM : E_CUDA;
     if (tokens_host &&
         cudaMemcpyAsync(tokens_host, m->bt_log, (size_t)steps * T * 4, cudaMemcpyDeviceToHost, m->stream))
         return E_CUDA;

@@ -847,11 +847,9 @@ int cats_gpu_llm_batch_enqueue_decode(cats_gpu_llm *h, int steps)
 {
     const char *what = "cats_gpu_llm_batch_enqueue_decode";
     if (!h || h->bt_T <= 0 || steps < 0 || h->bt_nb != h->bt_T) return fail(CATS_ERR_ARG, what);
-    const cudaError_t e = llm_batch_decode_enqueue(&h->m, h->bt_T, steps);
-    // (the paged cache: no room, or past the context)
-    if (h->m.paged && (e == cudaErrorMemoryAllocation || e == cudaErrorInvalidValue))
-        return fail(e == cudaErrorMemoryAllocation ? CATS_ERR_NOMEM : CATS_ERR_ARG, what);
-    return check(e, what);
+    if (h->m.paged && steps > 0)   // no room, or past the context
+        if (int rc = llm_paged_extend(&h->m, h->bt_T, steps)) return fail(rc, what);
+    return check(llm_batch_decode_enqueue(&h->m, h->bt_T, steps), what);
 }
 
 int cats_gpu_llm_time_product(cats_gpu_llm *h, int kind, int T, int reps, float *ms_per_launch,

@@ -183,7 +183,7 @@ int llm_forward_batch(LlmModel *m, const int *tokens, const int *pos, const int 
 int llm_score_batch(LlmModel *m, const int *tokens, const int *pos, const int *seqs, int T, const int *targets, int k,
                     float *logprob, float *entropy, int *top_ids, float *top_logprob);
 int llm_generate_batch(LlmModel *m, int T, int steps, int *tokens_host);
-cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps);
+cudaError_t llm_batch_decode_enqueue(LlmModel *m, int T, int steps);   // (paged: after llm_paged_extend)
 // Device time of one kind of batched product (0 qkv, 1 wo, 2 w13, 3 w2,
 // 4 classifier) at T tokens: `reps` passes over every layer's weight of that
 // kind, back to back on the model's stream (CUDA events).  Reports ms per

@@ -116,3 +116,25 @@ def test_enqueued_steps_do_not_wait_for_the_stream(llm, orc):
     assert all(np.array_equal(a[i], b[i]) for a, b in zip(kept, again) for i in (0, 1))
     assert want.shape == (130, 3)
     m.close()
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_what_a_refused_generation_reports(llm, orc, paged):
+    """Past the context: a bad argument with either cache; past the pool: no memory."""
+    from catseye_b200 import _lib
+    m, toks = start(llm, orc)
+    lib, ids = _lib.load(), np.zeros(1000, np.int32)
+    if not paged:
+        m.cache_q4(0)
+    t, p = np.array([5], np.int32), np.array([70 if paged else 0], np.int32)
+    run = lambda steps: lib.cats_gpu_llm_generate_batch(m.h, t.ctypes.data, p.ctypes.data, 1, steps, ids.ctypes.data)  # noqa: E731
+    assert run(321) == 2
+    if paged:
+        m.cache_fork(0, 1, 70)
+        m.cache_fork(0, 2, 70)
+        m.batch_set([5, 6, 7], [70, 70, 70], [0, 1, 2])
+        assert lib.cats_gpu_llm_batch_enqueue_decode(m.h, 251) == 2
+        assert lib.cats_gpu_llm_batch_enqueue_decode(m.h, 180) == 3
+    lib.cats_gpu_clear_error()
+    assert run(3) == 0
+    m.close()
