@@ -46,9 +46,14 @@ def _ints(x):
     if isinstance(x, (list, tuple)):   # a third of the time through numpy
         a = array("i", x)
         return a.buffer_info()[0], len(a), a
-    a = np.ascontiguousarray(x, np.int32)
+    a = np.asarray(x)
     if a.ndim != 1:
         raise ValueError("a list of integers is wanted")
+    if a.size and a.dtype.kind not in "iu":
+        raise TypeError(f"integers are wanted, not {a.dtype}")
+    if a.size and not -2**31 <= int(a.min()) <= int(a.max()) < 2**31:
+        raise OverflowError("page numbers of 32 bits are wanted")
+    a = np.ascontiguousarray(a, np.int32)
     return a.ctypes.data, a.size, a
 
 

@@ -1,0 +1,24 @@
+"""Arguments of catseye_b200.kv and .score that are refused before any device call."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from catseye_b200 import kv
+
+
+@pytest.mark.parametrize("bad,error", [(np.array([1.0, 2.0]), TypeError), (np.array([0.5]), TypeError), ([1.5], TypeError),
+                                       (np.array([True]), TypeError), (np.array([2**32 + 5]), OverflowError),
+                                       (np.array([-2**31 - 1]), OverflowError), ([2**32 + 5], OverflowError),
+                                       (np.array([2**63], np.uint64), OverflowError), (np.zeros((1, 2), np.int32), ValueError)])
+def test_page_lists_that_are_not_page_numbers(bad, error):
+    with pytest.raises(error):
+        kv._ints(bad)
+
+
+@pytest.mark.parametrize("good", [[3, -1, 7], (3, -1, 7), np.array([3, -1, 7]), np.array([3, -1, 7], np.int8),
+                                  np.array([3, 0, -1, 0, 7, 0], np.int32)[::2]])
+def test_page_lists(good):
+    at, n, owner = kv._ints(good)
+    assert n == 3 and list((C.c_int * 3).from_address(at)) == [3, -1, 7] and owner is not None
+    assert kv._ints([])[1] == kv._ints(np.array([]))[1] == 0
