@@ -234,3 +234,10 @@ def other_stream(device, stream, tensors):
         if t is not None:
             t.record_stream(other)
     return other
+
+
+def no_gradient(what):
+    """Refuse a tensor that wants a gradient, as torch does for `out=`, unless none is recorded."""
+    import torch
+    if torch.is_grad_enabled():
+        raise ValueError(f"{what} requires a gradient, which this call does not give: detach it, or call under torch.no_grad()")

@@ -9,6 +9,7 @@ position of the first row.  stream: a cudaStream_t, or None for torch's current
 one (the legacy default: the library's own, which is ordered with it).  A
 call is asynchronous on its stream: what else works on its tensors on another
 is the caller's to order.  Their memory is kept until the call is done with it.
+No gradient passes through the cache: rows that want one are refused.
 """
 import ctypes as C
 from array import array
@@ -67,6 +68,8 @@ def _rows(t, heads, hs, device, what):
     s0, s1, s2 = t.stride()
     if (s2 != 1 and hs > 1) or (s1 != hs and heads > 1):
         raise ValueError(f"{what}: the values of a row must be contiguous")
+    if t.requires_grad:
+        _lib.no_gradient(what)
     width = heads * hs
     if shape[0] <= 1:
         return width

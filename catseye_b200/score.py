@@ -11,8 +11,11 @@ def logprobs(logits, targets=None, k=0, entropy=True, stream=None):
     entropy [rows] or None, ids of the k <= 32 likeliest [rows, k], their log
     probabilities [rows, k]).  A negative target gives 0; of equal logits the
     lower id comes first.  stream: a cudaStream_t, or None for the current one;
-    the results are made on it, and whoever reads them on another waits for it."""
+    the results are made on it, and whoever reads them on another waits for it.
+    They carry no gradient: logits that want one are refused."""
     import torch
+    if logits.requires_grad:
+        _lib.no_gradient("logits")
     if logits.dim() != 2 or not logits.is_cuda or logits.shape[1] == 0 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: a CUDA tensor [rows, vocab] with contiguous rows is wanted")
     rows, vocab = logits.shape

@@ -22,3 +22,17 @@ def test_page_lists(good):
     at, n, owner = kv._ints(good)
     assert n == 3 and list((C.c_int * 3).from_address(at)) == [3, -1, 7] and owner is not None
     assert kv._ints([])[1] == kv._ints(np.array([]))[1] == 0
+
+
+def test_tensors_that_want_a_gradient():
+    """Nothing silently stops a gradient; without one being recorded the same tensors pass."""
+    import torch
+    from catseye_b200 import score
+    x, cpu = torch.zeros(2, 1, 32, requires_grad=True), torch.device("cpu")
+    for call in (lambda: kv._rows(x, 1, 32, cpu, "k"), lambda: kv._rows(x * 2, 1, 32, cpu, "q"),
+                 lambda: score.logprobs(torch.zeros(2, 5, requires_grad=True))):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        assert kv._rows(x, 1, 32, cpu, "k") == 32
+    assert kv._rows(x.detach(), 1, 32, cpu, "k") == 32
