@@ -272,8 +272,10 @@ cudaError_t launch_kv_read(const KvView &c, int type, const KvRows &k, const KvR
 
 // -------------------------------------------------------------- attention
 cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, const KvRows &q, int n_heads,
-                                const KvBatch &b, cudaStream_t st)
+                                const KvBatch &b0, cudaStream_t st)
 {
+    KvBatch b = b0;
+    b.max_rows = std::min(b.max_rows, q.rows);
     KvAttn a{};
     a.c = c;
     a.out = out;

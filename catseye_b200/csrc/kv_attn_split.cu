@@ -797,7 +797,11 @@ cudaError_t launch_kv_attn_split(const KvAttn &a0, int max_rows, int max_len, cu
     // 157 and 145.
     const int nt = q <= sp_rows(split, 1) ? 1 : 2, rows = sp_rows(split, nt), slots = 148 * sp_resident(nt);
     a.tiles = (int)std::min<long long>((q + rows - 1) / rows, 1 << 16);
-    const long long units = (long long)a.n_runs * a.c.n_kv * a.tiles, halves = std::max(1, max_len / SP_TOK + (max_len % SP_TOK != 0));
+    // (a CTA goes through a run's further tiles itself: the grid of a batch of many
+    // runs, one of them long, stays bounded)
+    const long long pairs = (long long)a.n_runs * a.c.n_kv;
+    if (pairs * a.tiles > 1 << 24) a.tiles = (int)std::max(1ll, (1 << 24) / pairs);
+    const long long units = pairs * a.tiles, halves = std::max(1, max_len / SP_TOK + (max_len % SP_TOK != 0));
     if (units > (1ll << 26)) return cudaErrorInvalidValue;
     // Many half pages: streamed, one CTA for each of the SMs' slots.  Else a cluster a
     // unit, up to 8 CTAs while each warp has a half page.

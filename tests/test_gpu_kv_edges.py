@@ -139,3 +139,26 @@ def test_long_sums_of_fp32_rows_are_rounded(hs, rows, hint):
         p = torch.softmax((q[:, h].double() @ k.T / math.sqrt(hs)).masked_fill(hidden, -math.inf), 1)
         off = (out[:, h].double() / (p @ v) - 1).abs().max()
         assert off <= 6 * 2**0.5 * 9e-7, off
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hs,n_runs,long", [(32, 9000, 4300), (96, 700, 90), (64, 70000, 40)])
+def test_many_runs_beside_a_long_one(dtype, hs, n_runs, long):
+    """Thousands of runs of one row or none and a longer one, and a hint far past what the tensor holds."""
+    n_kv, lens = 16, [long + 10, 30]
+    c = make(lens, n_kv, hs, layers=1)
+    fill(c, lens)
+    single = [(long + i, 1, 1, 20 + i) for i in range(5)]
+    runs = [(0, 0, 1, 0)] * 100 + single[:2] + [(0, long, 0, 10)] + [(0, 0, 0, 7)] * (n_runs - 106) + single[2:]
+    q = randn(long + 6, n_kv, hs, seed=7).to(dtype)
+    outs = []
+    for hint in ((long, long + 10), (2**31 - 1, 2**31 - 1)):
+        out = torch.full_like(q, 3)
+        c.attention(0, out, q, runs_of(runs), *hint)
+        outs.append(out)
+    torch.cuda.synchronize()
+    few = [(long, 1, 1, 20), (long + 4, 1, 1, 24), (0, 2, 0, 10), (long - 1, 1, 0, long + 9)]
+    for out in outs:
+        check_attention(c, 0, q, out, few, 1)
+        assert (out[long + 5:] == 3).all() and out[:long + 5].isfinite().all()
+    assert _lib.load().cats_gpu_device_error() == 0
