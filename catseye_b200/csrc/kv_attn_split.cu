@@ -18,7 +18,8 @@
 // the sum a product and always towards zero: of a warp's 32768 tokens of one
 // sign 2e-4 were lost.  fp32 rows therefore start every product of p v (16
 // tokens) at zero and add it, rounded (1e-6; 16 sequences of 2048 tokens 55.3 ->
-// 55.9 us).
+// 55.9 us).  Rows of 16 bits do so after 64 products, which is 6e-6 (64 ragged
+// sequences 113 -> 114 us; after each product 116).
 //
 // Two ways to share the work.  Few half pages: a cluster of up to 8 CTAs a
 // (row tile, kv head), joined through distributed shared memory, one launch.
@@ -48,6 +49,7 @@ namespace cg = cooperative_groups;
 constexpr int SP_STAGES = 3;
 constexpr int SP_WARPS = 4;
 constexpr int SP_TOK = 32;          // tokens of a stage: half a page
+constexpr int SP_FOLD = 32;         // 16-bit rows: half pages of a warp that share an accumulator
 constexpr float SP_P_BITS = 15.f;   // probabilities are held times 2^15: fp16 keeps those down to 2^-39
 
 // a stage: K codes [32 tokens], V codes, K scales, V scales
@@ -512,8 +514,36 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
             }
         };
 
+        // 16-bit rows: after SP_FOLD half pages the sums join those before, kept in
+        // local memory with the maxima they are relative to.
+        constexpr int ACC = NT * 2 * HB * 4;
+        float store[SPLIT ? 1 : ACC + NS];
+        float *kept = store;
+        asm volatile("" : "+l"(kept));   // (memory, not registers: it is rarely touched)
+        auto join_kept = [&] {
+            float f[NS];
+#pragma unroll
+            for (int r = 0; r < NS; r++) f[r] = kept[ACC + r] == -INFINITY ? 0.f : kv_exp2(kept[ACC + r] - m[r]);
+#pragma unroll
+            for (int k = 0; k < ACC; k++) {
+                float &v = o[k / (8 * HB)][k / 4 % (2 * HB)][k % 4];
+                v = fmaf(kept[k], f[2 * (k / (8 * HB)) + k % 2], v);
+            }
+        };
+
         int st = 0;
         for (int i = 0; i < mine; i++) {
+            if (!SPLIT && i > 0 && i % SP_FOLD == 0) {
+                if (i > SP_FOLD) join_kept();
+#pragma unroll
+                for (int k = 0; k < ACC; k++) {
+                    float &v = o[k / (8 * HB)][k / 4 % (2 * HB)][k % 4];
+                    kept[k] = v;
+                    v = 0.f;
+                }
+#pragma unroll
+                for (int r = 0; r < NS; r++) kept[ACC + r] = m[r];
+            }
             const int page = here[0], p0 = (first + i * step) * SP_TOK, nx = i + SP_STAGES - 1;
             if ((nx & 31) == 0) {   // nx starts the next group of 32
                 pages = ahead;
@@ -531,6 +561,7 @@ k_kv_attn_split(const __grid_constant__ KvAttn a, const __grid_constant__ SpWork
             }
             st = st + 1 == SP_STAGES ? 0 : st + 1;
         }
+        if (!SPLIT && mine > SP_FOLD) join_kept();
         asm volatile("cp.async.wait_all;" ::: "memory");
         __syncwarp();
 

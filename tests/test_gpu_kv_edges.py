@@ -162,3 +162,32 @@ def test_many_runs_beside_a_long_one(dtype, hs, n_runs, long):
         check_attention(c, 0, q, out, few, 1)
         assert (out[long + 5:] == 3).all() and out[:long + 5].isfinite().all()
     assert _lib.load().cats_gpu_device_error() == 0
+
+
+@pytest.mark.parametrize("hs", [32, 64, 96, 128])
+@pytest.mark.parametrize("rows,mul,hint", [(1, 4, (1, 1)), (8, 4, (8, 1)), (1, 4, (1, LONG)), (60, 4, (60, 140000))])
+def test_long_sums_of_fp16_rows_are_not_cut_off(hs, rows, mul, hint):
+    """The same for fp16 rows, where the outputs' roundings hide single sums but
+    not their mean: an output is off by 2^-11 / sqrt(12) of itself rms at most
+    (its rounding), 1.4e-4, so the mean of 4 hs outputs by 1.4e-4 / sqrt(4 hs);
+    six of those.  What the sums are cut off by goes one way: accumulators hold
+    the products of 4096 tokens at most before they are added, rounded, to the
+    rest; 256 products of 2^-23 lose 2^-16 on average over them as they grow."""
+    n = 131072
+    c = make([n], 1, hs, layers=1)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = torch.randn(n, 1, hs, generator=g, device="cuda"), torch.rand(n, 1, hs, generator=g, device="cuda") + 0.5
+    runs = runs_of([(0, n, 0, 0)])
+    c.append(0, k, v, runs, n)
+    c.read(0, k, v, runs, n)
+    q = (torch.randn(rows, mul, hs, generator=g, device="cuda") * 0.3).half()
+    out = torch.full_like(q, 3)
+    c.attention(0, out, q, runs_of([(0, rows, 0, n - rows)]), *hint)
+    k, v = k[:, 0].double(), v[:, 0].double()
+    hidden = torch.arange(n, device="cuda") > torch.arange(n - rows, n, device="cuda")[:, None]
+    off = []
+    for h in range(4):
+        p = torch.softmax((q[:, h].double() @ k.T / math.sqrt(hs)).masked_fill(hidden, -math.inf), 1)
+        off.append(out[:, h].double() / (p @ v) - 1)
+    off = torch.stack(off).mean()
+    assert off.abs() <= 6 * 1.4e-4 / math.sqrt(4 * hs) + 2**-16, off
