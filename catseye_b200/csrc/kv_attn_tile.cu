@@ -23,7 +23,7 @@
 // Bound by a tile's chain: 128 tokens take a row's thread some 2900 cycles (its
 // exponentials alone 1024, sixteen a cycle and SM) and then the products 1000,
 // which the other tile's rows hide only in part.  4096 rows of 32 heads of 128
-// (bf16, causal): 225 us, 611 TFLOP/s; 64 tokens at a time with S twice 260 us,
+// (bf16, causal): 219 us, 628 TFLOP/s (the variants against 225 then): 64 tokens at a time with S twice 260 us,
 // two threads a row 313 us, eight dequantizing warps 249 us, S loaded a piece
 // ahead 250 us: all of them more code, and the roles share one instruction
 // cache.  The accumulator is not rescaled for every new maximum: m is only moved
@@ -42,6 +42,7 @@ constexpr int TI_KV = 128;
 __host__ __device__ constexpr int ti_q_tiles(int hs, bool f32) { return f32 && hs == 128 ? 1 : 2; }
 constexpr int TI_SOFT = 8, TI_DEQ = 4, TI_MMA_WARP = TI_SOFT + TI_DEQ, TI_LOAD_WARP = TI_MMA_WARP + 1,
               TI_THREADS = (TI_LOAD_WARP + 1) * 32;
+constexpr int TI_FOLD = 32;   // 16-bit rows: tiles of tokens that share an accumulator
 constexpr float TI_P_BITS = 7.f, TI_LAG = 8.f;   // probabilities are held times 2^7 and may reach 2^15
 
 // shared memory, from a 1024-byte boundary: Q [2][HS/64][128 rows][128 B] (fp32
@@ -192,6 +193,19 @@ __device__ __noinline__ void ti_fold(uint32_t O, uint32_t R, int cols, bool more
         }
     }
     ti_wait_st();
+}
+
+// kept = kept * f + O (more: kept has something), rounded; kept is the thread's own memory
+__device__ __noinline__ void ti_keep(uint32_t O, float *kept, int cols, float f, bool more)
+{
+#pragma unroll 1
+    for (int ch = 0; ch < cols; ch += 16) {
+        uint32_t v[16];
+        ti_ld16(v, O + ch);
+        ti_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) kept[ch + k] = more ? fmaf(kept[ch + k], f, __uint_as_float(v[k])) : __uint_as_float(v[k]);
+    }
 }
 
 template <int HS, bool F32>
@@ -347,8 +361,21 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
             // rounding them, some 2^-25 of the sum an instruction, always towards zero.
             // So O holds one tile of tokens and is then added, rounded, to R.  (2.1e-6 off
             // after 1200 tokens with one accumulator throughout, 5e-7 with R.)
+            // 16-bit rows lost 8.4e-4 over 131072 tokens of one sign: TI_FOLD tiles are added
+            // at a time (3e-5), to the thread's own memory, as TMEM is full at heads of 128.
+            float store[F32 ? 1 : HS], km = -INFINITY;   // km: the maximum they are relative to
+            float *kept = store;
+            asm volatile("" : "+l"(kept));
             const size_t to = (size_t)(run.first + tok) * a.out.ld + (size_t)head * HS;
             for (int j = 0; j < n[i]; j++) {
+                if (!F32 && j > 0 && j % TI_FOLD == 0) {
+                    ok = ti_wait(&bar[B_O + i], o_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    ti_keep(O, kept, HS, km == -INFINITY ? 0.f : kv_exp2(km - m), j > TI_FOLD);
+                    km = m;
+                }
                 if (F32 && j > 0) {   // while the products for S run
                     ok = ti_wait(&bar[B_O + i], o_it[i]++, abort_s, a.c.err, CATS_DEVERR_ATTN_WAIT);
                     ok = __all_sync(0xffffffffu, ok);
@@ -389,7 +416,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                         sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
                         if (far) m = mn;
                         // (the products so far are complete: S came after them)
-                        ti_rescale<F32>(F32 ? R : O, j > 0 ? HS : 0, S, ch, al);
+                        ti_rescale<F32>(F32 ? R : O, (F32 ? j > 0 : j % TI_FOLD > 0) ? HS : 0, S, ch, al);
                     }
                     const float ref = m == -INFINITY ? 0.f : TI_P_BITS - m;
 #pragma unroll
@@ -421,6 +448,7 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 if (F32) ti_fold(O, R, HS, n[i] > 1);
             }
             const float inv = !ok || *abort_s ? NAN : l == 0.f ? 0.f : 1.f / l;
+            const float kf2 = km == -INFINITY ? 0.f : kv_exp2(km - m);
 #pragma unroll 1
             for (int ch = 0; ch < HS; ch += 32) {
                 uint32_t v[32];
@@ -429,6 +457,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                 if (n[i] > 0) {
                     ti_ld32(v, (F32 ? R : O) + ch);
                     ti_wait_ld();
+                    if (!F32 && n[i] > TI_FOLD) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) v[k] = __float_as_uint(fmaf(kept[ch + k], kf2, __uint_as_float(v[k])));
+                    }
                 }
                 if (real) {
                     bool nan = false;   // this block of 32 has one that the row sees
@@ -632,10 +664,10 @@ __global__ void __launch_bounds__(TI_THREADS, 1) k_kv_attn_tile(const __grid_con
                         for (int k = 0; k < TI_KV / 16; k++) {
                             const uint64_t vk = vs + ((k >> 2) * L::V_PAGE + (k & 3) * 32) / 16;
                             const uint32_t o = tmem + O_AT + O_STEP * i, p = tmem + 128 * i + (F32 ? 32 * (k >> 1) + 8 * (k & 1) : 8 * k);
-                            ti_mma_ts(o, p, vk, id_pv, (!F32 && j > 0) || k > 0);
+                            ti_mma_ts(o, p, vk, id_pv, (!F32 && j % TI_FOLD > 0) || k > 0);
                             if (F32) ti_mma_ts(o, p + 16, vk, id_pv, 1);
                         }
-                        if (F32 || j + 1 == n[i]) ti_commit(&bar[B_O + i]);
+                        if (F32 || j + 1 == n[i] || (j + 1) % TI_FOLD == 0) ti_commit(&bar[B_O + i]);
                     }
                     __syncwarp();
                     if (j + 1 < n[i]) qk(i, it + 1);

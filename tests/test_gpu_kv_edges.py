@@ -167,13 +167,16 @@ def test_many_runs_beside_a_long_one(dtype, hs, n_runs, long):
 @pytest.mark.parametrize("hs", [32, 64, 96, 128])
 @pytest.mark.parametrize("rows,mul,hint", [(1, 4, (1, 1)), (8, 4, (8, 1)), (1, 4, (1, LONG)), (60, 4, (60, 140000))])
 def test_long_sums_of_fp16_rows_are_not_cut_off(hs, rows, mul, hint):
+    long_fp16_sums(hs, rows, mul, hint, 131072)
+
+
+def long_fp16_sums(hs, rows, mul, hint, n):
     """The same for fp16 rows, where the outputs' roundings hide single sums but
     not their mean: an output is off by 2^-11 / sqrt(12) of itself rms at most
     (its rounding), 1.4e-4, so the mean of 4 hs outputs by 1.4e-4 / sqrt(4 hs);
     six of those.  What the sums are cut off by goes one way: accumulators hold
     the products of 4096 tokens at most before they are added, rounded, to the
     rest; 256 products of 2^-23 lose 2^-16 on average over them as they grow."""
-    n = 131072
     c = make([n], 1, hs, layers=1)
     g = torch.Generator(device="cuda").manual_seed(1)
     k, v = torch.randn(n, 1, hs, generator=g, device="cuda"), torch.rand(n, 1, hs, generator=g, device="cuda") + 0.5
@@ -191,3 +194,10 @@ def test_long_sums_of_fp16_rows_are_not_cut_off(hs, rows, mul, hint):
         off.append(out[:, h].double() / (p @ v) - 1)
     off = torch.stack(off).mean()
     assert off.abs() <= 6 * 1.4e-4 / math.sqrt(4 * hs) + 2**-16, off
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+@pytest.mark.parametrize("n", [16384, 131072, 4096, 4097, 8192 + 77])
+def test_long_sums_of_fp16_prompts_are_not_cut_off(hs, n):
+    """The same for prompts, at lengths around the ends of what one accumulator takes."""
+    long_fp16_sums(hs, 300, 16, (300, n), n)
