@@ -816,7 +816,9 @@ int cats_gpu_llm_batch_reserve(cats_gpu_llm *h, int max_tokens, int n_seqs)
 {
     const char *what = "cats_gpu_llm_batch_reserve";
     if (!h || max_tokens <= 0 || n_seqs <= 0) return fail(CATS_ERR_ARG, what);
+    const int cap = h->m.bt_cap;
     int rc = llm_batch_reserve(&h->m, max_tokens, n_seqs);
+    if (h->m.bt_cap != cap) h->bt_T = 0;   // the set batch went with its buffers
     return rc ? fail(rc, what) : CATS_OK;
 }
 

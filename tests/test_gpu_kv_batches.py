@@ -138,3 +138,24 @@ def test_what_a_refused_generation_reports(llm, orc, paged):
     lib.cats_gpu_clear_error()
     assert run(3) == 0
     m.close()
+
+
+@pytest.mark.parametrize("paged", [True, False])
+def test_a_set_batch_goes_with_the_buffers_it_was_set_in(llm, orc, paged):
+    """Larger buffers hold no batch yet; those that stay keep theirs."""
+    m, toks = start(llm, orc)
+    if not paged:
+        m.cache_q4(0)
+    m.batch_set(toks[:2], [0, 1], [0, 0])
+    m.batch_reserve(64, 1)                            # not larger than what there is
+    m.batch_enqueue()
+    m.synchronize()
+    m.batch_set(toks[:1], [0], [0])
+    m.batch_reserve(300, 1)
+    for call in (m.batch_enqueue, lambda: m.batch_enqueue_decode(1)):
+        with pytest.raises(RuntimeError):
+            call()
+    m.batch_set(toks[:1], [0], [0])
+    m.batch_enqueue_decode(2)
+    m.synchronize()
+    m.close()
