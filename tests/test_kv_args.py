@@ -36,3 +36,22 @@ def test_tensors_that_want_a_gradient():
     with torch.no_grad():
         assert kv._rows(x, 1, 32, cpu, "k") == 32
     assert kv._rows(x.detach(), 1, 32, cpu, "k") == 32
+
+
+@pytest.mark.parametrize("tp", [1, 2])
+def test_rows_of_a_rank_hold_its_own_heads(tp):
+    """cache_read of a tensor-parallel rank: the arrays it hands over are its kv heads' wide."""
+    from catseye_b200 import llm
+
+    class Lib:
+        def cats_gpu_llm_cache_read(self, h, layer, seq, n, k, v):
+            for i, p in enumerate((k, v)):
+                C.memset(p.value, i + 1, n * 128 // tp * 4)
+            return 0
+
+    m = llm.GpuLLM.__new__(llm.GpuLLM)
+    m.lib, m.h, m._tp_size = Lib(), None, tp
+    m.cfg = llm.LlmConfig(dim=256, hidden=256, n_layers=1, n_heads=8, n_kv_heads=4, vocab=512, seq_len=64, wtype=2)
+    k, v = m.cache_read(0, 0, 5)
+    assert k.shape == v.shape == (5, 128 // tp)
+    assert (k.view(np.uint8) == 1).all() and (v.view(np.uint8) == 2).all()
