@@ -18,7 +18,8 @@ namespace cats {
 // by issue: 15 instructions an element appended, 9 read back (36 and 20 with a
 // page and 64-bit offsets for every pair, and 16-bit values quantized in fp32).
 // 4096 bf16 rows of 32 heads of 128: appended in 24 us, read back in 18 (86 MB
-// each: 3.6 and 4.7 TB/s); 16 rows of 8 heads 5 us, which is the launch.
+// each: 3.6 and 4.7 TB/s), fp32 rows 85 us for both (306 MB, 3.6 TB/s); 16 rows of
+// 8 heads 5 us, which is the launch.
 constexpr int KV_EIGHT = 8;   // tokens of a thread's turn
 
 // eight elements of a row, as they lie (TYPE 16 bits) or as floats
@@ -295,7 +296,8 @@ cudaError_t launch_kv_attention(const KvView &c, int type, const KvRows &out, co
     // for calls with 3200 query rows and more for each wave of its CTAs.
     // Measured, tile / split, heads of 128: 16 runs of 4 rows x 64 heads after 1000
     // tokens 35 / 55 us (fp16), 55 / 61 us (fp32); 64 rows of 32 heads after 8000
-    // tokens 164 / 84 us, 238 / 111 us; fp32, 2048 rows of 32 heads 203 / 1335 us.
+    // tokens 164 / 84 us, 238 / 111 us; fp32, 2048 rows of 32 heads 181 / 1335 us.
+    // (The tile kernel takes heads of 64 and 128 only: kv_attn_tile_takes.)
     const long long q_run = (long long)std::max(b.max_rows, 1) * a.mul;
     const long long rows = std::min((long long)b.n_runs * std::max(b.max_rows, 1), (long long)q.rows);
     const int per = kv_attn_tile_rows(a);

@@ -1,5 +1,5 @@
 // kv.cuh — the paged KV cache held in Q4_0 blocks: its layout, the block
-// quantizer, and the launchers that the C API (kv.cu) and the batched step
+// quantizer, and the launchers that the C API (kv_capi.cu) and the batched step
 // (batch.cu) share.
 //
 // A page holds CATS_KV_PAGE = 64 tokens of every layer and kv head:

@@ -823,9 +823,11 @@ cudaError_t launch_kv_attn_split(const KvAttn &a0, int max_rows, int max_len, cu
     KvAttn a = a0;
     const bool split = a.type == KV_F32;
     const long long q = (long long)std::max(max_rows, 1) * a.mul;
-    // One tile of columns while the query rows fit it: 64 sequences of 4000 tokens,
-    // 8 kv heads, fp16, 8 rows each 94 us with one tile and 139 with two; 16 rows each
-    // 157 and 145.
+    // One tile of columns while the query rows fit it, else two: 64 sequences of 3900
+    // tokens, 8 kv heads, fp16: 8 rows each 88 us with one (139 with two), 9, 12 and 16
+    // rows 144, 146 and 148 us with two and 153, 155 and 157 with one; fp32: 4 rows 88 us,
+    // 5 and 8 rows 115 us with two and 155 and 158 with one.  (Two tiles of 16-bit rows
+    // with heads of 128 spill, some 500 bytes a thread.)
     const int nt = q <= sp_rows(split, 1) ? 1 : 2, rows = sp_rows(split, nt), slots = 148 * sp_resident(nt);
     a.tiles = (int)std::min<long long>((q + rows - 1) / rows, 1 << 16);
     // (a CTA goes through a run's further tiles itself: the grid of a batch of many

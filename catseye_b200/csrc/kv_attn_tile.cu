@@ -23,10 +23,10 @@
 // Bound by a tile's chain: 128 tokens take a row's thread some 2900 cycles (its
 // exponentials alone 1024, sixteen a cycle and SM) and then the products 1000,
 // which the other tile's rows hide only in part.  4096 rows of 32 heads of 128
-// (bf16, causal): 219 us, 628 TFLOP/s (the variants against 225 then): 64 tokens at a time with S twice 260 us,
-// two threads a row 313 us, eight dequantizing warps 249 us, S loaded a piece
-// ahead 250 us: all of them more code, and the roles share one instruction
-// cache.  The accumulator is not rescaled for every new maximum: m is only moved
+// (bf16, causal): 219 us, 628 TFLOP/s.  When it took 225: 64 tokens at a time
+// with S twice 260 us, two threads a row 313 us, eight dequantizing warps 249 us,
+// S loaded a piece ahead 250 us: all of them more code, and the roles share one
+// instruction cache.  The accumulator is not rescaled for every new maximum: m is only moved
 // when a row's maximum passes it by 2^8, which happens once or twice a row.
 //
 // Every wait is bounded; TMEM is freed on every path.
@@ -707,6 +707,9 @@ template <int HS, bool F32> static cudaError_t launch_tile(const KvAttn &a, dim3
 
 int kv_attn_tile_rows(const KvAttn &a) { return 128 * ti_q_tiles(a.c.hs, a.type == KV_F32); }
 
+// Heads of 32 and 96 stay with the split kernel whatever the work: the operands'
+// slices are 64 elements wide here.  4096 causal rows of 32 heads, bf16: heads of 64 171 us and
+// of 128 220 us here, of 32 1259 us and of 96 2662 us there.
 bool kv_attn_tile_takes(const KvAttn &a) { return (a.c.hs == 64 || a.c.hs == 128) && a.n_runs <= 65535; }
 
 cudaError_t launch_kv_attn_tile(const KvAttn &a0, int max_rows, cudaStream_t st)

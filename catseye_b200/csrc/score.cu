@@ -7,23 +7,23 @@
 // its own maximum; the threads' triples are joined at the end.
 //
 // The row is read once, a chunk of 4096 elements in the CTA's registers at a
-// time and the next one on its way.  The k <= 32 largest cost no second read: the k-th largest of the 256
-// threads' maxima of the first chunk is a bound that at least k elements reach
-// and few others; what reaches it, there and in the later chunks, goes to a
+// time and the next one on its way.  The k <= 32 largest mostly cost no second
+// read: the k-th largest of the 256 threads' maxima of the first chunk is a
+// bound that at least k elements reach and, in a row of one make, few others; what reaches it, there and in the later chunks, goes to a
 // list in shared memory that is ranked by counting at the end, and for a closer
 // bound after 4, 16, 64 chunks (after 2, 4, 8 too: 85 us for 72).  (Equal values by the
-// thousand, or a rising row, overflow the list: then the row's chunks are gone
-// through again, the bound renewed for each, and as a last resort a chunk's k
-// largest taken one by one.)
+// thousand, or a row that rises behind its first chunk, overflow the list: then the
+// row's chunks are read again, which doubles the time (1500 such rows 149 us), the
+// bound renewed for each, and as a last resort a chunk's k largest taken one by
+// one.)
 //
 // A logit of -inf is no candidate: rows that are mostly masked have short lists
 // (1500 rows of 32000 with 40 tokens left, k = 32: 77 us, 69 without a mask), and
 // where fewer than k are left the lowest other ids follow them.
 //
-// Bound by issue (72% of the slots; some 27 instructions an element, of which
-// the exponential and the sums are 6, maxima and candidates most of the rest):
-// 2048 fp32 rows of 32000 with the 20 likeliest 72 us, 3.65 TB/s, 56% of a copy's
-// rate.
+// Bound by issue (72% of the slots; some 27 instructions an element): 2048 fp32
+// rows of 32000 with the 20 likeliest 72 us, 3.65 TB/s, 56% of a copy's rate, of
+// which the pass without candidates (k = 0) is 52; bf16 rows 72 and 39 us.
 //
 // Few rows: a cluster of up to 8 CTAs shares a row's chunks and joins through
 // distributed shared memory.
