@@ -57,6 +57,7 @@ int llm_cache_q4(LlmModel *m, int n_pages, int n_seqs)
         p = new LlmPaged(n_pages, n_seqs, max_pages);
         p->sent.assign((size_t)n_seqs * max_pages, -1);
     } catch (const std::bad_alloc &) {
+        delete p;
         return E_NOMEM;
     }
     p->page_bytes = page_bytes;
