@@ -301,8 +301,10 @@ int cats_gpu_llm_score_batch(cats_gpu_llm *m, const int *tokens, const int *pos,
  * 0 goes back to the dense cache.  head_size must be a multiple of 32 up to
  * 128 (else CATS_ERR_UNSUPPORTED).  A step's positions may rewrite a sequence
  * or extend it, without a gap and each once (else CATS_ERR_ARG); too few free
- * pages: CATS_ERR_NOMEM, the cache as it was.  Queries and attention output
- * are fp16.  The single-token engines keep their own dense cache:
+ * pages: CATS_ERR_NOMEM, the cache as it was.  Positions count (_cache_length)
+ * once the step that writes them is enqueued; the pages of a batch that was
+ * set and never ran are free again when the next one is set.  Queries and
+ * attention output are fp16.  The single-token engines keep their own dense cache:
  * _cache_to_dense copies a sequence's first n tokens into it.
  * _cache_fork: dst becomes the first len tokens of src, sharing its pages;
  * pages are copied when one of their sequences writes.  _cache_truncate: keep
@@ -392,7 +394,8 @@ int cats_gpu_kv_read_dev(const cats_gpu_kv *c, int layer, void *k, void *v, int 
  * a kv head (llm/catseye_llm.h:1677-1723).  A row at a negative position sees
  * nothing and gets zeros.  Sums and softmax statistics are fp32; fp32 rows
  * enter the tensor cores as two fp16 halves each of q and of the
- * probabilities, other types as one.  out and q share no memory (the same
+ * probabilities, other types as one; what an accumulator takes is bounded, so
+ * that the sums' error does not grow with the length.  out and q share no memory (the same
  * pointer: CATS_ERR_ARG). */
 int cats_gpu_kv_attention_dev(const cats_gpu_kv *c, int layer, void *out, const void *q, int type, int n_heads,
                               long long ld_out, long long ld_q, int rows, const int *runs, int n_runs, int max_rows,
