@@ -58,6 +58,13 @@ def _ints(x):
     return a.ctypes.data, a.size, a
 
 
+def _int32(*values):
+    """Refuse what C's int would wrap."""
+    for x in values:
+        if not -2**31 <= x < 2**31:
+            raise OverflowError(f"{x} does not fit 32 bits")
+
+
 def _rows(t, heads, hs, device, what):
     """Row stride of a tensor [rows][heads][hs] whose rows are whole."""
     shape = t.shape
@@ -170,6 +177,7 @@ class Pages:
     """Which page of a cache holds which tokens of which sequence (host only)."""
 
     def __init__(self, n_pages, n_seqs, max_pages):
+        _int32(n_pages, n_seqs, max_pages)
         self._lib = _lib.load()
         self._shape = (n_seqs, max_pages)
         self.n_pages = n_pages
@@ -185,16 +193,19 @@ class Pages:
 
     def write(self, seq, pos, n):
         """Make n positions from pos writable; returns the page copies (src, dst) to make first."""
+        _int32(seq, pos, n)
         return self._copies(max(n, 0) // PAGE + 2,
                             lambda s, d, c: self._lib.cats_gpu_kv_pages_write(self._h, seq, pos, n, s, d, c),
                             "kv_pages_write")
 
     def fork(self, src_seq, dst_seq, length):
         """dst_seq becomes the first `length` tokens of src_seq, sharing its pages."""
+        _int32(src_seq, dst_seq, length)
         _lib.check(self._lib.cats_gpu_kv_pages_fork(self._h, src_seq, dst_seq, length), "kv_pages_fork")
 
     def truncate(self, seq, length):
         """Keep the first `length` tokens of a sequence (0: free it)."""
+        _int32(seq, length)
         _lib.check(self._lib.cats_gpu_kv_pages_truncate(self._h, seq, length), "kv_pages_truncate")
 
     def compact(self):
@@ -203,6 +214,7 @@ class Pages:
                             "kv_pages_compact")
 
     def length(self, seq):
+        _int32(seq)
         return self._lib.cats_gpu_kv_pages_length(self._h, seq)
 
     @property

@@ -55,3 +55,16 @@ def test_rows_of_a_rank_hold_its_own_heads(tp):
     k, v = m.cache_read(0, 0, 5)
     assert k.shape == v.shape == (5, 128 // tp)
     assert (k.view(np.uint8) == 1).all() and (v.view(np.uint8) == 2).all()
+
+
+def test_page_bookkeeping_refuses_what_c_would_wrap():
+    p = kv.Pages(4, 2, 3)
+    p.write(0, 0, 70)
+    big = 2**32
+    for call in (lambda: p.write(0, big, 1), lambda: p.write(big, 70, 1), lambda: p.write(0, 70, big + 1),
+                 lambda: p.fork(0, big + 1, 10), lambda: p.fork(big, 1, 10), lambda: p.fork(0, 1, big + 10),
+                 lambda: p.truncate(0, big), lambda: p.truncate(big, 0), lambda: p.length(big),
+                 lambda: kv.Pages(big + 1, 1, 1)):
+        with pytest.raises(OverflowError):
+            call()
+    assert p.length(0) == 70 and p.length(1) == 0 and p.free == 2
