@@ -1,5 +1,6 @@
 """Attention over the paged Q4_0 cache where a call leaves the ordinary: rows
-behind the table, values that are NaN."""
+behind the table, values that are NaN, sums over very long sequences, very many
+runs."""
 import math
 
 import numpy as np
